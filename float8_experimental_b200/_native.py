@@ -50,6 +50,15 @@ EXPORTS = (
     "f8b200_rmsnorm_bwd",
     "f8b200_swiglu_bwd",
     "f8b200_swiglu_bwd_approx",
+    "f8b200_cast_blockwise",
+    "f8b200_uncast_blockwise",
+    "f8b200_gemm_blockwise",
+    "f8b200_layer_norm",
+    "f8b200_layer_norm_bwd_workspace_bytes",
+    "f8b200_layer_norm_bwd",
+    "f8b200_multi_norm_workspace_bytes",
+    "f8b200_multi_norm",
+    "f8b200_multi_clip",
     "f8b200_read_device_error",
     "f8b200_check_device_error",
 )
@@ -110,6 +119,20 @@ def load() -> ctypes.CDLL:
     lib.f8b200_gemm_fp8_scatter_rows.argtypes = [vp, i32, i32, i64, vp, i32, i32, i64, vp, vp, vp, i32, ctypes.POINTER(vp),
                                                  i32, i64, i64, i64, i64, i64, vp, i64, vp]
     lib.f8b200_sum_slots.argtypes = [vp, i32, i64, i32, i64, vp, vp]
+    lib.f8b200_cast_blockwise.argtypes = [vp, i32, i64, i64, i64, i32, i32, vp, i64, vp, i64, vp, i64, vp, i64, vp]
+    lib.f8b200_uncast_blockwise.argtypes = [vp, i32, i64, i64, i64, vp, i64, i64, i32, i32, i32, vp, i64, vp]
+    lib.f8b200_gemm_blockwise.argtypes = [vp, i32, i32, i64, vp, i64, i64, i32, vp, i32, i32, i64, vp, i64, i64, i32, vp, i32,
+                                          vp, i64, i64, i64, i64, vp]
+    lib.f8b200_layer_norm.argtypes = [vp, i32, i64, i64, i64, vp, vp, i32, ctypes.c_float, vp, i64, vp, vp, vp]
+    lib.f8b200_layer_norm_bwd_workspace_bytes.argtypes = [i64]
+    lib.f8b200_layer_norm_bwd_workspace_bytes.restype = i64
+    lib.f8b200_layer_norm_bwd.argtypes = [vp, vp, i32, i64, i64, i64, i64, vp, i32, vp, vp, vp, i64, vp, vp, vp, i64, vp]
+    lib.f8b200_multi_norm_workspace_bytes.argtypes = [ctypes.POINTER(i64), i32]
+    lib.f8b200_multi_norm_workspace_bytes.restype = i64
+    lib.f8b200_multi_norm.argtypes = [ctypes.POINTER(vp), ctypes.POINTER(i64), ctypes.POINTER(i32), i32, i32, i32, vp, vp,
+                                      i64, vp]
+    lib.f8b200_multi_clip.argtypes = [ctypes.POINTER(vp), ctypes.POINTER(i64), ctypes.POINTER(i32), i32, vp, ctypes.c_float,
+                                      vp]
     for name in EXPORTS:
         fn = getattr(lib, name)
         if fn.restype is not ctypes.c_char_p and fn.restype is not i64:
@@ -562,6 +585,104 @@ def swiglu_bwd(a: torch.Tensor, b: torch.Tensor, g: torch.Tensor, rows: int, col
             _check(load().f8b200_swiglu_bwd_approx(*args), "f8b200_swiglu_bwd_approx")
         else:
             _check(load().f8b200_swiglu_bwd(*args), "f8b200_swiglu_bwd")
+
+
+def cast_blockwise(x: torch.Tensor, rows: int, cols: int, ld_x: int, fp8_kind: int, by_square: bool,
+                   out_r: Optional[torch.Tensor], ld_r: int, scale_r: Optional[torch.Tensor], ld_scale_r: int,
+                   out_c: Optional[torch.Tensor], ld_c: int, scale_c: Optional[torch.Tensor], ld_scale_c: int) -> None:
+    _require_cuda(x, out_r, scale_r, out_c, scale_c)
+    with _Launch("cast_block", x.device):
+        _check(
+            load().f8b200_cast_blockwise(x.data_ptr(), hp_code(x.dtype), rows, cols, ld_x, fp8_kind, int(by_square),
+                                         _ptr(out_r), ld_r, _ptr(scale_r), ld_scale_r, _ptr(out_c), ld_c, _ptr(scale_c),
+                                         ld_scale_c, _stream(x)),
+            "f8b200_cast_blockwise",
+        )
+
+
+def uncast_blockwise(q: torch.Tensor, rows: int, cols: int, ld_q: int, scale: torch.Tensor, block_rows: int,
+                     block_cols: int, y: torch.Tensor, ld_y: int) -> None:
+    _require_cuda(q, scale, y)
+    with _Launch("uncast_block", q.device):
+        _check(
+            load().f8b200_uncast_blockwise(q.data_ptr(), fp8_code(q.dtype), rows, cols, ld_q, scale.data_ptr(),
+                                           scale.stride(0), scale.stride(1), block_rows, block_cols, hp_code(y.dtype),
+                                           y.data_ptr(), ld_y, _stream(q)),
+            "f8b200_uncast_blockwise",
+        )
+
+
+def gemm_blockwise(a: torch.Tensor, lda: int, a_mn_major: bool, scale_a: torch.Tensor, a_block_rows: int,
+                   b: torch.Tensor, ldb: int, b_mn_major: bool, scale_b: torch.Tensor, b_block_rows: int,
+                   bias: Optional[torch.Tensor], out: torch.Tensor, ldo: int, m: int, n: int, k: int) -> None:
+    _require_cuda(a, b, scale_a, scale_b, bias, out)
+    with _Launch("gemm_block", a.device):
+        _check(
+            load().f8b200_gemm_blockwise(a.data_ptr(), fp8_code(a.dtype), int(a_mn_major), lda, scale_a.data_ptr(),
+                                         scale_a.stride(0), scale_a.stride(1), a_block_rows, b.data_ptr(),
+                                         fp8_code(b.dtype), int(b_mn_major), ldb, scale_b.data_ptr(), scale_b.stride(0),
+                                         scale_b.stride(1), b_block_rows, _ptr(bias), hp_code(out.dtype), out.data_ptr(),
+                                         ldo, m, n, k, _stream(a)),
+            "f8b200_gemm_blockwise",
+        )
+
+
+def layer_norm(x: torch.Tensor, rows: int, cols: int, ld_x: int, weight: Optional[torch.Tensor],
+               bias: Optional[torch.Tensor], affine_dtype: torch.dtype, eps: float, y: torch.Tensor,
+               mean: Optional[torch.Tensor], rstd: Optional[torch.Tensor]) -> None:
+    _require_cuda(x, weight, bias, y, mean, rstd)
+    with _Launch("layer_norm", x.device):
+        _check(
+            load().f8b200_layer_norm(x.data_ptr(), hp_code(x.dtype), rows, cols, ld_x, _ptr(weight), _ptr(bias),
+                                     hp_code(affine_dtype), float(eps), y.data_ptr(), cols, _ptr(mean), _ptr(rstd),
+                                     _stream(x)),
+            "f8b200_layer_norm",
+        )
+
+
+def layer_norm_bwd(x: torch.Tensor, g: torch.Tensor, rows: int, cols: int, ld_x: int, ld_g: int,
+                   weight: Optional[torch.Tensor], affine_dtype: torch.dtype, mean: torch.Tensor, rstd: torch.Tensor,
+                   dx: Optional[torch.Tensor], dw: Optional[torch.Tensor], db: Optional[torch.Tensor]) -> None:
+    _require_cuda(x, g, weight, mean, rstd, dx, dw, db)
+    nbytes = int(load().f8b200_layer_norm_bwd_workspace_bytes(cols)) if dw is not None or db is not None else 0
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    with _Launch("layer_norm_bwd", x.device, (1 if dx is not None else 0) + (2 if nbytes else 0)):
+        _check(
+            load().f8b200_layer_norm_bwd(x.data_ptr(), g.data_ptr(), hp_code(x.dtype), rows, cols, ld_x, ld_g,
+                                         _ptr(weight), hp_code(affine_dtype), mean.data_ptr(), rstd.data_ptr(), _ptr(dx),
+                                         cols, _ptr(dw), _ptr(db), _ptr(ws), nbytes, _stream(x)),
+            "f8b200_layer_norm_bwd",
+        )
+
+
+def _tensor_arrays(xs: Sequence[torch.Tensor]):
+    n = len(xs)
+    return ((ctypes.c_void_p * n)(*[t.data_ptr() for t in xs]), (ctypes.c_int64 * n)(*[t.numel() for t in xs]),
+            (ctypes.c_int * n)(*[hp_code(t.dtype) for t in xs]))
+
+
+MULTI_TENSORS_PER_LAUNCH = 1024  # tensors whose addresses fit one launch's parameters (csrc/grad_clip.cu)
+
+
+def multi_norm(xs: Sequence[torch.Tensor], kind: int, root: bool, out: torch.Tensor) -> None:
+    """`f8b200_multi_norm` over dense tensors of one device, each taken as its storage lies."""
+    n = len(xs)
+    _require_cuda(out, *xs)
+    ptrs, numels, codes = _tensor_arrays(xs)
+    nbytes = int(load().f8b200_multi_norm_workspace_bytes(numels, n))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=out.device) if nbytes else None
+    with _Launch("multi_norm", out.device, 1 + -(-n // MULTI_TENSORS_PER_LAUNCH)):
+        _check(load().f8b200_multi_norm(ptrs, numels, codes, n, kind, int(root), out.data_ptr(), _ptr(ws), nbytes,
+                                        _stream(out)), "f8b200_multi_norm")
+
+
+def multi_clip(xs: Sequence[torch.Tensor], total_norm: torch.Tensor, max_norm: float) -> None:
+    n = len(xs)
+    _require_cuda(total_norm, *xs)
+    ptrs, numels, codes = _tensor_arrays(xs)
+    with _Launch("multi_clip", total_norm.device, -(-n // MULTI_TENSORS_PER_LAUNCH)):
+        _check(load().f8b200_multi_clip(ptrs, numels, codes, n, total_norm.data_ptr(), float(max_norm),
+                                        _stream(total_norm)), "f8b200_multi_clip")
 
 
 def check_device_error() -> None:

@@ -20,10 +20,18 @@ Ops (namespace `f8b200`):
   rmsnorm_cast(x, weight, rstd, amax, kind) -> (data, scale)               f8b200_rmsnorm_cast
   swiglu_amax(a, b, write_y, approx) -> (amax fp32 0-dim, y or empty)      f8b200_swiglu_amax[_approx]
   swiglu_cast(a, b, amax, kind) -> (data, scale)                           f8b200_swiglu_cast
+  cast_blockwise(x, kind, by_row, by_col) -> (data, scale_inv, data_c, scale_inv_c)   f8b200_cast_blockwise
+  cast_blockwise_square(x, kind) -> (data, scale_inv)                      f8b200_cast_blockwise, 128 x 128 blocks
+  uncast_blockwise(q, scale_inv, block_rows, block_cols, dtype) -> y       f8b200_uncast_blockwise
+  blockwise_mm(a, b_t, scale_a, scale_b, a_block_rows, b_block_rows, bias, out_dtype) -> out   f8b200_gemm_blockwise
+  layer_norm(x, weight, bias, eps, save_stats) -> (y, mean, rstd)          f8b200_layer_norm
+  layer_norm_bwd(x, grad_y, weight, mean, rstd, affine_dtype, need_dx, need_dw, need_db) -> (dx, dw, db)
+  multi_norm(xs, kind, root) -> fp32 0-dim                                 f8b200_multi_norm
+  multi_clip_(xs!, total_norm, max_norm)                                   f8b200_multi_clip
 """
 from __future__ import annotations
 
-from typing import List, Tuple
+from typing import List, Optional, Tuple
 
 import torch
 
@@ -56,6 +64,22 @@ _lib.define("swiglu_amax(Tensor a, Tensor b, bool write_y, bool approx=False) ->
 _lib.define("rmsnorm_bwd(Tensor x, Tensor grad_y, Tensor weight, Tensor rstd) -> (Tensor, Tensor)")
 _lib.define("swiglu_bwd(Tensor a, Tensor b, Tensor grad_y, bool approx=False) -> (Tensor, Tensor)")
 _lib.define("swiglu_cast(Tensor a, Tensor b, Tensor amax, int fp8_kind) -> (Tensor, Tensor)")
+_lib.define("cast_blockwise(Tensor x, int fp8_kind, bool by_row, bool by_col) -> (Tensor, Tensor, Tensor, Tensor)")
+_lib.define("cast_blockwise_square(Tensor x, int fp8_kind) -> (Tensor, Tensor)")
+_lib.define("uncast_blockwise(Tensor q, Tensor scale_inv, int block_rows, int block_cols, ScalarType dtype) -> Tensor")
+_lib.define(
+    "blockwise_mm(Tensor a, Tensor b_t, Tensor scale_a, Tensor scale_b, int a_block_rows, int b_block_rows, "
+    "Tensor? bias, ScalarType out_dtype) -> Tensor"
+)
+_lib.define(
+    "layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps, bool save_stats) -> (Tensor, Tensor, Tensor)"
+)
+_lib.define(
+    "layer_norm_bwd(Tensor x, Tensor grad_y, Tensor? weight, Tensor mean, Tensor rstd, ScalarType affine_dtype, "
+    "bool need_dx, bool need_dw, bool need_db) -> (Tensor, Tensor, Tensor)"
+)
+_lib.define("multi_norm(Tensor[] xs, int kind, bool root) -> Tensor")
+_lib.define("multi_clip_(Tensor(a!)[] xs, Tensor total_norm, float max_norm) -> ()")
 
 
 def _as_matrix(x: torch.Tensor) -> Tuple[torch.Tensor, int, int, int]:
@@ -266,6 +290,169 @@ def _swiglu_bwd_cuda(a, b, grad_y, approx: bool = False):
     return da, db
 
 
+def _one_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) > 1:
+        raise RuntimeError(f"{what}: tensors on different devices ({', '.join(sorted(map(str, devices)))})")
+
+
+def _blocks(size: int) -> int:
+    return -(-size // 128)
+
+
+def _empty_fp8_matrix(rows: int, cols: int, fp8_kind: int, device) -> torch.Tensor:
+    """[rows, cols] fp8 whose rows start on 16-byte boundaries, so that the GEMM reads it where it lies."""
+    return torch.empty((rows, _pitch16(cols)), dtype=N.FP8_DTYPE[fp8_kind], device=device)[:, :cols]
+
+
+def _cast_blockwise_cuda(x, fp8_kind: int, by_row: bool, by_col: bool):
+    if x.dim() != 2 or not (by_row or by_col):
+        raise RuntimeError("cast_blockwise: takes a matrix and at least one of by_row, by_col")
+    xm, _, _, ld = _as_matrix(x)
+    rows, cols = x.shape
+    none8 = torch.empty((0, 0), dtype=N.FP8_DTYPE[fp8_kind], device=x.device)
+    none32 = torch.empty((0, 0), dtype=torch.float32, device=x.device)
+    data = _empty_fp8_matrix(rows, cols, fp8_kind, x.device) if by_row else none8
+    data_c = _empty_fp8_matrix(rows, cols, fp8_kind, x.device) if by_col else none8
+    # one factor per (block, row) resp. (block, column): the GEMM's lanes read neighbouring rows
+    scale = torch.empty((_blocks(cols), rows), dtype=torch.float32, device=x.device) if by_row else none32
+    scale_c = torch.empty((_blocks(rows), cols), dtype=torch.float32, device=x.device) if by_col else none32
+    if x.numel():
+        N.cast_blockwise(xm, rows, cols, ld, fp8_kind, False, data if by_row else None, data.stride(0),
+                         scale if by_row else None, rows, data_c if by_col else None, data_c.stride(0),
+                         scale_c if by_col else None, cols)
+    return data, scale.t(), data_c, scale_c
+
+
+def _cast_blockwise_square_cuda(x, fp8_kind: int):
+    if x.dim() != 2:
+        raise RuntimeError("cast_blockwise_square: takes a matrix")
+    xm, _, _, ld = _as_matrix(x)
+    rows, cols = x.shape
+    data = _empty_fp8_matrix(rows, cols, fp8_kind, x.device)
+    scale = torch.empty((_blocks(rows), _blocks(cols)), dtype=torch.float32, device=x.device)
+    if x.numel():
+        N.cast_blockwise(xm, rows, cols, ld, fp8_kind, True, data, data.stride(0), scale, scale.shape[1], None, 0, None, 0)
+    return data, scale
+
+
+def _uncast_blockwise_cuda(q, scale_inv, block_rows: int, block_cols: int, dtype):
+    _one_device("uncast_blockwise", q, scale_inv)
+    rows, cols = q.shape
+    if rows != 1 and cols != 1 and q.stride(0) == 1:  # a transposed matrix: read it as it lies
+        return _uncast_blockwise_cuda(q.t(), scale_inv.t(), block_cols, block_rows, dtype).t()
+    if q.stride(1) != 1 or q.stride(0) < cols:
+        q = q.contiguous()
+    y = torch.empty((rows, cols), dtype=dtype, device=q.device)
+    if q.numel():
+        N.uncast_blockwise(q, rows, cols, max(q.stride(0), cols), scale_inv, block_rows, block_cols, y, cols)
+    return y
+
+
+def _blockwise_mm_cuda(a, b_t, scale_a, scale_b, a_block_rows: int, b_block_rows: int, bias, out_dtype):
+    _one_device("blockwise_mm", a, b_t, scale_a, scale_b, bias)
+    m, k = a.shape
+    n, k2 = b_t.shape
+    if k != k2:
+        raise RuntimeError(f"blockwise_mm: inner dimensions differ ({k} vs {k2})")
+    for name, s, rows, block in (("scale_a", scale_a, m, a_block_rows), ("scale_b", scale_b, n, b_block_rows)):
+        want = (_blocks(rows) if block == 128 else rows, _blocks(k))
+        if s.dtype != torch.float32 or tuple(s.shape) != want:
+            raise RuntimeError(f"blockwise_mm: {name} must be float32 {want}, got {s.dtype} {tuple(s.shape)}")
+    if bias is not None and tuple(bias.shape) != (n,):
+        raise RuntimeError(f"blockwise_mm: the bias must have {n} elements, got {tuple(bias.shape)}")
+    if bias is not None:
+        bias = bias.to(out_dtype).contiguous()
+    out = torch.empty((m, n), dtype=out_dtype, device=a.device)
+    if m == 0 or n == 0:
+        return out
+    if k == 0:
+        return out.zero_() if bias is None else out.copy_(bias)
+    a, lda, a_mn = _gemm_operand(a)
+    b_t, ldb, b_mn = _gemm_operand(b_t)
+    N.gemm_blockwise(a, lda, a_mn, scale_a, a_block_rows, b_t, ldb, b_mn, scale_b, b_block_rows, bias, out, n, m, n, k)
+    return out
+
+
+def _affine_dtype(x, weight, bias) -> torch.dtype:
+    """The type of the norm's weight and bias: x's or fp32, the same for both."""
+    cols = x.shape[-1]
+    kinds = {t.dtype for t in (weight, bias) if t is not None}
+    if len(kinds) > 1 or not kinds <= {x.dtype, torch.float32}:
+        raise RuntimeError(f"layer_norm: weight and bias must both have x's dtype {x.dtype} or both float32")
+    if any(tuple(t.shape) != (cols,) for t in (weight, bias) if t is not None):
+        raise RuntimeError(f"layer_norm: weight and bias must have one element per column ({cols})")
+    return kinds.pop() if kinds else x.dtype
+
+
+def _layer_norm_cuda(x, weight, bias, eps: float, save_stats: bool):
+    _one_device("layer_norm", x, weight, bias)
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise RuntimeError("layer_norm: the last dimension must have at least one element")
+    affine = _affine_dtype(x, weight, bias)
+    xm, rows, cols, ld = _as_matrix(x)
+    y = _empty_like_shape(x, x.dtype)
+    stats = torch.empty((2, rows if save_stats else 0), dtype=torch.float32, device=x.device)
+    if rows:
+        N.layer_norm(xm, rows, cols, ld, None if weight is None else weight.contiguous(),
+                     None if bias is None else bias.contiguous(), affine, eps, y,
+                     stats[0] if save_stats else None, stats[1] if save_stats else None)
+    return y, stats[0], stats[1]
+
+
+def _layer_norm_bwd_cuda(x, grad_y, weight, mean, rstd, affine_dtype, need_dx: bool, need_dw: bool, need_db: bool):
+    _one_device("layer_norm_bwd", x, grad_y, weight, mean, rstd)
+    xm, rows, cols, ld = _as_matrix(x)
+    gm, _, _, ldg = _as_matrix(grad_y)
+    dx = _empty_like_shape(x, x.dtype) if need_dx else x.new_empty((0,))
+    # no rows: nothing to sum
+    new = torch.empty if rows else torch.zeros
+    dw = new((cols if need_dw else 0,), dtype=affine_dtype, device=x.device)
+    db = new((cols if need_db else 0,), dtype=affine_dtype, device=x.device)
+    if rows and (need_dx or need_dw or need_db):
+        N.layer_norm_bwd(xm, gm, rows, cols, ld, ldg, None if weight is None else weight.contiguous(), affine_dtype,
+                         mean, rstd, dx if need_dx else None, dw if need_dw else None, db if need_db else None)
+    return dx, dw, db
+
+
+def _check_dense(what: str, xs: List[torch.Tensor]) -> None:
+    """The kernels walk a tensor's storage: its elements must fill a range of it, each once, in any order."""
+    for t in xs:
+        if t.is_contiguous():
+            continue
+        step = 1
+        for size, stride in sorted(zip(t.shape, t.stride()), key=lambda d: d[1]):
+            if size == 1:
+                continue
+            if stride != step:
+                raise RuntimeError(f"{what}: a tensor of shape {tuple(t.shape)} and strides {t.stride()} is not dense")
+            step *= size
+
+
+def _multi_norm_cuda(xs: List[torch.Tensor], kind: int, root: bool):
+    _one_device("multi_norm", *xs)
+    _check_dense("multi_norm", xs)
+    out = torch.empty((), dtype=torch.float32, device=xs[0].device if xs else torch.device("cuda"))
+    N.multi_norm(xs, kind, root, out)
+    return out
+
+
+def _multi_clip_cuda(xs: List[torch.Tensor], total_norm, max_norm: float) -> None:
+    _one_device("multi_clip_", total_norm, *xs)
+    _check_dense("multi_clip_", xs)
+    if total_norm.numel() != 1 or total_norm.dtype != torch.float32:
+        raise RuntimeError("multi_clip_: total_norm must be one float32 value")
+    N.multi_clip(xs, total_norm, max_norm)
+
+
+_lib.impl("cast_blockwise", _cast_blockwise_cuda, "CUDA")
+_lib.impl("cast_blockwise_square", _cast_blockwise_square_cuda, "CUDA")
+_lib.impl("uncast_blockwise", _uncast_blockwise_cuda, "CUDA")
+_lib.impl("blockwise_mm", _blockwise_mm_cuda, "CUDA")
+_lib.impl("layer_norm", _layer_norm_cuda, "CUDA")
+_lib.impl("layer_norm_bwd", _layer_norm_bwd_cuda, "CUDA")
+_lib.impl("multi_norm", _multi_norm_cuda, "CUDA")
+_lib.impl("multi_clip_", _multi_clip_cuda, "CUDA")
 _lib.impl("rmsnorm_bwd", _rmsnorm_bwd_cuda, "CUDA")
 _lib.impl("swiglu_bwd", _swiglu_bwd_cuda, "CUDA")
 _lib.impl("swiglu_amax", _swiglu_amax_cuda, "CUDA")
@@ -377,6 +564,59 @@ def _delayed_sync_fake(amax, hist, n_e4m3, orig_dtype, scale_out, hist_out):
 @torch.library.register_fake("f8b200::scaled_mm")
 def _scaled_mm_fake(a, b_t, scale_a, scale_b, bias, out_dtype, use_fast_accum):
     return a.new_empty((a.shape[0], b_t.shape[0]), dtype=out_dtype)
+
+
+@torch.library.register_fake("f8b200::cast_blockwise")
+def _cast_blockwise_fake(x, fp8_kind, by_row, by_col):
+    rows, cols = x.shape
+    f8 = N.FP8_DTYPE[fp8_kind]
+
+    def data(on):
+        return x.new_empty((rows, _pitch16(cols)), dtype=f8)[:, :cols] if on else x.new_empty((0, 0), dtype=f8)
+
+    scale = x.new_empty((_blocks(cols), rows) if by_row else (0, 0), dtype=torch.float32)
+    scale_c = x.new_empty((_blocks(rows), cols) if by_col else (0, 0), dtype=torch.float32)
+    return data(by_row), scale.t(), data(by_col), scale_c
+
+
+@torch.library.register_fake("f8b200::cast_blockwise_square")
+def _cast_blockwise_square_fake(x, fp8_kind):
+    rows, cols = x.shape
+    data = x.new_empty((rows, _pitch16(cols)), dtype=N.FP8_DTYPE[fp8_kind])[:, :cols]
+    return data, x.new_empty((_blocks(rows), _blocks(cols)), dtype=torch.float32)
+
+
+@torch.library.register_fake("f8b200::uncast_blockwise")
+def _uncast_blockwise_fake(q, scale_inv, block_rows, block_cols, dtype):
+    return q.new_empty(q.shape, dtype=dtype)
+
+
+@torch.library.register_fake("f8b200::blockwise_mm")
+def _blockwise_mm_fake(a, b_t, scale_a, scale_b, a_block_rows, b_block_rows, bias, out_dtype):
+    return a.new_empty((a.shape[0], b_t.shape[0]), dtype=out_dtype)
+
+
+@torch.library.register_fake("f8b200::layer_norm")
+def _layer_norm_fake(x, weight, bias, eps, save_stats):
+    stats = x.new_empty((2, x.numel() // max(x.shape[-1], 1) if save_stats else 0), dtype=torch.float32)
+    return x.new_empty(x.shape), stats[0], stats[1]
+
+
+@torch.library.register_fake("f8b200::layer_norm_bwd")
+def _layer_norm_bwd_fake(x, grad_y, weight, mean, rstd, affine_dtype, need_dx, need_dw, need_db):
+    cols = x.shape[-1]
+    return (x.new_empty(x.shape if need_dx else (0,)), x.new_empty((cols if need_dw else 0,), dtype=affine_dtype),
+            x.new_empty((cols if need_db else 0,), dtype=affine_dtype))
+
+
+@torch.library.register_fake("f8b200::multi_norm")
+def _multi_norm_fake(xs, kind, root):
+    return xs[0].new_empty((), dtype=torch.float32)
+
+
+@torch.library.register_fake("f8b200::multi_clip_")
+def _multi_clip_fake(xs, total_norm, max_norm):
+    return None
 
 
 ops = torch.ops.f8b200

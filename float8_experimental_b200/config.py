@@ -14,9 +14,10 @@ class ScalingType(enum.Enum):
 
     DELAYED = "delayed"  # scale comes from a history of earlier amaxes
     DYNAMIC = "dynamic"  # scale comes from the amax of the tensor being cast
+    BLOCKWISE = "blockwise"  # one scale per block of 128, from the block's amax (all three tensors together)
 
     def short_str(self) -> str:
-        return {"delayed": "del", "dynamic": "dyn"}[self.value]
+        return {"delayed": "del", "dynamic": "dyn", "blockwise": "blk"}[self.value]
 
 
 @dataclass(frozen=True)

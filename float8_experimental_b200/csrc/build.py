@@ -13,12 +13,12 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
 LIB_DIR = os.path.join(PKG, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libf8b200.so")
-SOURCES = ["capi.cu", "cast.cu", "gemm.cu", "norm.cu", "reduce.cu"]
+SOURCES = ["capi.cu", "cast.cu", "cast_block.cu", "gemm.cu", "grad_clip.cu", "layer_norm.cu", "norm.cu", "reduce.cu"]
 # Single-GPU extra: the cluster-multicast GEMM lives in a library of its own, so that runs on
 # several GPUs can leave its source and binary out altogether (it includes gemm.cu).
 MC_LIB_PATH = os.path.join(LIB_DIR, "libf8b200_mc.so")
 MC_SOURCES = ["capi.cu", "gemm_mc.cu"]
-HEADERS = ["common.cuh", os.path.join("..", "..", "include", "f8b200.h")]
+HEADERS = ["common.cuh", "gemm_block.cuh", os.path.join("..", "..", "include", "f8b200.h")]
 
 
 def _nvcc() -> str:

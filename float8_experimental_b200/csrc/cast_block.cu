@@ -1,0 +1,376 @@
+// Casts to fp8 with one scale per block of 128, and the way back.
+//
+// A block is 1 x 128 (by rows), 128 x 1 (by columns) or 128 x 128.  With a = max(max|x|, 1e-12) over the block and
+// e the largest whole number with a * 2^e <= the format's maximum,
+//     q = fp8(x * 2^e)  (nearest even),    scale_inv = 2^-e,    the block stands for q * scale_inv.
+// A power of two moves the exponent only: neither the product nor its inverse rounds, so the only rounding of the
+// cast is the one to fp8, and it costs no accuracy against amax / max: fp8 is a floating format, whose
+// relative step does not depend on where in its range a value lies.  A block that holds an infinity
+// or a NaN is stored as NaN in every place, with a NaN factor.
+//
+// One CTA takes a 128 x 128 tile, so every block lies inside one CTA and x is read once for all the forms asked
+// for: 256 threads, 8 columns and 8 rows (16 apart) per thread, held in registers.
+#include "common.cuh"
+
+namespace f8b200 {
+namespace {
+
+constexpr int kBlk = 128;
+constexpr int kThreads = 256;
+enum { kByRow = 1, kByCol = 2, kBySquare = 4 };
+
+struct BlockCastArgs {
+  const char* x;
+  int64_t rows, cols, ld;  // elements
+  uint8_t *out_r, *out_c;  // by rows or squares, by columns
+  int64_t ld_r, ld_c;
+  float *scale_r, *scale_c;
+  int64_t ld_scale_r, ld_scale_c;
+  int64_t tiles_k;
+};
+
+// up = 2^e and down = 2^-e of a block whose amax has these fp32 bits
+template <int KIND>
+__device__ __forceinline__ void block_scale(uint32_t amax_bits, float& up, float& down) {
+  if (amax_bits >= 0x7F800000u) {
+    up = down = __uint_as_float(0x7FFFFFFFu);
+    return;
+  }
+  const uint32_t a = max(amax_bits, __float_as_uint(kEps));
+  // both maxima are 1.75 * 2^kTop: one power less when the amax's fraction exceeds 1.75
+  constexpr int kTop = KIND == F8B200_E4M3 ? 8 : 15;
+  const int e = kTop - ((int)(a >> 23) - 127) - ((a & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+  up = __uint_as_float((uint32_t)(127 + e) << 23);
+  down = __uint_as_float((uint32_t)(127 - e) << 23);
+}
+
+template <int HP>
+__device__ __forceinline__ uint32_t widen_bits(uint32_t h) {  // |x| bits of T -> fp32 bits
+  if constexpr (HP == F8B200_BF16) return h << 16;
+  else return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
+}
+
+// Eight consecutive elements of a row as fp32; `n` of them exist.
+template <int HP, bool VEC>
+__device__ __forceinline__ void load8(const char* p, int n, float (&v)[8]) {
+  if constexpr (HP == F8B200_FP32) {
+    const float* f = reinterpret_cast<const float*>(p);
+    if constexpr (VEC) {
+      if (n > 0) {
+        const float4 a = __ldcs(reinterpret_cast<const float4*>(f)), b = __ldcs(reinterpret_cast<const float4*>(f) + 1);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        return;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < n ? __ldcs(f + j) : 0.f;
+  } else {
+    const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+    if (VEC) {
+      if (n > 0) {
+        const uint4 q = __ldcs(reinterpret_cast<const uint4*>(p));
+        w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < n) w[j >> 1] |= (uint32_t)__ldcs(h + j) << (16 * (j & 1));
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (HP == F8B200_BF16) {
+        v[2 * j] = __uint_as_float(w[j] << 16);
+        v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+        v[2 * j] = f.x;
+        v[2 * j + 1] = f.y;
+      }
+    }
+  }
+}
+
+template <bool VEC>
+__device__ __forceinline__ void store8(uint8_t* p, int n, uint32_t lo, uint32_t hi) {
+  if constexpr (VEC) {
+    if (n > 0) *reinterpret_cast<uint2*>(p) = make_uint2(lo, hi);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n) p[j] = (uint8_t)((j < 4 ? lo : hi) >> (8 * (j & 3)));
+  }
+}
+
+template <int HP, int KIND, int FORMS, bool VEC>
+__global__ void __launch_bounds__(kThreads) cast_block_kernel(const BlockCastArgs p) {
+  __shared__ uint32_t col_max[kThreads / 32][kBlk];
+  __shared__ uint32_t warp_max[kThreads / 32];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t tm = blockIdx.x / p.tiles_k, tk = blockIdx.x - tm * p.tiles_k;
+  const int64_t row0 = tm * kBlk, col = tk * kBlk + tx * 8;
+  const int n = (int)max((int64_t)0, min((int64_t)8, p.cols - col));
+  constexpr int kEs = HP == F8B200_FP32 ? 4 : 2;
+
+  float v[8][8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t r = row0 + ty + 16 * i;
+    load8<HP, VEC>(p.x + (r * p.ld + col) * kEs, r < p.rows ? n : 0, v[i]);
+  }
+
+  uint32_t rmax[8];  // |x| bits, fp32: unsigned order is the order of the values, NaN above infinity
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[i][j]) & 0x7FFFFFFFu);
+    rmax[i] = m;
+  }
+  if constexpr (FORMS & kByCol) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i][j]) & 0x7FFFFFFFu);
+      m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 16));
+      if (lane < 16) col_max[warp][tx * 8 + j] = m;
+    }
+  }
+  float up_sq = 0.f;
+  if constexpr (FORMS & kBySquare) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, rmax[i]);
+    m = warp_max_u32(m);
+    if (lane == 0) warp_max[warp] = m;
+  }
+  if constexpr ((FORMS & (kByCol | kBySquare)) != 0) __syncthreads();
+  if constexpr (FORMS & kBySquare) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) m = max(m, warp_max[w]);
+    float down;
+    block_scale<KIND>(m, up_sq, down);
+    if (threadIdx.x == 0) p.scale_r[tm * p.ld_scale_r + tk] = down;
+  }
+
+  if constexpr (FORMS & (kByRow | kBySquare)) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int64_t r = row0 + ty + 16 * i;
+      float up = up_sq;
+      if constexpr (FORMS & kByRow) {
+        uint32_t m = rmax[i];
+#pragma unroll
+        for (int off = 8; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, off));
+        float down;
+        block_scale<KIND>(m, up, down);
+        if (tx == 0 && r < p.rows) p.scale_r[tk * p.ld_scale_r + r] = down;
+      }
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = cvt_pair_raw<KIND>(v[i][2 * j] * up, v[i][2 * j + 1] * up);
+      if (r < p.rows) store8<VEC>(p.out_r + r * p.ld_r + col, n, w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+    }
+  }
+  if constexpr (FORMS & kByCol) {
+    float up[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int w = 0; w < kThreads / 32; ++w) m = max(m, col_max[w][tx * 8 + j]);
+      float down;
+      block_scale<KIND>(m, up[j], down);
+      if (ty == 0 && j < n) p.scale_c[tm * p.ld_scale_c + col + j] = down;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int64_t r = row0 + ty + 16 * i;
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = cvt_pair_raw<KIND>(v[i][2 * j] * up[2 * j], v[i][2 * j + 1] * up[2 * j + 1]);
+      if (r < p.rows) store8<VEC>(p.out_c + r * p.ld_c + col, n, w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+    }
+  }
+}
+
+template <int HP, int KIND, bool VEC>
+int launch_forms(const BlockCastArgs& p, int forms, int64_t tiles, cudaStream_t st) {
+  const unsigned grid = (unsigned)tiles;
+  if (forms == kByRow) cast_block_kernel<HP, KIND, kByRow, VEC><<<grid, kThreads, 0, st>>>(p);
+  else if (forms == kByCol) cast_block_kernel<HP, KIND, kByCol, VEC><<<grid, kThreads, 0, st>>>(p);
+  else if (forms == (kByRow | kByCol)) cast_block_kernel<HP, KIND, kByRow | kByCol, VEC><<<grid, kThreads, 0, st>>>(p);
+  else cast_block_kernel<HP, KIND, kBySquare, VEC><<<grid, kThreads, 0, st>>>(p);
+  return check_launch();
+}
+
+// fp8 -> T: y = q * scale_inv(block).  16 consecutive columns per thread; they share a factor unless the blocks are
+// one column wide (16 divides 128).
+struct BlockUncastArgs {
+  const uint8_t* q;
+  int64_t rows, cols, ld_q;
+  const float* scale;
+  int64_t s_row, s_col;    // strides of the factors
+  int row_shift, col_shift;  // 7: one factor per 128 rows / columns, 0: per row / column
+  char* y;
+  int64_t ld_y;
+  int64_t chunks;  // ceil(cols / 16)
+};
+
+template <int HP>
+__device__ __forceinline__ void store_hp(char* base, int64_t i, float v) {
+  if constexpr (HP == F8B200_BF16) reinterpret_cast<__nv_bfloat16*>(base)[i] = __float2bfloat16_rn(v);
+  else if constexpr (HP == F8B200_FP16) reinterpret_cast<__half*>(base)[i] = __float2half_rn(v);
+  else reinterpret_cast<float*>(base)[i] = v;
+}
+
+template <int HP, int KIND, bool VEC>
+__global__ void __launch_bounds__(kThreads) uncast_block_kernel(const BlockUncastArgs p) {
+  constexpr __nv_fp8_interpretation_t kInterp = KIND == F8B200_E4M3 ? __NV_E4M3 : __NV_E5M2;
+  const int64_t total = p.rows * p.chunks;
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
+    const int64_t r = i / p.chunks, c = (i - r * p.chunks) * 16;
+    const int n = (int)min((int64_t)16, p.cols - c);
+    const uint8_t* q = p.q + r * p.ld_q + c;
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+    if constexpr (VEC) {
+      const uint4 t = __ldcs(reinterpret_cast<const uint4*>(q));
+      w[0] = t.x, w[1] = t.y, w[2] = t.z, w[3] = t.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (j < n) w[j >> 2] |= (uint32_t)q[j] << (8 * (j & 3));
+    }
+    const float* sp = p.scale + (r >> p.row_shift) * p.s_row;
+    float y[16];
+    const float s0 = __ldg(sp + (c >> p.col_shift) * p.s_col);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((w[j >> 1] >> (16 * (j & 1))) & 0xFFFFu), kInterp);
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+      float sa = s0, sb = s0;
+      if (p.col_shift == 0) {
+        sa = 2 * j < n ? __ldg(sp + (c + 2 * j) * p.s_col) : 0.f;
+        sb = 2 * j + 1 < n ? __ldg(sp + (c + 2 * j + 1) * p.s_col) : 0.f;
+      }
+      y[2 * j] = f.x * sa;
+      y[2 * j + 1] = f.y * sb;
+    }
+    if constexpr (VEC) {
+      if constexpr (HP == F8B200_FP32) {
+        float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.y) + r * p.ld_y + c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) __stcs(o + j, make_float4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]));
+      } else {
+        uint4* o = reinterpret_cast<uint4*>(p.y + (r * p.ld_y + c) * 2);
+        uint32_t h[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if constexpr (HP == F8B200_BF16) {
+            const __nv_bfloat162 t = __floats2bfloat162_rn(y[2 * j], y[2 * j + 1]);
+            h[j] = *reinterpret_cast<const uint32_t*>(&t);
+          } else {
+            const __half2 t = __floats2half2_rn(y[2 * j], y[2 * j + 1]);
+            h[j] = *reinterpret_cast<const uint32_t*>(&t);
+          }
+        }
+        __stcs(o, make_uint4(h[0], h[1], h[2], h[3]));
+        __stcs(o + 1, make_uint4(h[4], h[5], h[6], h[7]));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (j < n) store_hp<HP>(p.y, r * p.ld_y + c + j, y[j]);
+    }
+  }
+}
+
+bool aligned(const void* p, int64_t to) { return p == nullptr || reinterpret_cast<uintptr_t>(p) % to == 0; }
+
+}  // namespace
+}  // namespace f8b200
+
+using namespace f8b200;
+
+extern "C" int f8b200_cast_blockwise(const void* x, int hp_dtype, int64_t rows, int64_t cols, int64_t ld_x, int fp8_kind,
+                                     int by_square, void* out_r, int64_t ld_r, float* scale_r, int64_t ld_scale_r,
+                                     void* out_c, int64_t ld_c, float* scale_c, int64_t ld_scale_c, void* stream) {
+  if (hp_dtype < 0 || hp_dtype > 2 || fp8_kind < 0 || fp8_kind > 1 || rows < 0 || cols < 0) return F8B200_ERR_BAD_ARG;
+  if (out_r == nullptr && out_c == nullptr) return F8B200_ERR_BAD_ARG;
+  if (by_square != 0 && (out_r == nullptr || out_c != nullptr)) return F8B200_ERR_BAD_ARG;
+  if (rows == 0 || cols == 0) return F8B200_OK;
+  const int64_t tiles_m = (rows + kBlk - 1) / kBlk, tiles_k = (cols + kBlk - 1) / kBlk;
+  if (x == nullptr || ld_x < cols) return F8B200_ERR_BAD_ARG;
+  if (out_r != nullptr && (scale_r == nullptr || ld_r < cols || ld_scale_r < (by_square ? tiles_k : rows))) return F8B200_ERR_BAD_ARG;
+  if (out_c != nullptr && (scale_c == nullptr || ld_c < cols || ld_scale_c < cols)) return F8B200_ERR_BAD_ARG;
+  if (tiles_m > 0x7FFFFFFFLL / tiles_k) return F8B200_ERR_UNSUPPORTED;
+  const int es = hp_size_of(hp_dtype);
+  if (!aligned(x, es) || !aligned(scale_r, 4) || !aligned(scale_c, 4)) return F8B200_ERR_ALIGNMENT;
+  int rc = f8b200_device_check();
+  if (rc != F8B200_OK) return rc;
+  BlockCastArgs p;
+  p.x = static_cast<const char*>(x);
+  p.rows = rows, p.cols = cols, p.ld = ld_x;
+  p.out_r = static_cast<uint8_t*>(out_r), p.out_c = static_cast<uint8_t*>(out_c);
+  p.ld_r = ld_r, p.ld_c = ld_c;
+  p.scale_r = scale_r, p.scale_c = scale_c;
+  p.ld_scale_r = ld_scale_r, p.ld_scale_c = ld_scale_c;
+  p.tiles_k = tiles_k;
+  const int forms = by_square ? kBySquare : (out_r != nullptr ? kByRow : 0) | (out_c != nullptr ? kByCol : 0);
+  // whole 8-element chunks, loaded in 16-byte words and stored in 8-byte ones
+  const bool vec = cols % 8 == 0 && (ld_x * es) % 16 == 0 && aligned(x, 16) && aligned(out_r, 8) && aligned(out_c, 8) &&
+                   (out_r == nullptr || ld_r % 8 == 0) && (out_c == nullptr || ld_c % 8 == 0);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int64_t tiles = tiles_m * tiles_k;
+#define F8_CAST(HP, KIND) (vec ? launch_forms<HP, KIND, true>(p, forms, tiles, st) : launch_forms<HP, KIND, false>(p, forms, tiles, st))
+  if (fp8_kind == F8B200_E4M3) {
+    if (hp_dtype == F8B200_BF16) return F8_CAST(F8B200_BF16, F8B200_E4M3);
+    if (hp_dtype == F8B200_FP16) return F8_CAST(F8B200_FP16, F8B200_E4M3);
+    return F8_CAST(F8B200_FP32, F8B200_E4M3);
+  }
+  if (hp_dtype == F8B200_BF16) return F8_CAST(F8B200_BF16, F8B200_E5M2);
+  if (hp_dtype == F8B200_FP16) return F8_CAST(F8B200_FP16, F8B200_E5M2);
+  return F8_CAST(F8B200_FP32, F8B200_E5M2);
+#undef F8_CAST
+}
+
+extern "C" int f8b200_uncast_blockwise(const void* q, int fp8_kind, int64_t rows, int64_t cols, int64_t ld_q,
+                                       const float* scale, int64_t scale_row_stride, int64_t scale_col_stride,
+                                       int block_rows, int block_cols, int hp_dtype, void* y, int64_t ld_y, void* stream) {
+  if (hp_dtype < 0 || hp_dtype > 2 || fp8_kind < 0 || fp8_kind > 1 || rows < 0 || cols < 0) return F8B200_ERR_BAD_ARG;
+  if ((block_rows != 1 && block_rows != kBlk) || (block_cols != 1 && block_cols != kBlk)) return F8B200_ERR_BAD_ARG;
+  if (rows == 0 || cols == 0) return F8B200_OK;
+  if (q == nullptr || scale == nullptr || y == nullptr || ld_q < cols || ld_y < cols) return F8B200_ERR_BAD_ARG;
+  if (scale_row_stride < 0 || scale_col_stride < 0) return F8B200_ERR_BAD_ARG;
+  const int es = hp_size_of(hp_dtype);
+  if (!aligned(y, es) || !aligned(scale, 4)) return F8B200_ERR_ALIGNMENT;
+  int rc = f8b200_device_check();
+  if (rc != F8B200_OK) return rc;
+  BlockUncastArgs p;
+  p.q = static_cast<const uint8_t*>(q);
+  p.rows = rows, p.cols = cols, p.ld_q = ld_q;
+  p.scale = scale, p.s_row = scale_row_stride, p.s_col = scale_col_stride;
+  p.row_shift = block_rows == kBlk ? 7 : 0, p.col_shift = block_cols == kBlk ? 7 : 0;
+  p.y = static_cast<char*>(y), p.ld_y = ld_y;
+  p.chunks = (cols + 15) / 16;
+  const bool vec = cols % 16 == 0 && ld_q % 16 == 0 && aligned(q, 16) && aligned(y, 16) && (ld_y * es) % 16 == 0;
+  const int64_t work = (rows * p.chunks + kThreads - 1) / kThreads, cap = (int64_t)sm_count() * 16;
+  const unsigned grid = (unsigned)(work < cap ? work : cap);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+#define F8_UNCAST(HP, KIND)                                                                   \
+  (vec ? (void)(uncast_block_kernel<HP, KIND, true><<<grid, kThreads, 0, st>>>(p))            \
+       : (void)(uncast_block_kernel<HP, KIND, false><<<grid, kThreads, 0, st>>>(p)))
+  if (fp8_kind == F8B200_E4M3) {
+    if (hp_dtype == F8B200_BF16) F8_UNCAST(F8B200_BF16, F8B200_E4M3);
+    else if (hp_dtype == F8B200_FP16) F8_UNCAST(F8B200_FP16, F8B200_E4M3);
+    else F8_UNCAST(F8B200_FP32, F8B200_E4M3);
+  } else {
+    if (hp_dtype == F8B200_BF16) F8_UNCAST(F8B200_BF16, F8B200_E5M2);
+    else if (hp_dtype == F8B200_FP16) F8_UNCAST(F8B200_FP16, F8B200_E5M2);
+    else F8_UNCAST(F8B200_FP32, F8B200_E5M2);
+  }
+#undef F8_UNCAST
+  return check_launch();
+}

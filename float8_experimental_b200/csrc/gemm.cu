@@ -2421,3 +2421,7 @@ extern "C" int f8b200_check_device_error(void) {
   if (rc != F8B200_OK) return rc;
   return flags != 0 ? F8B200_ERR_TIMEOUT : F8B200_OK;
 }
+
+#ifndef F8B200_MC_LIBRARY
+#include "gemm_block.cuh"
+#endif

@@ -1,0 +1,648 @@
+// fp8 GEMM with one scale per block of 128 along K (included by gemm.cu, whose device helpers it uses):
+//   out[m,n] = sum_j sa(m,j) * sb(n,j) * (sum_{k in block j} A[m,k] * B[n,k])  (+ bias[n])
+// sa has one fp32 factor per row of A or per 128 rows, sb the same for B; both are read through two strides,
+// so a transposed or broadcast scale tensor needs no copy.
+//
+// The scale changes with the 128-wide block of K, so the tensor cores' sum over one block is a value of its
+// own: every block's MMAs start a fresh tensor-memory accumulator, and the epilogue warps add it, multiplied by
+// its scale, to fp32 sums that stay in registers for the whole tile.  Per block that costs a 128x256 tile's
+// CTA 32768 fp32 FMAs (256 cycles of its FMA pipes) and as many tensor-memory words against the 512 cycles of the
+// MMAs, and it runs beside them: two accumulators alternate.
+//
+// Two kernels:
+//   block pair kernel   two CTAs per 256x256 tile, tcgen05.mma.cta_group::2 as in the pair kernel of gemm.cu;
+//                       eight epilogue warps per CTA, one row and 128 columns per thread.
+//   few-rows kernel     A has few rows (tokens being served): B's rows take the 128-wide side of the MMA and A's
+//                       the narrow one, and the CTAs of a cluster split K and join their sums through
+//                       distributed shared memory, so that a product of a few tiles still uses every SM's share
+//                       of the memory bandwidth that B's bytes need.
+// Both are bounded in every wait like the kernels of gemm.cu.
+
+namespace f8b200 {
+namespace gemm {
+namespace block {
+
+using namespace pair;
+
+// factor of (row, block j) = p[(row >> shift) * row_stride + j * kb_stride]
+struct BlockScale {
+  const float* p;
+  int64_t row_stride, kb_stride;
+  int shift;  // 0: one factor per row, 7: per 128 rows
+};
+
+__device__ __forceinline__ void tc_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+// two fp32 values in one 64-bit register pair
+__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+  return v;
+}
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) { return pack2(__float_as_uint(lo), __float_as_uint(hi)); }
+__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) {
+  uint32_t a, b;
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
+  lo = __uint_as_float(a);
+  hi = __uint_as_float(b);
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2f(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+constexpr int BTHREADS = 320;  // TMA warp, MMA warp, 8 epilogue warps
+constexpr int BSTAGES = 6;
+constexpr int BSTAGE_BYTES = PA_BYTES + PB_BYTES;
+
+struct __align__(16) BlockBars {
+  float col_scale[8][2][128];  // per epilogue warp, two k-blocks: the factors of its 128 columns of B
+  uint64_t full[BSTAGES];
+  uint64_t empty[BSTAGES];
+  uint64_t tmem_full[2];
+  uint64_t tmem_empty[2];
+  uint32_t tmem_base;
+  volatile uint32_t abort_flag;
+};
+constexpr int BSMEM_BYTES = BSTAGES * BSTAGE_BYTES + 1024 + (int)sizeof(BlockBars);
+
+// PER_COL: B has one factor per row (a column of the output); otherwise one per 128 of them, which is one per
+// epilogue thread and k-block because a thread's 128 columns start on a multiple of 128.
+template <typename OutT, bool PER_COL>
+__global__ void __launch_bounds__(BTHREADS, 1)
+gemm_block_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
+                       const BlockScale scale_a, const BlockScale scale_b, const OutT* __restrict__ bias,
+                       OutT* __restrict__ out, int64_t ldo, int m, int n, int k, uint32_t idesc, int out_vec_ok,
+                       int raster) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  BlockBars* bars = reinterpret_cast<BlockBars*>(tiles + BSTAGES * BSTAGE_BYTES);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const uint32_t peer = rank ^ 1u;
+  const bool leader = rank == 0;
+  const int tiles_m = (m + PBM - 1) / PBM, tiles_n = (n + PBN - 1) / PBN;
+  const int64_t num_tiles = (int64_t)tiles_m * tiles_n;
+  const int num_kb = (k + BK - 1) / BK;
+  const int64_t cluster_id = blockIdx.x >> 1, num_clusters = gridDim.x >> 1;
+  const bool a_mn = (raster >> LAYOUT_A_MN_BIT) & 1, b_mn = (raster >> LAYOUT_B_MN_BIT) & 1;
+  const uint64_t step_a = desc_k_step(a_mn), step_b = desc_k_step(b_mn);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < BSTAGES; ++s) {
+      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&bars->tmem_full[a], 1);
+      mbar_init(&bars->tmem_empty[a], 16);
+    }
+    bars->abort_flag = 0u;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem_base)),
+                 "r"((uint32_t)TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem_base = bars->tmem_base;
+
+  if (warp == 0) {
+    // ---------------- TMA producer (one per CTA) ----------------
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int64_t t = cluster_id; ok && t < num_tiles; t += num_clusters) {
+        const TileCoord tc = tile_coord(t, tiles_m, tiles_n, raster);
+        const int row_a = tc.m * PBM + (int)rank * 128;
+        const int row_b = tc.n * PBN + (int)rank * 128;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!pair_wait(&bars->empty[stage], phase ^ 1u, bars, peer, 1u, 64u)) { ok = false; break; }
+          uint8_t* sa = tiles + stage * BSTAGE_BYTES;
+          if (leader) mbar_expect_tx(&bars->full[stage], 2 * BSTAGE_BYTES);
+          const uint32_t full_in_leader = mapa_u32(smem_u32(&bars->full[stage]), 0u);
+          tma_load_2d_pair_plain(sa, &tma_a, a_mn ? row_a : kb * BK, a_mn ? kb * BK : row_a, full_in_leader);
+          tma_load_2d_pair_plain(sa + PA_BYTES, &tma_b, b_mn ? row_b : kb * BK, b_mn ? kb * BK : row_b,
+                                 full_in_leader);
+          if (++stage == BSTAGES) { stage = 0; phase ^= 1u; }
+        }
+      }
+      // tail: every release the leader multicast to this CTA's empty barriers has landed
+      for (int s = 0; ok && s < BSTAGES; ++s) {
+        if (!pair_wait(&bars->empty[stage], phase ^ 1u, bars, peer, 1u, 64u)) { ok = false; break; }
+        if (++stage == BSTAGES) { stage = 0; phase ^= 1u; }
+      }
+      if (!ok) {  // give the loads in flight time to land before the CTA leaves
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000LL) {}
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer (leader CTA only) ----------------
+    if (leader && lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      uint32_t g = 0;  // k-blocks issued so far: their accumulators alternate
+      for (int64_t t = cluster_id; ok && t < num_tiles; t += num_clusters) {
+        for (int kb = 0; kb < num_kb; ++kb, ++g) {
+          const uint32_t acc = g & 1u;
+          if (!pair_wait(&bars->full[stage], phase, bars, peer, 4u)) { ok = false; break; }
+          if (!pair_wait(&bars->tmem_empty[acc], ((g >> 1) & 1u) ^ 1u, bars, peer, 2u)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t a_addr = smem_u32(tiles + stage * BSTAGE_BYTES);
+          const uint64_t da = a_mn ? make_smem_desc_mn(a_addr, PA_BYTES) : make_smem_desc(a_addr);
+          const uint64_t db = b_mn ? make_smem_desc_mn(a_addr + PA_BYTES, PB_BYTES) : make_smem_desc(a_addr + PA_BYTES);
+          const uint32_t tmem_d = tmem_base + acc * (uint32_t)PBN;
+#pragma unroll
+          for (int kk = 0; kk < BK / UMMA_K; ++kk)
+            tc_mma_f8_pair(tmem_d, da + (uint64_t)kk * step_a, db + (uint64_t)kk * step_b, idesc, kk != 0 ? 1u : 0u);
+          tc_commit_pair(&bars->empty[stage]);
+          tc_commit_pair(&bars->tmem_full[acc]);
+          if (++stage == BSTAGES) { stage = 0; phase ^= 1u; }
+        }
+      }
+    }
+  } else {
+    // ---------------- epilogue (warps 2..9 of both CTAs) ----------------
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t taddr0 = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128);
+    const uint32_t empty_in_leader[2] = {mapa_u32(smem_u32(&bars->tmem_empty[0]), 0u),
+                                         mapa_u32(smem_u32(&bars->tmem_empty[1]), 0u)};
+    bool ok = true;
+    uint32_t g = 0;
+    for (int64_t t = cluster_id; ok && t < num_tiles; t += num_clusters) {
+      const TileCoord tc = tile_coord(t, tiles_m, tiles_n, raster);
+      const int row = tc.m * PBM + (int)rank * 128 + quarter * 32 + lane;
+      const int col0 = tc.n * PBN + half * 128;
+      const bool row_in = row < m, cols_in = col0 < n;
+      const float* pa = scale_a.p + (int64_t)((row_in ? row : 0) >> scale_a.shift) * scale_a.row_stride;
+      const float* pb = scale_b.p + (int64_t)((cols_in ? col0 : 0) >> scale_b.shift) * scale_b.row_stride;
+      uint64_t acc[64];
+#pragma unroll
+      for (int i = 0; i < 64; ++i) acc[i] = 0ull;
+      float sa = row_in ? __ldg(pa) : 0.f;
+      float sb = 0.f, sc[4] = {0.f, 0.f, 0.f, 0.f};
+      auto load_cols = [&](int kb) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int c = col0 + lane + 32 * j;
+          sc[j] = c < n ? __ldg(scale_b.p + (int64_t)(c >> scale_b.shift) * scale_b.row_stride +
+                                (int64_t)kb * scale_b.kb_stride) : 0.f;
+        }
+      };
+      if constexpr (PER_COL) load_cols(0); else sb = cols_in ? __ldg(pb) : 0.f;
+      for (int kb = 0; kb < num_kb; ++kb, ++g) {
+        const uint32_t buf = g & 1u;
+        const float* cs = bars->col_scale[warp - 2][kb & 1];
+        if constexpr (PER_COL) {
+          float* w = bars->col_scale[warp - 2][kb & 1];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[lane + 32 * j] = sc[j];
+          __syncwarp();
+        }
+        const float s = PER_COL ? sa : sa * sb;
+        const uint64_t s2 = pack2(s, s);
+        if (kb + 1 < num_kb) {  // the next block's factors travel while this one is added up
+          sa = row_in ? __ldg(pa + (int64_t)(kb + 1) * scale_a.kb_stride) : 0.f;
+          if constexpr (PER_COL) load_cols(kb + 1);
+          else sb = cols_in ? __ldg(pb + (int64_t)(kb + 1) * scale_b.kb_stride) : 0.f;
+        }
+        if (!pair_wait(&bars->tmem_full[buf], (g >> 1) & 1u, bars, peer, 8u)) { ok = false; break; }
+        __syncwarp();
+        tc_fence_after();
+        const uint32_t taddr = taddr0 + buf * (uint32_t)PBN;
+        uint32_t r[2][16];
+        tc_ld_32x32b_x16(taddr, r[0]);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          tc_wait_ld();
+          if (c < 7) {
+            tc_ld_32x32b_x16(taddr + (uint32_t)(16 * (c + 1)), r[(c + 1) & 1]);
+          } else {  // everything is in registers: the accumulator is free for the MMAs of the next but one block
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(empty_in_leader[buf]);
+          }
+          const uint32_t(&v)[16] = r[c & 1];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            uint64_t f = s2;
+            if constexpr (PER_COL) f = mul2f(s2, *reinterpret_cast<const uint64_t*>(cs + c * 16 + 2 * i));
+            acc[c * 8 + i] = fma2(pack2(v[2 * i], v[2 * i + 1]), f, acc[c * 8 + i]);
+          }
+        }
+      }
+      if (!ok) break;
+      if (row_in) {
+        OutT* orow = out + (int64_t)row * ldo;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int col = col0 + c * 32;
+          const int ncols = min(32, n - col);
+          if (ncols > 0) {
+            float v[32];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) unpack2(acc[c * 16 + i], v[2 * i], v[2 * i + 1]);
+            if (bias != nullptr) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (i < ncols) v[i] += static_cast<float>(bias[col + i]);
+            }
+            store_chunk<OutT>(orow + col, v, ncols, out_vec_ok != 0);
+          }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // neither CTA leaves while the other may still touch its barriers or TMEM
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)TMEM_COLS)
+                 : "memory");
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------
+// Few rows of A.  D[128 rows of B, T rows of A] per CTA, K split over the CTAs of a cluster.
+// ---------------------------------------------------------------------------------------------------
+constexpr int FTHREADS = 192;  // TMA warp, MMA warp, 4 epilogue warps
+
+template <int T>
+struct FewCfg {
+  static constexpr int kXBytes = T * BK;
+  static constexpr int kStageBytes = 128 * BK + kXBytes;
+  static constexpr int kStages = T <= 32 ? 5 : T <= 64 ? 4 : 3;  // about 100 KB, so that two CTAs share an SM
+  static constexpr int kTmemCols = 2 * T < 32 ? 32 : 2 * T;
+  static constexpr int kJoinBytes = T * 128 * 4;   // fp32 sums handed over at the end, over the stages
+  static_assert(kJoinBytes <= kStages * kStageBytes, "the sums have to fit into the stages");
+};
+template <int T>
+struct __align__(16) FewBars {
+  float x_scale[4][2][T];  // per epilogue warp, two k-blocks: the factors of A's rows
+  uint64_t full[FewCfg<T>::kStages];
+  uint64_t empty[FewCfg<T>::kStages];
+  uint64_t tmem_full[2];
+  uint64_t tmem_empty[2];
+  uint32_t tmem_base;
+  volatile uint32_t abort_flag;
+};
+template <int T>
+constexpr int few_smem_bytes() {
+  return FewCfg<T>::kStages * FewCfg<T>::kStageBytes + 1024 + (int)sizeof(FewBars<T>);
+}
+template <typename Bars>
+__device__ __forceinline__ bool few_wait(uint64_t* bar, uint32_t parity, Bars* bars, uint32_t who) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  for (uint32_t it = 0; it < 0x7FFFFFFFu; ++it) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((it & 63u) == 63u) {
+      if (bars->abort_flag != 0u) return false;
+      if (clock64() - t0 > WAIT_BUDGET_CYCLES) break;
+    }
+  }
+  bars->abort_flag = 1u;
+  atomicOr(&g_device_error, who | 0x200u);
+  return false;
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+  return v;
+}
+
+// grid: x = K split (the cluster), y = tiles of 128 rows of B, z = tiles of T rows of A
+template <typename OutT, int T>
+__global__ void __launch_bounds__(FTHREADS)
+gemm_block_few_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_constant__ CUtensorMap tma_x,
+                      const BlockScale scale_w, const BlockScale scale_x, const OutT* __restrict__ bias,
+                      OutT* __restrict__ out, int64_t ldo, int m, int n, int k, uint32_t idesc, int w_mn) {
+  using Cfg = FewCfg<T>;
+  constexpr int S = Cfg::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  FewBars<T>* bars = reinterpret_cast<FewBars<T>*>(tiles + S * Cfg::kStageBytes);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = (int)gridDim.x;
+  const uint32_t rank = split > 1 ? cluster_ctarank() : 0u;
+  const int num_kb_all = (k + BK - 1) / BK;
+  const int kb0 = (int)((int64_t)num_kb_all * rank / split), kb1 = (int)((int64_t)num_kb_all * (rank + 1) / split);
+  const int row_w = (int)blockIdx.y * 128, row_x = (int)blockIdx.z * T;
+  const uint64_t step_w = desc_k_step(w_mn != 0), step_x = desc_k_step(false);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&bars->tmem_full[a], 1);
+      mbar_init(&bars->tmem_empty[a], 4);
+    }
+    bars->abort_flag = 0u;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem_base)),
+                 "r"((uint32_t)Cfg::kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = bars->tmem_base;
+
+  bool good = true;
+  float acc[T];
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!few_wait(&bars->empty[stage], phase ^ 1u, bars, 1u)) { ok = false; break; }
+        uint8_t* sw = tiles + stage * Cfg::kStageBytes;
+        mbar_expect_tx(&bars->full[stage], Cfg::kStageBytes);
+        tma_load_2d(sw, &tma_w, w_mn ? row_w : kb * BK, w_mn ? kb * BK : row_w, &bars->full[stage]);
+        tma_load_2d(sw + 128 * BK, &tma_x, kb * BK, row_x, &bars->full[stage]);
+        if (++stage == S) { stage = 0; phase ^= 1u; }
+      }
+      // tail: the MMAs have read every stage (the stages are reused for the sums below)
+      for (int s = 0; ok && s < S; ++s) {
+        if (!few_wait(&bars->empty[stage], phase ^ 1u, bars, 1u)) { ok = false; break; }
+        if (++stage == S) { stage = 0; phase ^= 1u; }
+      }
+      if (!ok) {
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000LL) {}
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0, g = 0;
+      for (int kb = kb0; kb < kb1; ++kb, ++g) {
+        const uint32_t buf = g & 1u;
+        if (!few_wait(&bars->full[stage], phase, bars, 4u)) break;
+        if (!few_wait(&bars->tmem_empty[buf], ((g >> 1) & 1u) ^ 1u, bars, 2u)) break;
+        tc_fence_after();
+        const uint32_t w_addr = smem_u32(tiles + stage * Cfg::kStageBytes);
+        const uint64_t dw = w_mn ? make_smem_desc_mn(w_addr, 128 * BK) : make_smem_desc(w_addr);
+        const uint64_t dx = make_smem_desc(w_addr + 128 * BK);
+#pragma unroll
+        for (int kk = 0; kk < BK / UMMA_K; ++kk)
+          tc_mma_f8(tmem_base + buf * T, dw + (uint64_t)kk * step_w, dx + (uint64_t)kk * step_x, idesc, kk != 0 ? 1u : 0u);
+        tc_commit(&bars->empty[stage]);
+        tc_commit(&bars->tmem_full[buf]);
+        if (++stage == S) { stage = 0; phase ^= 1u; }
+      }
+    }
+  } else {
+    const int quarter = warp & 3;
+    const int row = row_w + quarter * 32 + lane;
+    const bool row_in = row < n;
+    const float* pw = scale_w.p + (int64_t)((row_in ? row : 0) >> scale_w.shift) * scale_w.row_stride;
+    constexpr int XL = (T + 31) / 32;  // factors of A's rows that one lane fetches per k-block
+    float sx[XL], sw = 0.f;
+    auto fetch = [&](int kb) {
+      sw = row_in ? __ldg(pw + (int64_t)kb * scale_w.kb_stride) : 0.f;
+#pragma unroll
+      for (int j = 0; j < XL; ++j) {
+        const int r = row_x + lane + 32 * j;
+        sx[j] = (lane + 32 * j < T && r < m) ? __ldg(scale_x.p + (int64_t)(r >> scale_x.shift) * scale_x.row_stride +
+                                                     (int64_t)kb * scale_x.kb_stride) : 0.f;
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < T; ++i) acc[i] = 0.f;
+    if (kb0 < kb1) fetch(kb0);
+    uint32_t g = 0;
+    for (int kb = kb0; kb < kb1; ++kb, ++g) {
+      const uint32_t buf = g & 1u;
+      float* xs = bars->x_scale[warp - 2][buf];
+#pragma unroll
+      for (int j = 0; j < XL; ++j)
+        if (lane + 32 * j < T) xs[lane + 32 * j] = sx[j];
+      __syncwarp();
+      const float s = sw;
+      if (kb + 1 < kb1) fetch(kb + 1);
+      if (!few_wait(&bars->tmem_full[buf], (g >> 1) & 1u, bars, 8u)) { good = false; break; }
+      __syncwarp();
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < T / 16; ++c) {
+        uint32_t r[16];
+        tc_ld_32x32b_x16(tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * T + c * 16, r);
+        tc_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[c * 16 + i] = fmaf(__uint_as_float(r[i]), s * xs[c * 16 + i], acc[c * 16 + i]);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->tmem_empty[buf]);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)Cfg::kTmemCols)
+                 : "memory");
+  }
+
+  // join: the sums lie as [token][128] in every CTA of the cluster; CTA r adds up and stores tokens r, r + split, ...
+  float* mine = reinterpret_cast<float*>(tiles);
+  if (warp >= 2 && good) {
+    const int r = (warp & 3) * 32 + lane;
+#pragma unroll
+    for (int i = 0; i < T; ++i) mine[i * 128 + r] = acc[i];
+  }
+  const bool failed = bars->abort_flag != 0u;
+  if (split > 1) cluster_sync_all(); else __syncthreads();
+  if (!failed) {
+    const int ntok = min(T, m - row_x);
+    for (int e = (int)threadIdx.x; e < ntok * 128; e += FTHREADS) {
+      const int i = e >> 7, c = e & 127, col = row_w + c;
+      if (i % split != (int)rank || col >= n) continue;
+      float v = 0.f;
+      if (split > 1) {
+        const uint32_t addr = smem_u32(mine + i * 128 + c);
+        for (int q = 0; q < split; ++q) v += ld_cluster_f32(mapa_u32(addr, (uint32_t)q));
+      } else {
+        v = mine[i * 128 + c];
+      }
+      if (bias != nullptr) v += static_cast<float>(bias[col]);
+      out[(int64_t)(row_x + i) * ldo + col] = static_cast<OutT>(v);
+    }
+  }
+  if (split > 1) cluster_sync_all();  // no CTA leaves while another may still read its sums
+}
+
+// ---- host side --------------------------------------------------------------------------------------
+static bool strides_ok(const BlockScale& s) { return s.row_stride >= 0 && s.kb_stride >= 0; }
+
+template <typename OutT, bool PER_COL>
+static int launch_block_pair(const CUtensorMap& ma, const CUtensorMap& mb, const BlockScale& sa, const BlockScale& sb,
+                             const void* bias, void* out, int64_t ldo, int m, int n, int k, uint32_t idesc, int vec_ok,
+                             int layouts, cudaStream_t st) {
+  static PerDeviceOnce setup;
+  int max_clusters = 0;
+  auto kernel = gemm_block_pair_kernel<OutT, PER_COL>;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.blockDim = dim3(BTHREADS);
+  cfg.dynamicSmemBytes = BSMEM_BYTES;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t attr_err = setup.run(
+      [&](int* clusters_out) {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BSMEM_BYTES);
+        if (e == cudaSuccess) {
+          cfg.gridDim = dim3(2 * (sm_count() / 2));
+          e = cudaOccupancyMaxActiveClusters(clusters_out, kernel, &cfg);
+        }
+        return e;
+      },
+      &max_clusters);
+  if (attr_err != cudaSuccess) return record_cuda_error(attr_err);
+  if (max_clusters < 1) return F8B200_ERR_UNSUPPORTED;
+  const int64_t tiles = (int64_t)((m + PBM - 1) / PBM) * ((n + PBN - 1) / PBN);
+  int clusters = max_clusters;
+  if (persistent_ctas() / 2 < clusters) clusters = persistent_ctas() / 2;
+  if (tiles < clusters) clusters = (int)tiles;
+  cfg.gridDim = dim3(2 * clusters);
+  return record_cuda_error(cudaLaunchKernelEx(&cfg, kernel, ma, mb, sa, sb, static_cast<const OutT*>(bias),
+                                              static_cast<OutT*>(out), ldo, m, n, k, idesc, vec_ok,
+                                              choose_raster(m, n, k, PBM, PBN) | layouts));
+}
+
+template <typename OutT, int T>
+static int launch_block_few(const CUtensorMap& mw, const CUtensorMap& mx, const BlockScale& sw, const BlockScale& sx,
+                            const void* bias, void* out, int64_t ldo, int m, int n, int k, uint32_t idesc, int w_mn,
+                            int split, cudaStream_t st) {
+  static PerDeviceOnce setup;
+  auto kernel = gemm_block_few_kernel<OutT, T>;
+  const cudaError_t attr_err = setup.run([&](int*) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, few_smem_bytes<T>());
+  });
+  if (attr_err != cudaSuccess) return record_cuda_error(attr_err);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = split;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.blockDim = dim3(FTHREADS);
+  cfg.dynamicSmemBytes = few_smem_bytes<T>();
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = split > 1 ? 1 : 0;
+  cfg.gridDim = dim3(split, (n + 127) / 128, (m + T - 1) / T);
+  return record_cuda_error(cudaLaunchKernelEx(&cfg, kernel, mw, mx, sw, sx, static_cast<const OutT*>(bias),
+                                              static_cast<OutT*>(out), ldo, m, n, k, idesc, w_mn));
+}
+
+// instruction descriptor of one CTA: 128 rows of B's side, `cols` rows of A's side
+static uint32_t make_idesc_few(int w_kind, int x_kind, int w_mn, int cols) {
+  return (1u << 4) | ((uint32_t)w_kind << 7) | ((uint32_t)x_kind << 10) | ((uint32_t)w_mn << 15) |
+         ((uint32_t)(cols >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+
+// CTAs of one cluster that split K: as many as keep the grid within two CTAs per SM and leave each at least four
+// k-blocks, in powers of two up to 8 (the portable cluster size).
+static int few_split(int64_t tiles, int num_kb) {
+  int split = 1;
+  while (split < 8 && tiles * split * 2 <= 2 * sm_count() && num_kb >= split * 2 * 4) split *= 2;
+  return split;
+}
+
+}  // namespace block
+}  // namespace gemm
+}  // namespace f8b200
+
+extern "C" int f8b200_gemm_blockwise(const void* a, int a_kind, int a_layout, int64_t lda, const float* scale_a,
+                                     int64_t sa_row_stride, int64_t sa_kb_stride, int a_block_rows, const void* b,
+                                     int b_kind, int b_layout, int64_t ldb, const float* scale_b, int64_t sb_row_stride,
+                                     int64_t sb_kb_stride, int b_block_rows, const void* bias, int out_dtype, void* out,
+                                     int64_t ldo, int64_t m, int64_t n, int64_t k, void* stream) {
+  using namespace gemm::block;
+  if ((a_block_rows != 1 && a_block_rows != 128) || (b_block_rows != 1 && b_block_rows != 128)) return F8B200_ERR_BAD_ARG;
+  const BlockScale sa{scale_a, sa_row_stride, sa_kb_stride, a_block_rows == 128 ? 7 : 0};
+  const BlockScale sb{scale_b, sb_row_stride, sb_kb_stride, b_block_rows == 128 ? 7 : 0};
+  if (!strides_ok(sa) || !strides_ok(sb)) return F8B200_ERR_BAD_ARG;
+  bool empty = false;
+  int rc = gemm_fp8_validate(a, a_kind, a_layout, lda, b, b_kind, b_layout, ldb, scale_a, scale_b, bias, out_dtype, out,
+                             ldo, m, n, k, &empty);
+  if (rc != F8B200_OK || empty) return rc;
+  const int osz = out_dtype == F8B200_FP32 ? 4 : 2;
+  const int vec_ok = (reinterpret_cast<uintptr_t>(out) % 16 == 0) && ((ldo * osz) % 16 == 0);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int layouts = (a_layout << gemm::LAYOUT_A_MN_BIT) | (b_layout << gemm::LAYOUT_B_MN_BIT);
+  CUtensorMap ma, mb;
+  // a box of an MN-major operand is 128 rows wide, so the few-rows kernel takes A K-major only
+  if (m <= 128 && a_layout == F8B200_K_MAJOR) {
+    const int t = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
+    rc = gemm::encode_operand_map(&ma, a, m, k, lda, t);
+    if (rc == F8B200_OK)
+      rc = b_layout ? gemm::encode_operand_map_mn(&mb, b, n, k, ldb) : gemm::encode_operand_map(&mb, b, n, k, ldb, 128);
+    if (rc != F8B200_OK) return rc;
+    const uint32_t idesc = make_idesc_few(b_kind, a_kind, b_layout, t);
+    const int split = few_split((n + 127) / 128, (int)((k + 127) / 128));
+    return dispatch_out_dtype(out_dtype, [&](auto* tag) {
+      using OutT = std::remove_pointer_t<decltype(tag)>;
+      auto go = [&](auto t_const) {
+        return launch_block_few<OutT, decltype(t_const)::value>(mb, ma, sb, sa, bias, out, ldo, (int)m, (int)n, (int)k,
+                                                                idesc, b_layout, split, st);
+      };
+      if (t == 16) return go(std::integral_constant<int, 16>{});
+      if (t == 32) return go(std::integral_constant<int, 32>{});
+      if (t == 64) return go(std::integral_constant<int, 64>{});
+      return go(std::integral_constant<int, 128>{});
+    });
+  }
+  rc = a_layout ? gemm::encode_operand_map_mn(&ma, a, m, k, lda) : gemm::encode_operand_map(&ma, a, m, k, lda, 128);
+  if (rc == F8B200_OK)
+    rc = b_layout ? gemm::encode_operand_map_mn(&mb, b, n, k, ldb) : gemm::encode_operand_map(&mb, b, n, k, ldb, 128);
+  if (rc != F8B200_OK) return rc;
+  const uint32_t idesc = gemm::pair::make_idesc_pair(a_kind, b_kind, a_layout, b_layout);
+  return dispatch_out_dtype(out_dtype, [&](auto* tag) {
+    using OutT = std::remove_pointer_t<decltype(tag)>;
+    return b_block_rows == 1
+               ? launch_block_pair<OutT, true>(ma, mb, sa, sb, bias, out, ldo, (int)m, (int)n, (int)k, idesc, vec_ok,
+                                               layouts, st)
+               : launch_block_pair<OutT, false>(ma, mb, sa, sb, bias, out, ldo, (int)m, (int)n, (int)k, idesc, vec_ok,
+                                                layouts, st);
+  });
+}

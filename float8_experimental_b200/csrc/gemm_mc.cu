@@ -25,6 +25,7 @@
 // one arrival per CTA that shares an operand with this one (itself included) and every MMA thread
 // releases a stage with a tcgen05.commit multicast to exactly those CTAs.  Tiles are claimed per
 // cluster by CTA 0 and published to all CTAs of the cluster through their tile rings.
+#define F8B200_MC_LIBRARY 1  // leaves out what gemm.cu includes for libf8b200.so alone
 #include "gemm.cu"
 
 namespace f8b200 {

@@ -1,0 +1,157 @@
+"""float8 with one scale per block of 128: casts, matrix products and the linear layer's products.
+
+Per-tensor scaling (the reference's only kind, float8_experimental/config.py:12-21) lets one large value push
+the rest of its tensor towards the small end of the format.  Here each block of 128 elements has a factor of
+its own.  A block is 1 x 128 (by rows: activations and gradients as a product's left operand), 128 x 1 (by
+columns: the same two in the product of the weight's gradient, where they are summed over rows) or 128 x 128
+(weights, whose bytes then serve a product and its transpose alike).
+
+The cast picks powers of two (`scale_inv = 2^-e`, e the largest whole number that keeps the block's amax within the
+format, amaxes below 1e-12 counting as that), so scaling moves exponents only and rounds nothing.  The product takes
+any fp32 factors, such as those that came with a checkpoint's weights.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _native as N
+from ._ops import _blocks, ops
+from .float8_utils import _kind, e4m3_dtype, e5m2_dtype
+
+__all__ = ["BLOCK", "Float8BlockTensor", "cast_to_float8_blockwise", "cast_to_float8_blockwise_both", "blockwise_mm"]
+
+BLOCK = 128
+_BLOCKS = ((1, BLOCK), (BLOCK, 1), (BLOCK, BLOCK))
+
+
+class Float8BlockTensor:
+    """A matrix held as fp8 bytes and one factor per block: `data[i, j] * scale_inv[i // block[0], j // block[1]]`.
+
+    data       [rows, cols] torch.float8_e4m3fn or float8_e5m2, in either memory order
+    scale_inv  float32 [ceil(rows / block[0]), ceil(cols / block[1])], any strides
+    block      (1, 128), (128, 1) or (128, 128); the last block of a dimension may be shorter
+    orig_dtype the dtype `to_original_precision` returns by default"""
+
+    __slots__ = ("data", "scale_inv", "block", "orig_dtype")
+
+    def __init__(self, data: torch.Tensor, scale_inv: torch.Tensor, block: Tuple[int, int],
+                 orig_dtype: torch.dtype = torch.bfloat16):
+        block = tuple(block)
+        if block not in _BLOCKS:
+            raise ValueError(f"Float8BlockTensor: block must be one of {_BLOCKS}, got {block}")
+        if data.dim() != 2 or data.dtype not in (e4m3_dtype, e5m2_dtype):
+            raise ValueError(f"Float8BlockTensor: data must be a float8 matrix, got {data.dtype} {tuple(data.shape)}")
+        want = tuple(_blocks(size) if b == BLOCK else size for size, b in zip(data.shape, block))
+        if scale_inv.dtype != torch.float32 or tuple(scale_inv.shape) != want:
+            raise ValueError(
+                f"Float8BlockTensor: scale_inv must be float32 {want} for blocks of {block}, got "
+                f"{scale_inv.dtype} {tuple(scale_inv.shape)}"
+            )
+        if scale_inv.device != data.device:
+            raise ValueError(f"Float8BlockTensor: data on {data.device}, scale_inv on {scale_inv.device}")
+        self.data, self.scale_inv, self.block, self.orig_dtype = data, scale_inv, block, orig_dtype
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.data.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.data.device
+
+    def t(self) -> "Float8BlockTensor":
+        """The transposed matrix: the same bytes and factors, nothing copied."""
+        return Float8BlockTensor(self.data.t(), self.scale_inv.t(), self.block[::-1], self.orig_dtype)
+
+    def to_original_precision(self, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        return ops.uncast_blockwise(self.data, self.scale_inv, *self.block, dtype or self.orig_dtype)
+
+    def __repr__(self):
+        return f"Float8BlockTensor({self.data.dtype}, shape={tuple(self.shape)}, block={self.block})"
+
+
+def _matrix(x: torch.Tensor, what: str) -> torch.Tensor:
+    if x.dim() != 2:
+        raise ValueError(f"{what}: takes a matrix, got {x.dim()} dimensions")
+    N.hp_code(x.dtype)  # bf16, fp16 or fp32
+    return x.detach()
+
+
+def cast_to_float8_blockwise(x: torch.Tensor, block: Tuple[int, int] = (1, BLOCK),
+                             float8_dtype: torch.dtype = e4m3_dtype) -> Float8BlockTensor:
+    """`x` [rows, cols] (bf16 / fp16 / fp32) cast with one power-of-two factor per block.  Not differentiable."""
+    block = tuple(block)
+    if block not in _BLOCKS:
+        raise ValueError(f"cast_to_float8_blockwise: block must be one of {_BLOCKS}, got {block}")
+    x, kind = _matrix(x, "cast_to_float8_blockwise"), _kind(float8_dtype)
+    if block == (BLOCK, BLOCK):
+        data, scale = ops.cast_blockwise_square(x, kind)
+    elif block == (1, BLOCK):
+        data, scale, _, _ = ops.cast_blockwise(x, kind, True, False)
+    else:
+        _, _, data, scale = ops.cast_blockwise(x, kind, False, True)
+    return Float8BlockTensor(data, scale, block, x.dtype)
+
+
+def cast_to_float8_blockwise_both(x: torch.Tensor, float8_dtype: torch.dtype = e4m3_dtype
+                                  ) -> Tuple[Float8BlockTensor, Float8BlockTensor]:
+    """`x` cast by rows (1 x 128 blocks) and by columns (128 x 1), from one read of it."""
+    x = _matrix(x, "cast_to_float8_blockwise_both")
+    data, scale, data_c, scale_c = ops.cast_blockwise(x, _kind(float8_dtype), True, True)
+    return (Float8BlockTensor(data, scale, (1, BLOCK), x.dtype), Float8BlockTensor(data_c, scale_c, (BLOCK, 1), x.dtype))
+
+
+def blockwise_mm(a: Float8BlockTensor, b: Float8BlockTensor, out_dtype: torch.dtype = torch.bfloat16,
+                 bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """a [M, K] @ b [K, N] (+ bias [N]), summed in fp32 and rounded once to `out_dtype` (bf16 / fp16 / fp32).
+
+    The blocks must be 128 long in K on both sides: `a` in 1 x 128 or 128 x 128 blocks, `b` in 128 x 1 (the
+    transposed form of 1 x 128) or 128 x 128.  Either operand may lie in either memory order, M, K and N are
+    free, and either may be e4m3 or e5m2."""
+    if not isinstance(a, Float8BlockTensor) or not isinstance(b, Float8BlockTensor):
+        raise TypeError("blockwise_mm: both operands must be Float8BlockTensor")
+    if a.block[1] != BLOCK or b.block[0] != BLOCK:
+        raise ValueError(f"blockwise_mm: blocks must be {BLOCK} long in the inner dimension, got {a.block} and {b.block}")
+    if a.shape[1] != b.shape[0]:
+        raise ValueError(f"blockwise_mm: inner dimensions differ ({a.shape[1]} vs {b.shape[0]})")
+    N.hp_code(out_dtype)
+    return ops.blockwise_mm(a.data, b.data.t(), a.scale_inv, b.scale_inv.t(), a.block[0], b.block[1], bias, out_dtype)
+
+
+@torch._dynamo.allow_in_graph
+class _float8_linear_blockwise(torch.autograd.Function):
+    """Forward and backward of a Float8Linear whose three tensors are scaled by blocks, on raw tensors.
+
+    All three are e4m3: with a factor per 128 elements the gradient needs no wider range, and e5m2 would cost it a
+    bit of precision.  `need_dw` asks the input's cast for the by-column form that the weight's gradient reads."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, need_dw: bool):
+        x2 = x.reshape(-1, x.shape[-1])
+        x8, sx, x8c, sxc = ops.cast_blockwise(x2, N.E4M3, True, need_dw)
+        w8, sw = ops.cast_blockwise_square(weight, N.E4M3)
+        y = ops.blockwise_mm(x8, w8, sx, sw, 1, BLOCK, bias, x.dtype)
+        ctx.save_for_backward(x8c, sxc, w8, sw)
+        ctx.dtypes = (weight.dtype, bias.dtype if bias is not None else None)
+        return y.reshape(*x.shape[:-1], y.shape[-1])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, go):
+        x8c, sxc, w8, sw = ctx.saved_tensors
+        need_dx, need_dw, need_db = ctx.needs_input_grad[:3]
+        go2 = go.reshape(-1, go.shape[-1])
+        dx = dw = db = None
+        if need_dx or need_dw:
+            g8, sg, g8c, sgc = ops.cast_blockwise(go2, N.E4M3, need_dx, need_dw)
+        if need_dx:  # dX = dY @ W: the weight's bytes and factors read transposed
+            dx = ops.blockwise_mm(g8, w8.t(), sg, sw.t(), 1, BLOCK, None, go.dtype)
+            dx = dx.reshape(*go.shape[:-1], dx.shape[-1])
+        if need_dw:  # dW = dY^T @ X, summed over rows: both by columns
+            dw = ops.blockwise_mm(g8c.t(), x8c.t(), sgc.t(), sxc.t(), 1, 1, None, ctx.dtypes[0])
+        if need_db:
+            db = go2.sum(0, dtype=torch.float32).to(ctx.dtypes[1])
+        return dx, dw, db, None

@@ -11,6 +11,7 @@ import torch
 from . import _native as N
 from ._ops import ops
 from .config import Float8LinearConfig, ScalingType
+from .float8_blockwise import _float8_linear_blockwise
 from .float8_scaling_utils import (
     _maybe_initialize_amaxes_scales_for_float8_cast,
     hp_tensor_to_float8_delayed,
@@ -108,7 +109,8 @@ class Float8Linear(torch.nn.Linear):
     """Drop-in for `nn.Linear` (created through `from_float` / `convert_to_float8_training`).
 
     input and weight are cast to e4m3, the gradient of the output to e5m2, each with
-    dynamic or delayed per-tensor scaling as configured."""
+    dynamic or delayed per-tensor scaling as configured; or, with ScalingType.BLOCKWISE for all three, each
+    of them to e4m3 with one scale per block of 128 (`float8_blockwise.py`)."""
 
     def __init__(self, *args, **kwargs):
         """Takes `nn.Linear`'s arguments plus the keyword `config: Float8LinearConfig`."""
@@ -124,6 +126,12 @@ class Float8Linear(torch.nn.Linear):
             self.scaling_type_weight,
             self.scaling_type_grad_output,
         )
+        scaling_types = {self.scaling_type_input, self.scaling_type_weight, self.scaling_type_grad_output}
+        self.blockwise_scaling = ScalingType.BLOCKWISE in scaling_types
+        if self.blockwise_scaling and len(scaling_types) > 1:
+            raise ValueError("ScalingType.BLOCKWISE applies to input, weight and grad_output together")
+        if self.blockwise_scaling and config.enable_fsdp_float8_all_gather:
+            raise ValueError("enable_fsdp_float8_all_gather needs a per-tensor scale: not with ScalingType.BLOCKWISE")
         self.create_buffers()
 
         def mm_cfg(gemm_cfg):
@@ -257,7 +265,18 @@ class Float8Linear(torch.nn.Linear):
         return os.environ.get("F8B200_LINEAR_SINGLE_NODE", "1") != "0" and \
             os.environ.get("F8B200_CAST_TRANSPOSED", "0") != "1"
 
+    def _forward_blockwise(self, input: torch.Tensor) -> torch.Tensor:
+        for name, t in (("input", input), ("weight", self.weight)):
+            if type(t) not in (torch.Tensor, torch.nn.Parameter):
+                raise RuntimeError(f"ScalingType.BLOCKWISE takes plain tensors, got a {type(t).__name__} as {name}")
+        if torch.is_autocast_enabled(input.device.type):
+            input = input.to(torch.get_autocast_dtype(input.device.type))
+        need_dw = torch.is_grad_enabled() and self.weight.requires_grad
+        return _float8_linear_blockwise.apply(input, self.weight, self.bias, need_dw)
+
     def forward(self, input: torch.Tensor) -> torch.Tensor:
+        if self.blockwise_scaling:
+            return self._forward_blockwise(input)
         if self._single_node_route(input):
             output = _float8_linear_dynamic.apply(input, self.weight, self.linear_mm_config)
             if self.bias is not None:

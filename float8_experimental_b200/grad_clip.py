@@ -1,0 +1,106 @@
+"""Norm of all gradients as one vector, and clipping to it: `torch.nn.utils.clip_grad_norm_` in three launches
+(partial sums of every tensor, their sum, the scaling, which the device skips when nothing exceeds the bound) in
+place of several per tensor, and without a host synchronisation.
+
+Gradients of one call lie on one device; bf16, fp16 and fp32 may be mixed.  DTensor gradients (FSDP2, tensor
+parallel) count once over their mesh: the local sums are all-reduced over the mesh dimensions a tensor is
+sharded on.
+"""
+from __future__ import annotations
+
+import math
+from typing import Dict, Iterable, List, Union
+
+import torch
+import torch.distributed as dist
+from torch.distributed._tensor import DTensor
+
+from ._ops import ops
+
+__all__ = ["get_total_norm", "clip_grads_with_norm_", "clip_grad_norm_"]
+
+_KINDS = {math.inf: 0, 1.0: 1, 2.0: 2}
+
+
+def _kind_of(norm_type: float) -> int:
+    kind = _KINDS.get(float(norm_type))
+    if kind is None:
+        raise ValueError(f"norm_type must be 1, 2 or inf, got {norm_type}")
+    return kind
+
+
+def _local(t: torch.Tensor) -> torch.Tensor:
+    return t._local_tensor if isinstance(t, DTensor) else t
+
+
+def _gradients(parameters: Union[torch.Tensor, Iterable[torch.Tensor]]) -> List[torch.Tensor]:
+    """The gradients of `parameters`, each once however often its parameter is listed."""
+    params = [parameters] if isinstance(parameters, torch.Tensor) else parameters
+    found: Dict[int, torch.Tensor] = {}
+    for p in params:
+        if p.grad is not None:
+            found.setdefault(id(p), p.grad)
+    return list(found.values())
+
+
+def _sharded_groups(t: DTensor):
+    """The process groups whose ranks hold different parts of `t`."""
+    groups = []
+    for dim, placement in enumerate(t.placements):
+        if placement.is_shard():
+            groups.append(t.device_mesh.get_group(dim))
+        elif placement.is_partial():
+            raise NotImplementedError("gradient norm of a Partial DTensor")
+    return tuple(groups)
+
+
+@torch.no_grad()
+def get_total_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: float = 2.0,
+                   error_if_nonfinite: bool = False) -> torch.Tensor:
+    """The `norm_type` (1, 2 or inf) norm of all `tensors` together, fp32, 0-dim, on their device.  No tensors: 0.
+
+    Squares are formed in fp32 as in torch: an element beyond 1.8e19 makes the 2-norm infinite."""
+    kind = _kind_of(norm_type)
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    if not tensors:
+        return torch.tensor(0.0)
+    by_groups: Dict[tuple, List[torch.Tensor]] = {}
+    for t in tensors:
+        by_groups.setdefault(_sharded_groups(t) if isinstance(t, DTensor) else (), []).append(_local(t))
+    if set(by_groups) == {()}:
+        total = ops.multi_norm(by_groups[()], kind, True)
+    else:
+        parts = []
+        for groups, local in by_groups.items():
+            part = ops.multi_norm(local, kind, False)
+            for group in groups:
+                dist.all_reduce(part, op=dist.ReduceOp.MAX if kind == 0 else dist.ReduceOp.SUM, group=group)
+            parts.append(part)
+        both = torch.stack(parts)
+        total = both.max() if kind == 0 else both.sum().sqrt() if kind == 2 else both.sum()
+    if error_if_nonfinite and not bool(torch.isfinite(total)):
+        raise RuntimeError(
+            f"The total norm of order {norm_type} for gradients is non-finite, so it cannot be clipped. "
+            "To disable this error and scale the gradients by the non-finite norm anyway, set `error_if_nonfinite=False`"
+        )
+    return total
+
+
+@torch.no_grad()
+def clip_grads_with_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float,
+                          total_norm: torch.Tensor) -> None:
+    """Multiplies every gradient by min(1, max_norm / (total_norm + 1e-6)), in place.  A NaN norm makes them NaN."""
+    grads = [_local(g) for g in _gradients(parameters)]
+    if grads:
+        ops.multi_clip_(grads, total_norm, float(max_norm))
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
+                    error_if_nonfinite: bool = False) -> torch.Tensor:
+    """Clips the gradients of `parameters` to a total norm of at most `max_norm`, in place, and returns the norm they had
+    (fp32, 0-dim, on their device).  `error_if_nonfinite=True` reads it back and synchronises."""
+    params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    total = get_total_norm(_gradients(params), norm_type, error_if_nonfinite)
+    clip_grads_with_norm_(params, max_norm, total)
+    return total

@@ -11,6 +11,8 @@ from typing import Callable, Optional
 import torch
 import torch.nn as nn
 
+from ._ops import ops
+from .float8_blockwise import BLOCK, cast_to_float8_blockwise
 from .float8_linear_utils import swap_linear_layers
 from .float8_tensor import (
     Float8Tensor,
@@ -28,11 +30,15 @@ class ActivationCasting(Enum):
 
     WEIGHT_ONLY  weights stored in fp8, dequantised for a high-precision matmul
     DYNAMIC      activations cast per call with a scale from their own amax
-    STATIC       activations cast per call with a fixed, calibrated scale"""
+    STATIC       activations cast per call with a fixed, calibrated scale
+    BLOCKWISE    activations cast per call with a scale per row and 128 columns, weights with one per 128 x 128
+                 square: `weight` holds the fp8 bytes, the buffer `weight_scale_inv` the squares' factors (any
+                 fp32 values, so a checkpoint that brings both can be loaded into them)"""
 
     WEIGHT_ONLY = auto()
     DYNAMIC = auto()
     STATIC = auto()
+    BLOCKWISE = auto()
 
 
 @dataclass(frozen=True)
@@ -84,6 +90,8 @@ class Float8InferenceLinear(torch.nn.Linear):
             self.static_quantization_scale = None
 
     def forward(self, input: torch.Tensor) -> torch.Tensor:
+        if self.activation_casting == ActivationCasting.BLOCKWISE:
+            return self._forward_blockwise(input)
         if self.activation_casting == ActivationCasting.WEIGHT_ONLY:
             return torch.nn.functional.linear(input, self.weight.to_original_precision())
         x_fp8 = cast_to_float8_e4m3_inference(
@@ -92,9 +100,23 @@ class Float8InferenceLinear(torch.nn.Linear):
         # linear(Float8Tensor, Float8Tensor, bias) lands in the op table's mm / addmm
         return torch.nn.functional.linear(x_fp8, self.weight, self.bias)
 
+    def _forward_blockwise(self, input: torch.Tensor) -> torch.Tensor:
+        if type(input) not in (torch.Tensor, nn.Parameter):
+            raise RuntimeError(f"ActivationCasting.BLOCKWISE takes plain tensors, got a {type(input).__name__}")
+        x8 = cast_to_float8_blockwise(input.reshape(-1, input.shape[-1]))
+        y = ops.blockwise_mm(x8.data, self.weight, x8.scale_inv, self.weight_scale_inv, 1, BLOCK, self.bias, input.dtype)
+        return y.reshape(*input.shape[:-1], y.shape[-1])
+
     def quantize_weight(self, dtype: torch.dtype = e4m3_dtype) -> None:
-        """Replaces the weight by its `Float8Tensor` (dynamic scale), frozen."""
-        assert not isinstance(self.weight, Float8Tensor), "Weight has already been quantized, cannot quantize again."
+        """Replaces the weight by its `Float8Tensor` (dynamic scale), frozen; with ActivationCasting.BLOCKWISE by its
+        fp8 bytes and the buffer `weight_scale_inv`."""
+        assert not isinstance(self.weight, Float8Tensor) and self.weight.element_size() > 1, \
+            "Weight has already been quantized, cannot quantize again."
+        if self.activation_casting == ActivationCasting.BLOCKWISE:
+            w8 = cast_to_float8_blockwise(self.weight, (BLOCK, BLOCK), dtype)
+            self.weight = nn.Parameter(w8.data, requires_grad=False)
+            self.register_buffer("weight_scale_inv", w8.scale_inv)
+            return
         with torch.no_grad():
             scale = tensor_to_scale(self.weight, dtype)
             w8 = hp_tensor_and_scale_to_float8(

@@ -400,6 +400,85 @@ int f8b200_swiglu_bwd_approx(const void* a, const void* b, const void* grad_y, i
                              int64_t ld_out, void* stream);
 
 /*
+ * fp8 with one factor per block of 128.  A block is 1 x 128 (by rows), 128 x 1 (by columns) or 128 x 128; the
+ * last block of a dimension may be shorter.  With a = max(max|x| over the block, 1e-12) and e the largest whole
+ * number with a * 2^e <= the format's maximum:  q = fp8(x * 2^e) (nearest even), scale_inv = 2^-e, and the block
+ * stands for q * scale_inv.  Scaling by a power of two rounds nothing.  A block that holds an infinity or a NaN becomes
+ * NaN throughout, its factor too.  No reference counterpart (the reference scales whole tensors).
+ *
+ * f8b200_cast_blockwise   x [rows, cols], row pitch ld_x, read once:
+ *     out_r (may be NULL)   by rows: bytes with row pitch ld_r; the factor of (row r, block j) at
+ *                           scale_r[j * ld_scale_r + r], ld_scale_r >= rows;
+ *     out_c (may be NULL)   by columns: bytes [rows, cols] with row pitch ld_c; the factor of (block i, column c) at
+ *                           scale_c[i * ld_scale_c + c], ld_scale_c >= cols;
+ *     by_square != 0        out_r in 128 x 128 blocks instead, the factor of (i, j) at scale_r[i * ld_scale_r + j],
+ *                           ld_scale_r >= ceil(cols / 128); out_c must be NULL.
+ * f8b200_uncast_blockwise y = RN_T(q * scale), the factor of a block (i, j) of block_rows x block_cols (1 or 128 each)
+ *                         at scale[i * scale_row_stride + j * scale_col_stride].
+ * Empty matrices return F8B200_OK without a launch.
+ */
+int f8b200_cast_blockwise(const void* x, int hp_dtype, int64_t rows, int64_t cols, int64_t ld_x,
+                          int fp8_kind, int by_square, void* out_r, int64_t ld_r, float* scale_r,
+                          int64_t ld_scale_r, void* out_c, int64_t ld_c, float* scale_c,
+                          int64_t ld_scale_c, void* stream);
+int f8b200_uncast_blockwise(const void* q, int fp8_kind, int64_t rows, int64_t cols, int64_t ld_q,
+                            const float* scale, int64_t scale_row_stride, int64_t scale_col_stride,
+                            int block_rows, int block_cols, int hp_dtype, void* y, int64_t ld_y,
+                            void* stream);
+
+/*
+ * out[m, n] = sum_j sa(m, j) * sb(n, j) * (sum of A[m, k] * B[n, k] over k in block j)  (+ bias[n])
+ * with blocks of 128 along K, fp32 sums, one rounding to out_dtype.  Operands, layouts, pitches and alignment as in
+ * f8b200_gemm_fp8_ws; K may be any number, the last block being shorter.  The factor of A's row m and block j lies
+ * at scale_a[(m / a_block_rows) * sa_row_stride + j * sa_kb_stride], a_block_rows 1 or 128, strides >= 0
+ * (elements); B's likewise.  Factors are arbitrary fp32 values.  `bias` has out_dtype or is NULL.  Needs no workspace.
+ */
+int f8b200_gemm_blockwise(const void* a, int a_kind, int a_layout, int64_t lda, const float* scale_a,
+                          int64_t sa_row_stride, int64_t sa_kb_stride, int a_block_rows, const void* b,
+                          int b_kind, int b_layout, int64_t ldb, const float* scale_b,
+                          int64_t sb_row_stride, int64_t sb_kb_stride, int b_block_rows,
+                          const void* bias, int out_dtype, void* out, int64_t ldo, int64_t m, int64_t n,
+                          int64_t k, void* stream);
+
+/*
+ * Layer norm over the columns of x [rows, cols], T = hp_dtype:
+ *   n = (x - mean) * rstd,  rstd = 1 / sqrt(mean of (x - mean)^2 + eps),  y = RN_T(n * weight + bias)
+ * in fp32.  weight and bias [cols] have affine_dtype (hp_dtype or FP32); either may be NULL (1 and 0).
+ * mean_out and rstd_out [rows] are both given or both NULL.
+ *
+ * f8b200_layer_norm_bwd  from x, grad_y and the saved mean and rstd, with h = grad_y * weight:
+ *   dx      = RN_T(rstd * (h - mean(h) - n * mean(h * n)))     row pitch ld_dx; may be NULL
+ *   dweight = RN(sum over rows of grad_y * n), dbias = RN(sum over rows of grad_y)   affine_dtype; may be NULL
+ * `workspace`: at least f8b200_layer_norm_bwd_workspace_bytes(cols) bytes, 16-byte aligned, for partial sums (no
+ * initialisation needed); NULL when neither dweight nor dbias is asked for.  Sums run in a fixed order.
+ */
+int f8b200_layer_norm(const void* x, int hp_dtype, int64_t rows, int64_t cols, int64_t ld_x,
+                      const void* weight, const void* bias, int affine_dtype, float eps, void* y,
+                      int64_t ld_y, float* mean_out, float* rstd_out, void* stream);
+int64_t f8b200_layer_norm_bwd_workspace_bytes(int64_t cols);
+int f8b200_layer_norm_bwd(const void* x, const void* grad_y, int hp_dtype, int64_t rows, int64_t cols,
+                          int64_t ld_x, int64_t ld_g, const void* weight, int affine_dtype,
+                          const float* mean, const float* rstd, void* dx, int64_t ld_dx, void* dweight,
+                          void* dbias, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Norm of n tensors taken as one vector, and their scaling.  `ptrs` (device addresses), `numels` and `hp_dtypes` are
+ * HOST arrays; each tensor is numels[i] contiguous elements of type hp_dtypes[i]; empty ones are skipped.
+ *
+ * f8b200_multi_norm  out[0] = (sum |x|^kind)^(1/kind) for kind 1 and 2, max |x| for kind 0 (NaN if any element is);
+ *                    with root == 0 the sum of powers itself (kind 2).  `workspace`: at least
+ *                    f8b200_multi_norm_workspace_bytes(numels, n) bytes, 8-byte aligned.  Sums run in a fixed order.
+ * f8b200_multi_clip  x = RN(x * f), f = min(1, max_norm / (total_norm[0] + 1e-6)), in place; nothing is touched when
+ *                    f == 1.  The tensors must not overlap.
+ */
+int64_t f8b200_multi_norm_workspace_bytes(const int64_t* numels, int n);
+int f8b200_multi_norm(const void* const* ptrs, const int64_t* numels, const int* hp_dtypes, int n,
+                      int kind, int root, float* out, void* workspace, int64_t workspace_bytes,
+                      void* stream);
+int f8b200_multi_clip(void* const* ptrs, const int64_t* numels, const int* hp_dtypes, int n,
+                      const float* total_norm, float max_norm, void* stream);
+
+/*
  * Reads and clears the device error word of the current device (synchronises the
  * device).  *flags_out != 0 means a bounded wait inside a kernel gave up since the
  * last read; the result of that launch is undefined.  Test and debugging aid.
