@@ -50,6 +50,7 @@ EXPORTS = (
     "f8b200_rmsnorm_bwd",
     "f8b200_swiglu_bwd",
     "f8b200_swiglu_bwd_approx",
+    "f8b200_block_exponent_bytes",
     "f8b200_cast_blockwise",
     "f8b200_uncast_blockwise",
     "f8b200_gemm_blockwise",
@@ -119,10 +120,12 @@ def load() -> ctypes.CDLL:
     lib.f8b200_gemm_fp8_scatter_rows.argtypes = [vp, i32, i32, i64, vp, i32, i32, i64, vp, vp, vp, i32, ctypes.POINTER(vp),
                                                  i32, i64, i64, i64, i64, i64, vp, i64, vp]
     lib.f8b200_sum_slots.argtypes = [vp, i32, i64, i32, i64, vp, vp]
-    lib.f8b200_cast_blockwise.argtypes = [vp, i32, i64, i64, i64, i32, i32, vp, i64, vp, i64, vp, i64, vp, i64, vp]
+    lib.f8b200_cast_blockwise.argtypes = [vp, i32, i64, i64, i64, i32, i32, vp, i64, vp, i64, vp, vp, i64, vp, i64, vp, vp]
+    lib.f8b200_block_exponent_bytes.argtypes = [i64, i64]
+    lib.f8b200_block_exponent_bytes.restype = i64
     lib.f8b200_uncast_blockwise.argtypes = [vp, i32, i64, i64, i64, vp, i64, i64, i32, i32, i32, vp, i64, vp]
-    lib.f8b200_gemm_blockwise.argtypes = [vp, i32, i32, i64, vp, i64, i64, i32, vp, i32, i32, i64, vp, i64, i64, i32, vp, i32,
-                                          vp, i64, i64, i64, i64, vp]
+    lib.f8b200_gemm_blockwise.argtypes = [vp, i32, i32, i64, vp, i64, i64, i32, vp, vp, i32, i32, i64, vp, i64, i64, i32, vp,
+                                          vp, i32, vp, i64, i64, i64, i64, vp]
     lib.f8b200_layer_norm.argtypes = [vp, i32, i64, i64, i64, vp, vp, i32, ctypes.c_float, vp, i64, vp, vp, vp]
     lib.f8b200_layer_norm_bwd_workspace_bytes.argtypes = [i64]
     lib.f8b200_layer_norm_bwd_workspace_bytes.restype = i64
@@ -589,13 +592,14 @@ def swiglu_bwd(a: torch.Tensor, b: torch.Tensor, g: torch.Tensor, rows: int, col
 
 def cast_blockwise(x: torch.Tensor, rows: int, cols: int, ld_x: int, fp8_kind: int, by_square: bool,
                    out_r: Optional[torch.Tensor], ld_r: int, scale_r: Optional[torch.Tensor], ld_scale_r: int,
-                   out_c: Optional[torch.Tensor], ld_c: int, scale_c: Optional[torch.Tensor], ld_scale_c: int) -> None:
-    _require_cuda(x, out_r, scale_r, out_c, scale_c)
+                   exp_r: Optional[torch.Tensor], out_c: Optional[torch.Tensor], ld_c: int,
+                   scale_c: Optional[torch.Tensor], ld_scale_c: int, exp_c: Optional[torch.Tensor]) -> None:
+    _require_cuda(x, out_r, scale_r, exp_r, out_c, scale_c, exp_c)
     with _Launch("cast_block", x.device):
         _check(
             load().f8b200_cast_blockwise(x.data_ptr(), hp_code(x.dtype), rows, cols, ld_x, fp8_kind, int(by_square),
-                                         _ptr(out_r), ld_r, _ptr(scale_r), ld_scale_r, _ptr(out_c), ld_c, _ptr(scale_c),
-                                         ld_scale_c, _stream(x)),
+                                         _ptr(out_r), ld_r, _ptr(scale_r), ld_scale_r, _ptr(exp_r), _ptr(out_c), ld_c,
+                                         _ptr(scale_c), ld_scale_c, _ptr(exp_c), _stream(x)),
             "f8b200_cast_blockwise",
         )
 
@@ -613,15 +617,15 @@ def uncast_blockwise(q: torch.Tensor, rows: int, cols: int, ld_q: int, scale: to
 
 
 def gemm_blockwise(a: torch.Tensor, lda: int, a_mn_major: bool, scale_a: torch.Tensor, a_block_rows: int,
-                   b: torch.Tensor, ldb: int, b_mn_major: bool, scale_b: torch.Tensor, b_block_rows: int,
-                   bias: Optional[torch.Tensor], out: torch.Tensor, ldo: int, m: int, n: int, k: int) -> None:
-    _require_cuda(a, b, scale_a, scale_b, bias, out)
+                   exp_a: Optional[torch.Tensor], b: torch.Tensor, ldb: int, b_mn_major: bool, scale_b: torch.Tensor,
+                   b_block_rows: int, exp_b: Optional[torch.Tensor], bias: Optional[torch.Tensor], out: torch.Tensor, ldo: int, m: int, n: int, k: int) -> None:
+    _require_cuda(a, b, scale_a, scale_b, exp_a, exp_b, bias, out)
     with _Launch("gemm_block", a.device):
         _check(
             load().f8b200_gemm_blockwise(a.data_ptr(), fp8_code(a.dtype), int(a_mn_major), lda, scale_a.data_ptr(),
-                                         scale_a.stride(0), scale_a.stride(1), a_block_rows, b.data_ptr(),
+                                         scale_a.stride(0), scale_a.stride(1), a_block_rows, _ptr(exp_a), b.data_ptr(),
                                          fp8_code(b.dtype), int(b_mn_major), ldb, scale_b.data_ptr(), scale_b.stride(0),
-                                         scale_b.stride(1), b_block_rows, _ptr(bias), hp_code(out.dtype), out.data_ptr(),
+                                         scale_b.stride(1), b_block_rows, _ptr(exp_b), _ptr(bias), hp_code(out.dtype), out.data_ptr(),
                                          ldo, m, n, k, _stream(a)),
             "f8b200_gemm_blockwise",
         )

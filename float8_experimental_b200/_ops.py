@@ -20,10 +20,12 @@ Ops (namespace `f8b200`):
   rmsnorm_cast(x, weight, rstd, amax, kind) -> (data, scale)               f8b200_rmsnorm_cast
   swiglu_amax(a, b, write_y, approx) -> (amax fp32 0-dim, y or empty)      f8b200_swiglu_amax[_approx]
   swiglu_cast(a, b, amax, kind) -> (data, scale)                           f8b200_swiglu_cast
-  cast_blockwise(x, kind, by_row, by_col) -> (data, scale_inv, data_c, scale_inv_c)   f8b200_cast_blockwise
-  cast_blockwise_square(x, kind) -> (data, scale_inv)                      f8b200_cast_blockwise, 128 x 128 blocks
+  cast_blockwise(x, kind, by_row, by_col) -> (data, scale_inv, exps, data_c, scale_inv_c, exps_c)
+                                                                           f8b200_cast_blockwise
+  cast_blockwise_square(x, kind) -> (data, scale_inv, exps, exps_t)        f8b200_cast_blockwise, 128 x 128 blocks
   uncast_blockwise(q, scale_inv, block_rows, block_cols, dtype) -> y       f8b200_uncast_blockwise
-  blockwise_mm(a, b_t, scale_a, scale_b, a_block_rows, b_block_rows, bias, out_dtype) -> out   f8b200_gemm_blockwise
+  blockwise_mm(a, b_t, scale_a, scale_b, a_block_rows, b_block_rows, exp_a, exp_b, bias, out_dtype) -> out
+                                                                           f8b200_gemm_blockwise
   layer_norm(x, weight, bias, eps, save_stats) -> (y, mean, rstd)          f8b200_layer_norm
   layer_norm_bwd(x, grad_y, weight, mean, rstd, affine_dtype, need_dx, need_dw, need_db) -> (dx, dw, db)
   multi_norm(xs, kind, root) -> fp32 0-dim                                 f8b200_multi_norm
@@ -64,12 +66,13 @@ _lib.define("swiglu_amax(Tensor a, Tensor b, bool write_y, bool approx=False) ->
 _lib.define("rmsnorm_bwd(Tensor x, Tensor grad_y, Tensor weight, Tensor rstd) -> (Tensor, Tensor)")
 _lib.define("swiglu_bwd(Tensor a, Tensor b, Tensor grad_y, bool approx=False) -> (Tensor, Tensor)")
 _lib.define("swiglu_cast(Tensor a, Tensor b, Tensor amax, int fp8_kind) -> (Tensor, Tensor)")
-_lib.define("cast_blockwise(Tensor x, int fp8_kind, bool by_row, bool by_col) -> (Tensor, Tensor, Tensor, Tensor)")
-_lib.define("cast_blockwise_square(Tensor x, int fp8_kind) -> (Tensor, Tensor)")
+_lib.define("cast_blockwise(Tensor x, int fp8_kind, bool by_row, bool by_col) -> "
+            "(Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)")
+_lib.define("cast_blockwise_square(Tensor x, int fp8_kind) -> (Tensor, Tensor, Tensor, Tensor)")
 _lib.define("uncast_blockwise(Tensor q, Tensor scale_inv, int block_rows, int block_cols, ScalarType dtype) -> Tensor")
 _lib.define(
     "blockwise_mm(Tensor a, Tensor b_t, Tensor scale_a, Tensor scale_b, int a_block_rows, int b_block_rows, "
-    "Tensor? bias, ScalarType out_dtype) -> Tensor"
+    "Tensor? exp_a, Tensor? exp_b, Tensor? bias, ScalarType out_dtype) -> Tensor"
 )
 _lib.define(
     "layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps, bool save_stats) -> (Tensor, Tensor, Tensor)"
@@ -305,6 +308,11 @@ def _empty_fp8_matrix(rows: int, cols: int, fp8_kind: int, device) -> torch.Tens
     return torch.empty((rows, _pitch16(cols)), dtype=N.FP8_DTYPE[fp8_kind], device=device)[:, :cols]
 
 
+def _exponent_bytes(rows: int, k: int) -> int:
+    """f8b200_block_exponent_bytes: four k-blocks to a word, the rows rounded up to a tile of 256."""
+    return -(-rows // 256) * 1024 * -(-k // 512)
+
+
 def _cast_blockwise_cuda(x, fp8_kind: int, by_row: bool, by_col: bool):
     if x.dim() != 2 or not (by_row or by_col):
         raise RuntimeError("cast_blockwise: takes a matrix and at least one of by_row, by_col")
@@ -317,11 +325,13 @@ def _cast_blockwise_cuda(x, fp8_kind: int, by_row: bool, by_col: bool):
     # one factor per (block, row) resp. (block, column): the GEMM's lanes read neighbouring rows
     scale = torch.empty((_blocks(cols), rows), dtype=torch.float32, device=x.device) if by_row else none32
     scale_c = torch.empty((_blocks(rows), cols), dtype=torch.float32, device=x.device) if by_col else none32
+    exps = torch.empty(_exponent_bytes(rows, cols) if by_row else 0, dtype=torch.uint8, device=x.device)
+    exps_c = torch.empty(_exponent_bytes(cols, rows) if by_col else 0, dtype=torch.uint8, device=x.device)
     if x.numel():
-        N.cast_blockwise(xm, rows, cols, ld, fp8_kind, False, data if by_row else None, data.stride(0),
-                         scale if by_row else None, rows, data_c if by_col else None, data_c.stride(0),
-                         scale_c if by_col else None, cols)
-    return data, scale.t(), data_c, scale_c
+        r = (data, data.stride(0), scale, rows, exps) if by_row else (None, 0, None, 0, None)
+        c = (data_c, data_c.stride(0), scale_c, cols, exps_c) if by_col else (None, 0, None, 0, None)
+        N.cast_blockwise(xm, rows, cols, ld, fp8_kind, False, *r, *c)
+    return data, scale.t(), exps, data_c, scale_c, exps_c
 
 
 def _cast_blockwise_square_cuda(x, fp8_kind: int):
@@ -331,9 +341,12 @@ def _cast_blockwise_square_cuda(x, fp8_kind: int):
     rows, cols = x.shape
     data = _empty_fp8_matrix(rows, cols, fp8_kind, x.device)
     scale = torch.empty((_blocks(rows), _blocks(cols)), dtype=torch.float32, device=x.device)
+    exps, exps_t = (torch.empty(_exponent_bytes(r, c), dtype=torch.uint8, device=x.device)
+                    for r, c in ((rows, cols), (cols, rows)))
     if x.numel():
-        N.cast_blockwise(xm, rows, cols, ld, fp8_kind, True, data, data.stride(0), scale, scale.shape[1], None, 0, None, 0)
-    return data, scale
+        N.cast_blockwise(xm, rows, cols, ld, fp8_kind, True, data, data.stride(0), scale, scale.shape[1], exps,
+                         None, 0, None, 0, exps_t)
+    return data, scale, exps, exps_t
 
 
 def _uncast_blockwise_cuda(q, scale_inv, block_rows: int, block_cols: int, dtype):
@@ -349,8 +362,8 @@ def _uncast_blockwise_cuda(q, scale_inv, block_rows: int, block_cols: int, dtype
     return y
 
 
-def _blockwise_mm_cuda(a, b_t, scale_a, scale_b, a_block_rows: int, b_block_rows: int, bias, out_dtype):
-    _one_device("blockwise_mm", a, b_t, scale_a, scale_b, bias)
+def _blockwise_mm_cuda(a, b_t, scale_a, scale_b, a_block_rows: int, b_block_rows: int, exp_a, exp_b, bias, out_dtype):
+    _one_device("blockwise_mm", a, b_t, scale_a, scale_b, exp_a, exp_b, bias)
     m, k = a.shape
     n, k2 = b_t.shape
     if k != k2:
@@ -359,6 +372,9 @@ def _blockwise_mm_cuda(a, b_t, scale_a, scale_b, a_block_rows: int, b_block_rows
         want = (_blocks(rows) if block == 128 else rows, _blocks(k))
         if s.dtype != torch.float32 or tuple(s.shape) != want:
             raise RuntimeError(f"blockwise_mm: {name} must be float32 {want}, got {s.dtype} {tuple(s.shape)}")
+    for name, e, rows in (("exp_a", exp_a, m), ("exp_b", exp_b, n)):
+        if e is not None and (e.dtype != torch.uint8 or not e.is_contiguous() or e.numel() != _exponent_bytes(rows, k)):
+            raise RuntimeError(f"blockwise_mm: {name} must be the {_exponent_bytes(rows, k)} exponent bytes of its cast")
     if bias is not None and tuple(bias.shape) != (n,):
         raise RuntimeError(f"blockwise_mm: the bias must have {n} elements, got {tuple(bias.shape)}")
     if bias is not None:
@@ -370,7 +386,8 @@ def _blockwise_mm_cuda(a, b_t, scale_a, scale_b, a_block_rows: int, b_block_rows
         return out.zero_() if bias is None else out.copy_(bias)
     a, lda, a_mn = _gemm_operand(a)
     b_t, ldb, b_mn = _gemm_operand(b_t)
-    N.gemm_blockwise(a, lda, a_mn, scale_a, a_block_rows, b_t, ldb, b_mn, scale_b, b_block_rows, bias, out, n, m, n, k)
+    N.gemm_blockwise(a, lda, a_mn, scale_a, a_block_rows, exp_a, b_t, ldb, b_mn, scale_b, b_block_rows, exp_b, bias, out, n,
+                     m, n, k)
     return out
 
 
@@ -576,14 +593,17 @@ def _cast_blockwise_fake(x, fp8_kind, by_row, by_col):
 
     scale = x.new_empty((_blocks(cols), rows) if by_row else (0, 0), dtype=torch.float32)
     scale_c = x.new_empty((_blocks(rows), cols) if by_col else (0, 0), dtype=torch.float32)
-    return data(by_row), scale.t(), data(by_col), scale_c
+    exps = x.new_empty((_exponent_bytes(rows, cols) if by_row else 0,), dtype=torch.uint8)
+    exps_c = x.new_empty((_exponent_bytes(cols, rows) if by_col else 0,), dtype=torch.uint8)
+    return data(by_row), scale.t(), exps, data(by_col), scale_c, exps_c
 
 
 @torch.library.register_fake("f8b200::cast_blockwise_square")
 def _cast_blockwise_square_fake(x, fp8_kind):
     rows, cols = x.shape
     data = x.new_empty((rows, _pitch16(cols)), dtype=N.FP8_DTYPE[fp8_kind])[:, :cols]
-    return data, x.new_empty((_blocks(rows), _blocks(cols)), dtype=torch.float32)
+    exps, exps_t = (x.new_empty((_exponent_bytes(r, c),), dtype=torch.uint8) for r, c in ((rows, cols), (cols, rows)))
+    return data, x.new_empty((_blocks(rows), _blocks(cols)), dtype=torch.float32), exps, exps_t
 
 
 @torch.library.register_fake("f8b200::uncast_blockwise")
@@ -592,7 +612,7 @@ def _uncast_blockwise_fake(q, scale_inv, block_rows, block_cols, dtype):
 
 
 @torch.library.register_fake("f8b200::blockwise_mm")
-def _blockwise_mm_fake(a, b_t, scale_a, scale_b, a_block_rows, b_block_rows, bias, out_dtype):
+def _blockwise_mm_fake(a, b_t, scale_a, scale_b, a_block_rows, b_block_rows, exp_a, exp_b, bias, out_dtype):
     return a.new_empty((a.shape[0], b_t.shape[0]), dtype=out_dtype)
 
 

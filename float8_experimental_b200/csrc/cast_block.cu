@@ -26,8 +26,18 @@ struct BlockCastArgs {
   int64_t ld_r, ld_c;
   float *scale_r, *scale_c;
   int64_t ld_scale_r, ld_scale_c;
+  uint8_t *exp_r, *exp_c;  // the factors' exponents as the tensor cores read them (see exponent_at); may be null
+  int64_t exp_pitch_r, exp_pitch_c;
   int64_t tiles_k;
 };
+
+// Where the exponent byte of operand row `row` and block `kb` of the reduction lies: four blocks make one 32-bit
+// word, 128 rows make 512 bytes in which row r has the word (r % 32) * 4 + r / 32 -- the order in which
+// tcgen05.cp takes 32 x 16 bytes into tensor memory.  `pitch`: bytes of all rows (a multiple of 1024).
+__device__ __forceinline__ int64_t exponent_at(int64_t row, int64_t kb, int64_t pitch) {
+  return (kb >> 2) * pitch + (row >> 7) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (kb & 3);
+}
+__device__ __forceinline__ uint8_t exponent_of(float down) { return (uint8_t)((__float_as_uint(down) >> 23) & 0xFFu); }
 
 // up = 2^e and down = 2^-e of a block whose amax has these fp32 bits
 template <int KIND>
@@ -153,6 +163,11 @@ __global__ void __launch_bounds__(kThreads) cast_block_kernel(const BlockCastArg
     float down;
     block_scale<KIND>(m, up_sq, down);
     if (threadIdx.x == 0) p.scale_r[tm * p.ld_scale_r + tk] = down;
+    if (p.exp_r != nullptr) {  // one factor for 128 rows of the matrix and of its transpose
+      const int t = threadIdx.x & 127;
+      if (threadIdx.x < 128) p.exp_r[exponent_at(row0 + t, tk, p.exp_pitch_r)] = exponent_of(down);
+      else p.exp_c[exponent_at(tk * kBlk + t, tm, p.exp_pitch_c)] = exponent_of(down);
+    }
   }
 
   if constexpr (FORMS & (kByRow | kBySquare)) {
@@ -166,7 +181,10 @@ __global__ void __launch_bounds__(kThreads) cast_block_kernel(const BlockCastArg
         for (int off = 8; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, off));
         float down;
         block_scale<KIND>(m, up, down);
-        if (tx == 0 && r < p.rows) p.scale_r[tk * p.ld_scale_r + r] = down;
+        if (tx == 0 && r < p.rows) {
+          p.scale_r[tk * p.ld_scale_r + r] = down;
+          if (p.exp_r != nullptr) p.exp_r[exponent_at(r, tk, p.exp_pitch_r)] = exponent_of(down);
+        }
       }
       uint32_t w[4];
 #pragma unroll
@@ -183,7 +201,10 @@ __global__ void __launch_bounds__(kThreads) cast_block_kernel(const BlockCastArg
       for (int w = 0; w < kThreads / 32; ++w) m = max(m, col_max[w][tx * 8 + j]);
       float down;
       block_scale<KIND>(m, up[j], down);
-      if (ty == 0 && j < n) p.scale_c[tm * p.ld_scale_c + col + j] = down;
+      if (ty == 0 && j < n) {
+        p.scale_c[tm * p.ld_scale_c + col + j] = down;
+        if (p.exp_c != nullptr) p.exp_c[exponent_at(col + j, tm, p.exp_pitch_c)] = exponent_of(down);
+      }
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -294,12 +315,20 @@ bool aligned(const void* p, int64_t to) { return p == nullptr || reinterpret_cas
 
 using namespace f8b200;
 
+static int64_t exponent_pitch(int64_t rows) { return (rows + 255) / 256 * 256 * 4; }
+
+extern "C" int64_t f8b200_block_exponent_bytes(int64_t rows, int64_t k) {
+  return rows <= 0 || k <= 0 ? 0 : exponent_pitch(rows) * ((k + 511) / 512);
+}
+
 extern "C" int f8b200_cast_blockwise(const void* x, int hp_dtype, int64_t rows, int64_t cols, int64_t ld_x, int fp8_kind,
                                      int by_square, void* out_r, int64_t ld_r, float* scale_r, int64_t ld_scale_r,
-                                     void* out_c, int64_t ld_c, float* scale_c, int64_t ld_scale_c, void* stream) {
+                                     void* exp_r, void* out_c, int64_t ld_c, float* scale_c, int64_t ld_scale_c,
+                                     void* exp_c, void* stream) {
   if (hp_dtype < 0 || hp_dtype > 2 || fp8_kind < 0 || fp8_kind > 1 || rows < 0 || cols < 0) return F8B200_ERR_BAD_ARG;
   if (out_r == nullptr && out_c == nullptr) return F8B200_ERR_BAD_ARG;
-  if (by_square != 0 && (out_r == nullptr || out_c != nullptr)) return F8B200_ERR_BAD_ARG;
+  if (by_square != 0 && (out_r == nullptr || out_c != nullptr || (exp_r == nullptr) != (exp_c == nullptr))) return F8B200_ERR_BAD_ARG;
+  if ((exp_r != nullptr && out_r == nullptr) || (exp_c != nullptr && out_c == nullptr && by_square == 0)) return F8B200_ERR_BAD_ARG;
   if (rows == 0 || cols == 0) return F8B200_OK;
   const int64_t tiles_m = (rows + kBlk - 1) / kBlk, tiles_k = (cols + kBlk - 1) / kBlk;
   if (x == nullptr || ld_x < cols) return F8B200_ERR_BAD_ARG;
@@ -307,7 +336,7 @@ extern "C" int f8b200_cast_blockwise(const void* x, int hp_dtype, int64_t rows, 
   if (out_c != nullptr && (scale_c == nullptr || ld_c < cols || ld_scale_c < cols)) return F8B200_ERR_BAD_ARG;
   if (tiles_m > 0x7FFFFFFFLL / tiles_k) return F8B200_ERR_UNSUPPORTED;
   const int es = hp_size_of(hp_dtype);
-  if (!aligned(x, es) || !aligned(scale_r, 4) || !aligned(scale_c, 4)) return F8B200_ERR_ALIGNMENT;
+  if (!aligned(x, es) || !aligned(scale_r, 4) || !aligned(scale_c, 4) || !aligned(exp_r, 16) || !aligned(exp_c, 16)) return F8B200_ERR_ALIGNMENT;
   int rc = f8b200_device_check();
   if (rc != F8B200_OK) return rc;
   BlockCastArgs p;
@@ -317,6 +346,8 @@ extern "C" int f8b200_cast_blockwise(const void* x, int hp_dtype, int64_t rows, 
   p.ld_r = ld_r, p.ld_c = ld_c;
   p.scale_r = scale_r, p.scale_c = scale_c;
   p.ld_scale_r = ld_scale_r, p.ld_scale_c = ld_scale_c;
+  p.exp_r = static_cast<uint8_t*>(exp_r), p.exp_c = static_cast<uint8_t*>(exp_c);
+  p.exp_pitch_r = exponent_pitch(rows), p.exp_pitch_c = exponent_pitch(cols);
   p.tiles_k = tiles_k;
   const int forms = by_square ? kBySquare : (out_r != nullptr ? kByRow : 0) | (out_c != nullptr ? kByCol : 0);
   // whole 8-element chunks, loaded in 16-byte words and stored in 8-byte ones

@@ -505,6 +505,290 @@ gemm_block_few_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
   if (split > 1) cluster_sync_all();  // no CTA leaves while another may still read its sums
 }
 
+// ---------------------------------------------------------------------------------------------------
+// Factors that are powers of two: the tensor cores apply them.  tcgen05.mma.kind::mxf8f6f4.block_scale multiplies the
+// products of 32 consecutive k by 2^(ea + eb - 254), one exponent byte per operand row and 32 k, read from tensor
+// memory; a block of 128 is four such steps with the same byte, so the accumulator stays in tensor memory over all
+// of K and the epilogue runs once per tile, as in the kernels with one factor per tensor.
+//
+// Tensor memory (512 columns): two accumulators of 256 columns that share 64 of them, at 0 and 192, and the
+// factors at 448.  The epilogue reads the shared columns first and then lets the next tile's MMAs start, which go to
+// the other accumulator, while it drains the rest.
+// Factors: one 32-bit word per operand row holds four k-blocks' bytes.  Every fourth k-block brings 128 words of A
+// (this CTA's rows) and 256 of B (the pair's) along by TMA, tcgen05.cp takes them to tensor memory, and the
+// instruction descriptor says which byte the MMA uses.  Two sets of them alternate.
+// ---------------------------------------------------------------------------------------------------
+constexpr int XTHREADS = 192;  // TMA warp, MMA warp, 4 epilogue warps
+constexpr int XSTAGES = 5;
+constexpr int XSF_A = 512, XSF_B = 1024;  // bytes of factors per CTA and four k-blocks
+constexpr int XSTAGE_BYTES = PA_BYTES + PB_BYTES;
+constexpr int XACC_STEP = 192, XSF_COL = 448, XSF_SET = 16;
+
+struct __align__(16) ScaledBars {
+  uint64_t full[XSTAGES];
+  uint64_t empty[XSTAGES];
+  uint64_t tmem_full[2];
+  uint64_t tmem_shared_free;  // in the leader: 8 arrivals, the shared columns have been read
+  uint32_t tmem_base;
+  volatile uint32_t abort_flag;
+};
+constexpr int XSMEM_BYTES = XSTAGES * (XSTAGE_BYTES + 2048) + EPI_STAGING_BYTES + 1024 + (int)sizeof(ScaledBars);
+
+__device__ __forceinline__ void tc_mma_mx_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
+                                               uint32_t tmem_sa, uint32_t tmem_sb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+          tmem_d),
+      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate)
+      : "memory");
+}
+// 512 bytes of shared memory, as 32 rows of 16, to 4 columns of tensor memory, repeated in the four lane quarters, in
+// both CTAs of the pair from the same offset of their own shared memory
+__device__ __forceinline__ void tc_copy_factors_pair(uint32_t taddr, uint32_t smem_addr) {
+  uint64_t d = 0;  // no swizzle; groups of eight 16-byte rows are 128 bytes apart
+  d |= (uint64_t)((smem_addr & 0x3FFFFu) >> 4);
+  d |= (uint64_t)(128 >> 4) << 16;
+  d |= (uint64_t)(128 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+}
+
+// Bits of the kind::mxf8f6f4 instruction descriptor: B's and A's factor byte at 4 and 29, formats at 7 and 10, MN-major
+// at 15 and 16, N / 8 at 17, 8-bit exponent factors at 23, M / 16 at 24.
+static uint32_t make_idesc_scaled(int a_kind, int b_kind, int a_mn, int b_mn) {
+  return ((uint32_t)a_kind << 7) | ((uint32_t)b_kind << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
+         ((uint32_t)(PBN >> 3) << 17) | (1u << 23) | ((uint32_t)(PBM >> 4) << 24);
+}
+
+// 64 accumulator columns of this warp's 32 rows, already in registers, to the output.
+template <typename OutT>
+__device__ __forceinline__ void store_columns(const EpilogueArgs<OutT>& e, const uint32_t (&r)[2][32], int row0, int col,
+                                              uint32_t& boxes) {
+  constexpr int COLS_PER_BOX = 128 / (int)sizeof(OutT);
+  const int lane = threadIdx.x & 31, row = row0 + lane;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int c0 = col + 32 * h, ncols = min(32, e.n - c0);
+    float v[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[h][i]);
+    if (e.bias != nullptr && ncols > 0) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (i < ncols) v[i] += static_cast<float>(e.bias[c0 + i]);
+    }
+    if (!e.use_tma) {
+      if (row < e.m && ncols > 0) store_chunk<OutT>(e.out + (int64_t)row * e.ldo + c0, v, ncols, e.out_vec_ok != 0);
+      continue;
+    }
+    const bool first = COLS_PER_BOX == 32 || h == 0, last = COLS_PER_BOX == 32 || h == 1;
+    const int box_col = COLS_PER_BOX == 32 ? c0 : col;
+    if (box_col >= e.n || row0 >= e.m) continue;  // the same for the whole warp; partial boxes are clipped by the map
+    uint8_t* box = e.staging + (boxes & 1u) * EPI_BOX_BYTES;
+    if (first && boxes >= 2u) {  // the store issued two boxes ago must have read this one
+      if (lane == 0) bulk_wait_read<1>();
+      __syncwarp();
+    }
+    uint8_t* rowp = box + lane * 128;  // 16-byte chunk j of row `lane` lives at j ^ (lane & 7)
+    if constexpr (sizeof(OutT) == 2) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        uint32_t w[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          OutT lo = static_cast<OutT>(v[q * 8 + 2 * t]), hi = static_cast<OutT>(v[q * 8 + 2 * t + 1]);
+          w[t] = (uint32_t)(*reinterpret_cast<unsigned short*>(&lo)) | ((uint32_t)(*reinterpret_cast<unsigned short*>(&hi)) << 16);
+        }
+        *reinterpret_cast<uint4*>(rowp + (((h * 4 + q) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        *reinterpret_cast<float4*>(rowp + ((q ^ (lane & 7)) << 4)) = make_float4(v[q * 4], v[q * 4 + 1], v[q * 4 + 2], v[q * 4 + 3]);
+    }
+    if (last) {
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_2d_hint(e.tma_out, box, box_col, row0, l2_policy(1));
+        bulk_commit();
+      }
+      ++boxes;
+    }
+  }
+}
+
+template <typename OutT>
+__global__ void __launch_bounds__(XTHREADS, 1)
+gemm_block_scaled_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
+                         const __grid_constant__ CUtensorMap tma_ea, const __grid_constant__ CUtensorMap tma_eb,
+                         const __grid_constant__ CUtensorMap tma_out, const OutT* __restrict__ bias,
+                         OutT* __restrict__ out, int64_t ldo, int m, int n, int k, uint32_t idesc, int out_vec_ok,
+                         int use_tma_store, int raster) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* staging = tiles + XSTAGES * XSTAGE_BYTES;
+  uint8_t* factors = staging + EPI_STAGING_BYTES;  // per stage: 512 bytes of A's, 1024 of B's
+  ScaledBars* bars = reinterpret_cast<ScaledBars*>(factors + XSTAGES * 2048);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const uint32_t peer = rank ^ 1u;
+  const bool leader = rank == 0;
+  const int tiles_m = (m + PBM - 1) / PBM, tiles_n = (n + PBN - 1) / PBN;
+  const int64_t num_tiles = (int64_t)tiles_m * tiles_n;
+  const int num_kb = (k + BK - 1) / BK;
+  const int64_t cluster_id = blockIdx.x >> 1, num_clusters = gridDim.x >> 1;
+  const bool a_mn = (raster >> LAYOUT_A_MN_BIT) & 1, b_mn = (raster >> LAYOUT_B_MN_BIT) & 1;
+  const uint64_t step_a = desc_k_step(a_mn), step_b = desc_k_step(b_mn);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < XSTAGES; ++s) {
+      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->empty[s], 1);
+    }
+    mbar_init(&bars->tmem_full[0], 1);
+    mbar_init(&bars->tmem_full[1], 1);
+    mbar_init(&bars->tmem_shared_free, 8);
+    bars->abort_flag = 0u;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem_base)),
+                 "r"((uint32_t)TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem_base = bars->tmem_base;
+
+  if (warp == 0) {
+    // ---------------- TMA producer (one per CTA) ----------------
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int64_t t = cluster_id; ok && t < num_tiles; t += num_clusters) {
+        const TileCoord tc = tile_coord(t, tiles_m, tiles_n, raster);
+        const int row_a = tc.m * PBM + (int)rank * 128;
+        const int row_b = tc.n * PBN + (int)rank * 128;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!pair_wait(&bars->empty[stage], phase ^ 1u, bars, peer, 1u, 64u)) { ok = false; break; }
+          uint8_t* sa = tiles + stage * XSTAGE_BYTES;
+          uint8_t* sf = factors + stage * 2048;
+          const bool with_factors = (kb & 3) == 0;
+          if (leader) mbar_expect_tx(&bars->full[stage], 2 * (XSTAGE_BYTES + (with_factors ? XSF_A + XSF_B : 0)));
+          const uint32_t full_in_leader = mapa_u32(smem_u32(&bars->full[stage]), 0u);
+          if (with_factors) {
+            tma_load_2d_pair_plain(sf, &tma_ea, row_a, kb >> 2, full_in_leader);
+            tma_load_2d_pair_plain(sf + XSF_A, &tma_eb, tc.n * PBN, kb >> 2, full_in_leader);
+          }
+          tma_load_2d_pair_plain(sa, &tma_a, a_mn ? row_a : kb * BK, a_mn ? kb * BK : row_a, full_in_leader);
+          tma_load_2d_pair_plain(sa + PA_BYTES, &tma_b, b_mn ? row_b : kb * BK, b_mn ? kb * BK : row_b,
+                                 full_in_leader);
+          if (++stage == XSTAGES) { stage = 0; phase ^= 1u; }
+        }
+      }
+      // tail: every release the leader multicast to this CTA's empty barriers has landed
+      for (int s = 0; ok && s < XSTAGES; ++s) {
+        if (!pair_wait(&bars->empty[stage], phase ^ 1u, bars, peer, 1u, 64u)) { ok = false; break; }
+        if (++stage == XSTAGES) { stage = 0; phase ^= 1u; }
+      }
+      if (!ok) {
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000LL) {}
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer (leader CTA only) ----------------
+    if (leader && lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0, set = 0;
+      bool ok = true;
+      uint32_t local = 0;
+      for (int64_t t = cluster_id; ok && t < num_tiles; t += num_clusters, ++local) {
+        const uint32_t acc = local & 1u;
+        // the columns that this accumulator shares with the previous tile's have been read
+        if (local > 0 && !pair_wait(&bars->tmem_shared_free, (local - 1) & 1u, bars, peer, 2u)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t tmem_d = tmem_base + acc * (uint32_t)XACC_STEP;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!pair_wait(&bars->full[stage], phase, bars, peer, 4u)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t a_addr = smem_u32(tiles + stage * XSTAGE_BYTES);
+          if ((kb & 3) == 0) {
+            set ^= 1u;
+            const uint32_t f = smem_u32(factors + stage * 2048), d = tmem_base + XSF_COL + set * XSF_SET;
+            tc_copy_factors_pair(d, f);
+            tc_copy_factors_pair(d + 4, f + XSF_A);
+            tc_copy_factors_pair(d + 8, f + XSF_A + 512);
+          }
+          const uint32_t sf = tmem_base + XSF_COL + set * XSF_SET;
+          const uint32_t id = idesc | ((uint32_t)(kb & 3) << 4) | ((uint32_t)(kb & 3) << 29);
+          const uint64_t da = a_mn ? make_smem_desc_mn(a_addr, PA_BYTES) : make_smem_desc(a_addr);
+          const uint64_t db = b_mn ? make_smem_desc_mn(a_addr + PA_BYTES, PB_BYTES) : make_smem_desc(a_addr + PA_BYTES);
+#pragma unroll
+          for (int kk = 0; kk < BK / UMMA_K; ++kk)
+            tc_mma_mx_pair(tmem_d, da + (uint64_t)kk * step_a, db + (uint64_t)kk * step_b, id, sf, sf + 4,
+                           (kb | kk) != 0 ? 1u : 0u);
+          tc_commit_pair(&bars->empty[stage]);
+          if (++stage == XSTAGES) { stage = 0; phase ^= 1u; }
+        }
+        if (!ok) break;
+        tc_commit_pair(&bars->tmem_full[acc]);
+      }
+    }
+  } else {
+    // ---------------- epilogue (warps 2..5 of both CTAs) ----------------
+    const int quarter = warp & 3;
+    const EpilogueArgs<OutT> ea{bias, out, ldo, m, n, out_vec_ok, use_tma_store, &tma_out,
+                                staging + (warp - 2) * 2 * EPI_BOX_BYTES, 1.0f, 1, nullptr};
+    const uint32_t free_in_leader = mapa_u32(smem_u32(&bars->tmem_shared_free), 0u);
+    uint32_t boxes = 0, local = 0;
+    bool ok = true;
+    for (int64_t t = cluster_id; ok && t < num_tiles; t += num_clusters, ++local) {
+      const TileCoord tc = tile_coord(t, tiles_m, tiles_n, raster);
+      const uint32_t acc = local & 1u;
+      int got = 1;
+      if (lane == 0) got = pair_wait(&bars->tmem_full[acc], (local >> 1) & 1u, bars, peer, 8u, WAIT_BY_HINT | 1000u) ? 1 : 0;
+      got = __shfl_sync(0xFFFFFFFFu, got, 0);
+      if (got == 0) { ok = false; break; }
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * (uint32_t)XACC_STEP;
+      const int row0 = tc.m * PBM + (int)rank * 128 + quarter * 32;
+#pragma unroll 1
+      for (int b = 0; b < 4; ++b) {
+        const int part = acc == 0 ? (b + 3) & 3 : b;  // the shared columns first: the last 64 of accumulator 0, the first of 1
+        uint32_t r[2][32];
+        tc_ld_32x32b_x32(taddr + (uint32_t)(part * 64), r[0]);
+        tc_ld_32x32b_x32(taddr + (uint32_t)(part * 64 + 32), r[1]);
+        tc_wait_ld();
+        if (b == 0) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(free_in_leader);
+        }
+        store_columns<OutT>(ea, r, row0, tc.n * PBN + part * 64, boxes);
+      }
+    }
+    if (use_tma_store && lane == 0) bulk_wait_all();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // neither CTA leaves while the other may still touch its barriers or TMEM
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)TMEM_COLS)
+                 : "memory");
+  }
+}
+
 // ---- host side --------------------------------------------------------------------------------------
 static bool strides_ok(const BlockScale& s) { return s.row_stride >= 0 && s.kb_stride >= 0; }
 
@@ -545,6 +829,62 @@ static int launch_block_pair(const CUtensorMap& ma, const CUtensorMap& mb, const
   cfg.gridDim = dim3(2 * clusters);
   return record_cuda_error(cudaLaunchKernelEx(&cfg, kernel, ma, mb, sa, sb, static_cast<const OutT*>(bias),
                                               static_cast<OutT*>(out), ldo, m, n, k, idesc, vec_ok,
+                                              choose_raster(m, n, k, PBM, PBN) | layouts));
+}
+
+// Exponent bytes of an operand (the layout of cast_block.cu's exponent_at) as a matrix of 32-bit words: one row per four
+// k-blocks, box = `words` of one of them.
+static int encode_exponent_map(CUtensorMap* map, const void* base, int64_t rows, int64_t k, int words) {
+  auto fn = get_encode_fn();
+  if (fn == nullptr) return F8B200_ERR_DRIVER;
+  const int64_t pitch_words = (rows + 255) / 256 * 256;
+  const cuuint64_t gdim[2] = {(cuuint64_t)pitch_words, (cuuint64_t)((k + 511) / 512)};
+  const cuuint64_t gstride[1] = {(cuuint64_t)(pitch_words * 4)};
+  const cuuint32_t box[2] = {(cuuint32_t)words, 1u};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(base), gdim, gstride, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? F8B200_OK : F8B200_ERR_DRIVER;
+}
+
+template <typename OutT>
+static int launch_block_scaled(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mea, const CUtensorMap& meb,
+                               const CUtensorMap& mo, int use_tma, const void* bias, void* out, int64_t ldo, int m, int n,
+                               int k, uint32_t idesc, int vec_ok, int layouts, cudaStream_t st) {
+  static PerDeviceOnce setup;
+  int max_clusters = 0;
+  auto kernel = gemm_block_scaled_kernel<OutT>;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.blockDim = dim3(XTHREADS);
+  cfg.dynamicSmemBytes = XSMEM_BYTES;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t attr_err = setup.run(
+      [&](int* clusters_out) {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, XSMEM_BYTES);
+        if (e == cudaSuccess) {
+          cfg.gridDim = dim3(2 * (sm_count() / 2));
+          e = cudaOccupancyMaxActiveClusters(clusters_out, kernel, &cfg);
+        }
+        return e;
+      },
+      &max_clusters);
+  if (attr_err != cudaSuccess) return record_cuda_error(attr_err);
+  if (max_clusters < 1) return F8B200_ERR_UNSUPPORTED;
+  const int64_t tiles = (int64_t)((m + PBM - 1) / PBM) * ((n + PBN - 1) / PBN);
+  int clusters = max_clusters;
+  if (persistent_ctas() / 2 < clusters) clusters = persistent_ctas() / 2;
+  if (tiles < clusters) clusters = (int)tiles;
+  cfg.gridDim = dim3(2 * clusters);
+  return record_cuda_error(cudaLaunchKernelEx(&cfg, kernel, ma, mb, mea, meb, mo, static_cast<const OutT*>(bias),
+                                              static_cast<OutT*>(out), ldo, m, n, k, idesc, vec_ok, use_tma,
                                               choose_raster(m, n, k, PBM, PBN) | layouts));
 }
 
@@ -593,10 +933,11 @@ static int few_split(int64_t tiles, int num_kb) {
 }  // namespace f8b200
 
 extern "C" int f8b200_gemm_blockwise(const void* a, int a_kind, int a_layout, int64_t lda, const float* scale_a,
-                                     int64_t sa_row_stride, int64_t sa_kb_stride, int a_block_rows, const void* b,
+                                     int64_t sa_row_stride, int64_t sa_kb_stride, int a_block_rows,
+                                     const void* exp_a, const void* b,
                                      int b_kind, int b_layout, int64_t ldb, const float* scale_b, int64_t sb_row_stride,
-                                     int64_t sb_kb_stride, int b_block_rows, const void* bias, int out_dtype, void* out,
-                                     int64_t ldo, int64_t m, int64_t n, int64_t k, void* stream) {
+                                     int64_t sb_kb_stride, int b_block_rows, const void* exp_b, const void* bias,
+                                     int out_dtype, void* out, int64_t ldo, int64_t m, int64_t n, int64_t k, void* stream) {
   using namespace gemm::block;
   if ((a_block_rows != 1 && a_block_rows != 128) || (b_block_rows != 1 && b_block_rows != 128)) return F8B200_ERR_BAD_ARG;
   const BlockScale sa{scale_a, sa_row_stride, sa_kb_stride, a_block_rows == 128 ? 7 : 0};
@@ -636,6 +977,20 @@ extern "C" int f8b200_gemm_blockwise(const void* a, int a_kind, int a_layout, in
   if (rc == F8B200_OK)
     rc = b_layout ? gemm::encode_operand_map_mn(&mb, b, n, k, ldb) : gemm::encode_operand_map(&mb, b, n, k, ldb, 128);
   if (rc != F8B200_OK) return rc;
+  if (exp_a != nullptr && exp_b != nullptr) {  // both sides' factors are powers of two
+    if (reinterpret_cast<uintptr_t>(exp_a) % 16 != 0 || reinterpret_cast<uintptr_t>(exp_b) % 16 != 0) return F8B200_ERR_ALIGNMENT;
+    CUtensorMap mea, meb, mo;
+    rc = encode_exponent_map(&mea, exp_a, m, k, 128);
+    if (rc == F8B200_OK) rc = encode_exponent_map(&meb, exp_b, n, k, 256);
+    memset(&mo, 0, sizeof(mo));
+    if (rc == F8B200_OK && vec_ok) rc = gemm::encode_output_map(&mo, out, m, n, ldo, out_dtype);
+    if (rc != F8B200_OK) return rc;
+    return dispatch_out_dtype(out_dtype, [&](auto* tag) {
+      using OutT = std::remove_pointer_t<decltype(tag)>;
+      return launch_block_scaled<OutT>(ma, mb, mea, meb, mo, vec_ok, bias, out, ldo, (int)m, (int)n, (int)k,
+                                       make_idesc_scaled(a_kind, b_kind, a_layout, b_layout), vec_ok, layouts, st);
+    });
+  }
   const uint32_t idesc = gemm::pair::make_idesc_pair(a_kind, b_kind, a_layout, b_layout);
   return dispatch_out_dtype(out_dtype, [&](auto* tag) {
     using OutT = std::remove_pointer_t<decltype(tag)>;

@@ -33,9 +33,13 @@ class Float8BlockTensor:
     data       [rows, cols] torch.float8_e4m3fn or float8_e5m2, in either memory order
     scale_inv  float32 [ceil(rows / block[0]), ceil(cols / block[1])], any strides
     block      (1, 128), (128, 1) or (128, 128); the last block of a dimension may be shorter
-    orig_dtype the dtype `to_original_precision` returns by default"""
+    orig_dtype the dtype `to_original_precision` returns by default
 
-    __slots__ = ("data", "scale_inv", "block", "orig_dtype")
+    A cast also keeps its power-of-two factors as the exponent bytes that the tensor cores read (of the matrix, and
+    of its transpose, as a product's operand).  They go with `scale_inv`: to give a matrix other factors, make a new
+    Float8BlockTensor of its `data`."""
+
+    __slots__ = ("data", "scale_inv", "block", "orig_dtype", "_exps", "_exps_t", "_version")
 
     def __init__(self, data: torch.Tensor, scale_inv: torch.Tensor, block: Tuple[int, int],
                  orig_dtype: torch.dtype = torch.bfloat16):
@@ -53,6 +57,15 @@ class Float8BlockTensor:
         if scale_inv.device != data.device:
             raise ValueError(f"Float8BlockTensor: data on {data.device}, scale_inv on {scale_inv.device}")
         self.data, self.scale_inv, self.block, self.orig_dtype = data, scale_inv, block, orig_dtype
+        self._exps = self._exps_t = self._version = None
+
+    def _with_exponents(self, exps, exps_t) -> "Float8BlockTensor":
+        self._exps, self._exps_t, self._version = exps, exps_t, self.scale_inv._version
+        return self
+
+    def _exponents(self, transposed: bool = False) -> Optional[torch.Tensor]:
+        """The exponent bytes, unless the factors were written to since the cast."""
+        return (self._exps_t if transposed else self._exps) if self._version == self.scale_inv._version else None
 
     @property
     def shape(self) -> torch.Size:
@@ -64,7 +77,9 @@ class Float8BlockTensor:
 
     def t(self) -> "Float8BlockTensor":
         """The transposed matrix: the same bytes and factors, nothing copied."""
-        return Float8BlockTensor(self.data.t(), self.scale_inv.t(), self.block[::-1], self.orig_dtype)
+        out = Float8BlockTensor(self.data.t(), self.scale_inv.t(), self.block[::-1], self.orig_dtype)
+        out._exps, out._exps_t, out._version = self._exps_t, self._exps, self._version
+        return out
 
     def to_original_precision(self, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         return ops.uncast_blockwise(self.data, self.scale_inv, *self.block, dtype or self.orig_dtype)
@@ -88,20 +103,23 @@ def cast_to_float8_blockwise(x: torch.Tensor, block: Tuple[int, int] = (1, BLOCK
         raise ValueError(f"cast_to_float8_blockwise: block must be one of {_BLOCKS}, got {block}")
     x, kind = _matrix(x, "cast_to_float8_blockwise"), _kind(float8_dtype)
     if block == (BLOCK, BLOCK):
-        data, scale = ops.cast_blockwise_square(x, kind)
+        data, scale, exps, exps_t = ops.cast_blockwise_square(x, kind)
     elif block == (1, BLOCK):
-        data, scale, _, _ = ops.cast_blockwise(x, kind, True, False)
+        data, scale, exps, _, _, _ = ops.cast_blockwise(x, kind, True, False)
+        exps_t = None
     else:
-        _, _, data, scale = ops.cast_blockwise(x, kind, False, True)
-    return Float8BlockTensor(data, scale, block, x.dtype)
+        _, _, _, data, scale, exps_t = ops.cast_blockwise(x, kind, False, True)
+        exps = None
+    return Float8BlockTensor(data, scale, block, x.dtype)._with_exponents(exps, exps_t)
 
 
 def cast_to_float8_blockwise_both(x: torch.Tensor, float8_dtype: torch.dtype = e4m3_dtype
                                   ) -> Tuple[Float8BlockTensor, Float8BlockTensor]:
     """`x` cast by rows (1 x 128 blocks) and by columns (128 x 1), from one read of it."""
     x = _matrix(x, "cast_to_float8_blockwise_both")
-    data, scale, data_c, scale_c = ops.cast_blockwise(x, _kind(float8_dtype), True, True)
-    return (Float8BlockTensor(data, scale, (1, BLOCK), x.dtype), Float8BlockTensor(data_c, scale_c, (BLOCK, 1), x.dtype))
+    data, scale, exps, data_c, scale_c, exps_c = ops.cast_blockwise(x, _kind(float8_dtype), True, True)
+    return (Float8BlockTensor(data, scale, (1, BLOCK), x.dtype)._with_exponents(exps, None),
+            Float8BlockTensor(data_c, scale_c, (BLOCK, 1), x.dtype)._with_exponents(None, exps_c))
 
 
 def blockwise_mm(a: Float8BlockTensor, b: Float8BlockTensor, out_dtype: torch.dtype = torch.bfloat16,
@@ -118,7 +136,8 @@ def blockwise_mm(a: Float8BlockTensor, b: Float8BlockTensor, out_dtype: torch.dt
     if a.shape[1] != b.shape[0]:
         raise ValueError(f"blockwise_mm: inner dimensions differ ({a.shape[1]} vs {b.shape[0]})")
     N.hp_code(out_dtype)
-    return ops.blockwise_mm(a.data, b.data.t(), a.scale_inv, b.scale_inv.t(), a.block[0], b.block[1], bias, out_dtype)
+    return ops.blockwise_mm(a.data, b.data.t(), a.scale_inv, b.scale_inv.t(), a.block[0], b.block[1],
+                            a._exponents(), b._exponents(transposed=True), bias, out_dtype)
 
 
 @torch._dynamo.allow_in_graph
@@ -131,27 +150,27 @@ class _float8_linear_blockwise(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, need_dw: bool):
         x2 = x.reshape(-1, x.shape[-1])
-        x8, sx, x8c, sxc = ops.cast_blockwise(x2, N.E4M3, True, need_dw)
-        w8, sw = ops.cast_blockwise_square(weight, N.E4M3)
-        y = ops.blockwise_mm(x8, w8, sx, sw, 1, BLOCK, bias, x.dtype)
-        ctx.save_for_backward(x8c, sxc, w8, sw)
+        x8, sx, ex, x8c, sxc, exc = ops.cast_blockwise(x2, N.E4M3, True, need_dw)
+        w8, sw, ew, ewt = ops.cast_blockwise_square(weight, N.E4M3)
+        y = ops.blockwise_mm(x8, w8, sx, sw, 1, BLOCK, ex, ew, bias, x.dtype)
+        ctx.save_for_backward(x8c, sxc, exc, w8, sw, ewt)
         ctx.dtypes = (weight.dtype, bias.dtype if bias is not None else None)
         return y.reshape(*x.shape[:-1], y.shape[-1])
 
     @staticmethod
     @once_differentiable
     def backward(ctx, go):
-        x8c, sxc, w8, sw = ctx.saved_tensors
+        x8c, sxc, exc, w8, sw, ewt = ctx.saved_tensors
         need_dx, need_dw, need_db = ctx.needs_input_grad[:3]
         go2 = go.reshape(-1, go.shape[-1])
         dx = dw = db = None
         if need_dx or need_dw:
-            g8, sg, g8c, sgc = ops.cast_blockwise(go2, N.E4M3, need_dx, need_dw)
+            g8, sg, eg, g8c, sgc, egc = ops.cast_blockwise(go2, N.E4M3, need_dx, need_dw)
         if need_dx:  # dX = dY @ W: the weight's bytes and factors read transposed
-            dx = ops.blockwise_mm(g8, w8.t(), sg, sw.t(), 1, BLOCK, None, go.dtype)
+            dx = ops.blockwise_mm(g8, w8.t(), sg, sw.t(), 1, BLOCK, eg, ewt, None, go.dtype)
             dx = dx.reshape(*go.shape[:-1], dx.shape[-1])
         if need_dw:  # dW = dY^T @ X, summed over rows: both by columns
-            dw = ops.blockwise_mm(g8c.t(), x8c.t(), sgc.t(), sxc.t(), 1, 1, None, ctx.dtypes[0])
+            dw = ops.blockwise_mm(g8c.t(), x8c.t(), sgc.t(), sxc.t(), 1, 1, egc, exc, None, ctx.dtypes[0])
         if need_db:
             db = go2.sum(0, dtype=torch.float32).to(ctx.dtypes[1])
         return dx, dw, db, None

@@ -104,7 +104,7 @@ class Float8InferenceLinear(torch.nn.Linear):
         if type(input) not in (torch.Tensor, nn.Parameter):
             raise RuntimeError(f"ActivationCasting.BLOCKWISE takes plain tensors, got a {type(input).__name__}")
         x8 = cast_to_float8_blockwise(input.reshape(-1, input.shape[-1]))
-        y = ops.blockwise_mm(x8.data, self.weight, x8.scale_inv, self.weight_scale_inv, 1, BLOCK, self.bias, input.dtype)
+        y = ops.blockwise_mm(x8.data, self.weight, x8.scale_inv, self.weight_scale_inv, 1, BLOCK, None, None, self.bias, input.dtype)
         return y.reshape(*input.shape[:-1], y.shape[-1])
 
     def quantize_weight(self, dtype: torch.dtype = e4m3_dtype) -> None:

@@ -413,14 +413,20 @@ int f8b200_swiglu_bwd_approx(const void* a, const void* b, const void* grad_y, i
  *                           scale_c[i * ld_scale_c + c], ld_scale_c >= cols;
  *     by_square != 0        out_r in 128 x 128 blocks instead, the factor of (i, j) at scale_r[i * ld_scale_r + j],
  *                           ld_scale_r >= ceil(cols / 128); out_c must be NULL.
+ *     exp_r, exp_c          (may be NULL; with by_square both or neither) the factors' exponent bytes in the order in
+ *                           which the tensor cores read them, for f8b200_gemm_blockwise: exp_r for out_r as an
+ *                           operand with rows `rows` and K = cols, f8b200_block_exponent_bytes(rows, cols) bytes;
+ *                           exp_c for the transpose of out_c (by_square: of out_r), ..._bytes(cols, rows) bytes.
+ *                           16-byte aligned.
  * f8b200_uncast_blockwise y = RN_T(q * scale), the factor of a block (i, j) of block_rows x block_cols (1 or 128 each)
  *                         at scale[i * scale_row_stride + j * scale_col_stride].
  * Empty matrices return F8B200_OK without a launch.
  */
+int64_t f8b200_block_exponent_bytes(int64_t rows, int64_t k);
 int f8b200_cast_blockwise(const void* x, int hp_dtype, int64_t rows, int64_t cols, int64_t ld_x,
                           int fp8_kind, int by_square, void* out_r, int64_t ld_r, float* scale_r,
-                          int64_t ld_scale_r, void* out_c, int64_t ld_c, float* scale_c,
-                          int64_t ld_scale_c, void* stream);
+                          int64_t ld_scale_r, void* exp_r, void* out_c, int64_t ld_c, float* scale_c,
+                          int64_t ld_scale_c, void* exp_c, void* stream);
 int f8b200_uncast_blockwise(const void* q, int fp8_kind, int64_t rows, int64_t cols, int64_t ld_q,
                             const float* scale, int64_t scale_row_stride, int64_t scale_col_stride,
                             int block_rows, int block_cols, int hp_dtype, void* y, int64_t ld_y,
@@ -431,13 +437,15 @@ int f8b200_uncast_blockwise(const void* q, int fp8_kind, int64_t rows, int64_t c
  * with blocks of 128 along K, fp32 sums, one rounding to out_dtype.  Operands, layouts, pitches and alignment as in
  * f8b200_gemm_fp8_ws; K may be any number, the last block being shorter.  The factor of A's row m and block j lies
  * at scale_a[(m / a_block_rows) * sa_row_stride + j * sa_kb_stride], a_block_rows 1 or 128, strides >= 0
- * (elements); B's likewise.  Factors are arbitrary fp32 values.  `bias` has out_dtype or is NULL.  Needs no workspace.
+ * (elements); B's likewise.  Factors are arbitrary fp32 values.  exp_a and exp_b (each may be NULL) are the exponent
+ * bytes that f8b200_cast_blockwise wrote beside those factors; with both given, products of more than a few rows let
+ * the tensor cores apply them.  `bias` has out_dtype or is NULL.  Needs no workspace.
  */
 int f8b200_gemm_blockwise(const void* a, int a_kind, int a_layout, int64_t lda, const float* scale_a,
-                          int64_t sa_row_stride, int64_t sa_kb_stride, int a_block_rows, const void* b,
-                          int b_kind, int b_layout, int64_t ldb, const float* scale_b,
-                          int64_t sb_row_stride, int64_t sb_kb_stride, int b_block_rows,
-                          const void* bias, int out_dtype, void* out, int64_t ldo, int64_t m, int64_t n,
+                          int64_t sa_row_stride, int64_t sa_kb_stride, int a_block_rows,
+                          const void* exp_a, const void* b, int b_kind, int b_layout, int64_t ldb,
+                          const float* scale_b, int64_t sb_row_stride, int64_t sb_kb_stride,
+                          int b_block_rows, const void* exp_b, const void* bias, int out_dtype, void* out, int64_t ldo, int64_t m, int64_t n,
                           int64_t k, void* stream);
 
 /*

@@ -7,7 +7,7 @@ import torch
 
 import float8_experimental_b200 as f8
 from float8_experimental_b200 import _native as N
-from float8_experimental_b200._ops import _check_dense
+from float8_experimental_b200._ops import _check_dense, _exponent_bytes
 from float8_experimental_b200.float8_blockwise import (
     blockwise_mm, cast_to_float8_blockwise, cast_to_float8_blockwise_both, Float8BlockTensor,
 )
@@ -97,14 +97,17 @@ def test_grad_clip_rules():
 def test_c_argument_checks_come_before_any_cuda_call():
     lib = N.load()
     cast = lambda **k: lib.f8b200_cast_blockwise(*{**dict(  # noqa: E731
-        x=P, dt=0, rows=4, cols=8, ld=8, kind=0, sq=0, o=P, ldo=8, s=P, lds=4, oc=None, ldc=0, sc=None, ldsc=0, st=None), **k}.values())
+        x=P, dt=0, rows=4, cols=8, ld=8, kind=0, sq=0, o=P, ldo=8, s=P, lds=4, e=None, oc=None, ldc=0, sc=None, ldsc=0, ec=None,
+        st=None), **k}.values())
     for bad in (dict(dt=3), dict(kind=2), dict(x=None), dict(ld=7), dict(o=None), dict(s=None), dict(ldo=7), dict(lds=3),
                 dict(rows=-1), dict(oc=P, ldc=8), dict(oc=P, ldc=7, sc=P, ldsc=8), dict(oc=P, ldc=8, sc=P, ldsc=7),
-                dict(sq=1, oc=P, ldc=8, sc=P, ldsc=8), dict(sq=1, lds=0)):
+                dict(sq=1, oc=P, ldc=8, sc=P, ldsc=8), dict(sq=1, lds=0), dict(sq=1, e=P), dict(ec=P)):
         assert cast(**bad) == -1, bad
     assert cast(s=vp(258)) == -2 and cast(x=vp(257)) == -2
     assert cast(rows=0) == 0 and cast(cols=0) == 0
     assert cast(rows=1 << 40, cols=1 << 20, ld=1 << 20, ldo=1 << 20, lds=1 << 40) == -6
+    assert lib.f8b200_block_exponent_bytes(1, 1) == 1024 and lib.f8b200_block_exponent_bytes(257, 513) == 4096
+    assert _exponent_bytes(257, 513) == 4096 and lib.f8b200_block_exponent_bytes(0, 5) == _exponent_bytes(0, 5) == 0
     unc = lambda **k: lib.f8b200_uncast_blockwise(*{**dict(  # noqa: E731
         q=P, kind=0, rows=4, cols=8, ld=8, s=P, sr=1, sc=1, br=1, bc=128, dt=0, y=P, ldy=8, st=None), **k}.values())
     for bad in (dict(q=None), dict(s=None), dict(y=None), dict(br=2), dict(bc=64), dict(ld=7), dict(ldy=7), dict(sr=-1),
@@ -112,7 +115,7 @@ def test_c_argument_checks_come_before_any_cuda_call():
         assert unc(**bad) == -1, bad
     assert unc(y=vp(257)) == -2 and unc(rows=0) == 0
     mm = lambda **k: lib.f8b200_gemm_blockwise(*{**dict(  # noqa: E731
-        a=P, ak=0, al=0, lda=16, sa=P, sar=1, sak=1, ab=1, b=P, bk=0, bl=0, ldb=16, sb=P, sbr=1, sbk=1, bb=128, bias=None,
+        a=P, ak=0, al=0, lda=16, sa=P, sar=1, sak=1, ab=1, ea=None, b=P, bk=0, bl=0, ldb=16, sb=P, sbr=1, sbk=1, bb=128, eb=None, bias=None,
         dt=0, out=P, ldo=4, m=4, n=4, k=16, st=None), **k}.values())
     assert mm(m=0) == 0 and mm(n=0) == 0 and mm(k=0) == -6
     assert mm(lda=24) == -2 and mm(a=vp(264)) == -2

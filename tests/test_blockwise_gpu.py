@@ -123,7 +123,7 @@ def check_product(m, n, k, a_block=1, b_block=128, fa=E4, fb=E4, out=BF, bias=Fa
     a, sa = operand(m, k, fa, a_block, seed, a_mn)
     b, sb = operand(n, k, fb, b_block, seed + 100, b_mn)
     bv = randn(n, seed=seed + 5).to(out) if bias else None
-    got = ops.blockwise_mm(a, b, sa, sb, a_block, b_block, bv, out)
+    got = ops.blockwise_mm(a, b, sa, sb, a_block, b_block, None, None, bv, out)
     ref, mag = product(a, sa, a_block, b, sb, b_block, bv)
     err = (got.double() - ref).abs() - product_tolerance(ref, mag, k, out)
     assert got.shape == (m, n) and got.dtype == out
@@ -177,9 +177,9 @@ def test_product_strided_and_broadcast_factors():
     one = torch.full((1, 1), 0.25, device="cuda")
     for s in (wide_sa[::2, ::2], sa.t().contiguous().t()):
         ref, mag = product(a, sa, 1, b, sb, 128)
-        got = ops.blockwise_mm(a, b, s, sb, 1, 128, None, FP32)
+        got = ops.blockwise_mm(a, b, s, sb, 1, 128, None, None, None, FP32)
         assert float(((got - ref).abs() - product_tolerance(ref, mag, 512, FP32)).max()) <= 0
-    got = ops.blockwise_mm(a, b, one.expand(200, 4), sb, 1, 128, None, FP32)
+    got = ops.blockwise_mm(a, b, one.expand(200, 4), sb, 1, 128, None, None, None, FP32)
     ref, mag = product(a, one.expand(200, 4), 1, b, sb, 128)
     assert float(((got - ref).abs() - product_tolerance(ref, mag, 512, FP32)).max()) <= 0
 
@@ -190,7 +190,7 @@ def test_product_factors_need_not_be_scaled_alike():
         a, sa = operand(m, 640, E4, 1, 8)
         b, sb = operand(256, 640, E4, 128, 9)
         sa = sa * torch.tensor([2.0 ** -60, 1.0, 2.0 ** 60, 2.0 ** -30, 2.0 ** 30], device="cuda")
-        got = ops.blockwise_mm(a, b, sa, sb, 1, 128, None, FP32)
+        got = ops.blockwise_mm(a, b, sa, sb, 1, 128, None, None, None, FP32)
         ref, mag = product(a, sa, 1, b, sb, 128)
         assert float(((got - ref).abs() - product_tolerance(ref, mag, 640, FP32)).max()) <= 0
 
@@ -205,6 +205,42 @@ def test_product_of_a_poisoned_block():
         bad[7] = True
         bad[:, 128:] = True
         assert torch.equal(torch.isnan(y), bad)
+
+
+@pytest.mark.parametrize("m,n,k", [(129, 128, 128), (200, 256, 512), (300, 260, 640), (513, 1000, 1030), (1, 200, 300),
+                                   (140, 77, 2333), (4100, 600, 520)])
+@pytest.mark.parametrize("out", [BF, FP16, FP32])
+@pytest.mark.parametrize("kinds", [(E4, E4), (E4, E5), (E5, E4)])
+def test_products_of_casts(m, n, k, out, kinds):
+    """Operands from the casts, whose power-of-two factors the tensor cores apply: all three products of a layer, against
+    the doubles of what the casts stand for."""
+    x = wide(m, k, BF, seed=m).clamp(-1e3, 1e3)
+    w, g = randn(n, k, seed=n).to(BF), randn(m, n, seed=k).to(BF)
+    if m > 20:
+        x[17, 3] = float("nan")
+    xr, xc = cast_to_float8_blockwise_both(x, kinds[0])
+    gr, gc = cast_to_float8_blockwise_both(g, kinds[0])
+    w8 = cast_to_float8_blockwise(w, (128, 128), kinds[1])
+    b = randn(n, seed=1).to(out)
+    for a, bt, bias, kk in ((xr, w8, b, k), (gr, w8.t(), None, n), (gc.t(), xc.t(), None, m)):
+        ref, mag = product(a.data, a.scale_inv, a.block[0], bt.data, bt.scale_inv, bt.block[0], bias)
+        got = blockwise_mm(a, bt.t(), out, bias)
+        err = (got.double() - ref).abs() - product_tolerance(ref, mag, kk, out)
+        top = torch.finfo(out).max
+        fits = ref.abs() < top * 0.99
+        assert torch.equal(torch.isnan(got), torch.isnan(ref))
+        assert float(torch.where(fits, err, -1.0).max()) <= 0
+
+
+def test_factors_written_after_the_cast_count():
+    for m in (20, 300):
+        x = cast_to_float8_blockwise(randn(m, 256, seed=1).to(BF))
+        w = cast_to_float8_blockwise(randn(128, 256, seed=2).to(BF), (128, 128))
+        blockwise_mm(x, w.t(), FP32)
+        x.scale_inv.mul_(2)
+        # another kernel's order of summation: both are held to the doubles, not to each other's bits
+        ref, mag = product(x.data, x.scale_inv, 1, w.data, w.scale_inv, 128)
+        assert float(((blockwise_mm(x, w.t(), FP32) - ref).abs() - product_tolerance(ref, mag, 256, FP32)).max()) <= 0
 
 
 def test_product_empty():
@@ -222,9 +258,9 @@ def test_product_repeats_to_the_bit():
     for m in (33, 700):
         a, sa = operand(m, 4096, E4, 1, 1)
         b, sb = operand(1024, 4096, E4, 1, 2)
-        first = ops.blockwise_mm(a, b, sa, sb, 1, 1, None, FP32)
+        first = ops.blockwise_mm(a, b, sa, sb, 1, 1, None, None, None, FP32)
         for _ in range(5):
-            assert torch.equal(first, ops.blockwise_mm(a, b, sa, sb, 1, 1, None, FP32))
+            assert torch.equal(first, ops.blockwise_mm(a, b, sa, sb, 1, 1, None, None, None, FP32))
 
 
 # ---- the layers ---------------------------------------------------------------------------------------
@@ -368,9 +404,9 @@ def test_refusals_on_the_gpu():
     with pytest.raises(RuntimeError, match="bias must have"):
         blockwise_mm(a, w.t(), bias=torch.zeros(63, device="cuda"))
     with pytest.raises(RuntimeError, match="scale_a must be"):
-        ops.blockwise_mm(a.data, w.data, a.scale_inv[:, :1], w.scale_inv, 1, 128, None, BF)
+        ops.blockwise_mm(a.data, w.data, a.scale_inv[:, :1], w.scale_inv, 1, 128, None, None, None, BF)
     with pytest.raises(RuntimeError, match="different devices"):
-        ops.blockwise_mm(a.data, w.data, a.scale_inv, w.scale_inv, 1, 128, torch.zeros(64), BF)
+        ops.blockwise_mm(a.data, w.data, a.scale_inv, w.scale_inv, 1, 128, None, None, torch.zeros(64), BF)
     with pytest.raises(N.F8B200Error, match="unsupported high-precision"):
         cast_to_float8_blockwise(torch.zeros(4, 4, device="cuda", dtype=torch.float64))
     layer = Float8Linear.from_float(torch.nn.Linear(256, 64, device="cuda", dtype=BF), blockwise_config())
