@@ -125,7 +125,7 @@ def load() -> ctypes.CDLL:
     lib.f8b200_block_exponent_bytes.restype = i64
     lib.f8b200_uncast_blockwise.argtypes = [vp, i32, i64, i64, i64, vp, i64, i64, i32, i32, i32, vp, i64, vp]
     lib.f8b200_gemm_blockwise.argtypes = [vp, i32, i32, i64, vp, i64, i64, i32, vp, vp, i32, i32, i64, vp, i64, i64, i32, vp,
-                                          vp, i32, vp, i64, i64, i64, i64, vp]
+                                          vp, i32, vp, i64, i64, i64, i64, vp, i64, vp]
     lib.f8b200_layer_norm.argtypes = [vp, i32, i64, i64, i64, vp, vp, i32, ctypes.c_float, vp, i64, vp, vp, vp]
     lib.f8b200_layer_norm_bwd_workspace_bytes.argtypes = [i64]
     lib.f8b200_layer_norm_bwd_workspace_bytes.restype = i64
@@ -620,13 +620,18 @@ def gemm_blockwise(a: torch.Tensor, lda: int, a_mn_major: bool, scale_a: torch.T
                    exp_a: Optional[torch.Tensor], b: torch.Tensor, ldb: int, b_mn_major: bool, scale_b: torch.Tensor,
                    b_block_rows: int, exp_b: Optional[torch.Tensor], bias: Optional[torch.Tensor], out: torch.Tensor, ldo: int, m: int, n: int, k: int) -> None:
     _require_cuda(a, b, scale_a, scale_b, exp_a, exp_b, bias, out)
+    # tiles are handed out through a word of memory; it belongs to this launch alone (a word per stream would be shared by
+    # graphs captured on it that are replayed at the same time)
+    ws = torch.empty(GEMM_WORKSPACE_BYTES, dtype=torch.uint8, device=a.device) if exp_a is not None and exp_b is not None \
+        and m * n > 74 * 256 * 256 else None
     with _Launch("gemm_block", a.device):
         _check(
             load().f8b200_gemm_blockwise(a.data_ptr(), fp8_code(a.dtype), int(a_mn_major), lda, scale_a.data_ptr(),
                                          scale_a.stride(0), scale_a.stride(1), a_block_rows, _ptr(exp_a), b.data_ptr(),
                                          fp8_code(b.dtype), int(b_mn_major), ldb, scale_b.data_ptr(), scale_b.stride(0),
                                          scale_b.stride(1), b_block_rows, _ptr(exp_b), _ptr(bias), hp_code(out.dtype), out.data_ptr(),
-                                         ldo, m, n, k, _stream(a)),
+                                         ldo, m, n, k, _ptr(ws), GEMM_WORKSPACE_BYTES if ws is not None else 0,
+                                         _stream(a)),
             "f8b200_gemm_blockwise",
         )
 

@@ -514,25 +514,33 @@ gemm_block_few_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
 // Tensor memory (512 columns): two accumulators of 256 columns that share 64 of them, at 0 and 192, and the
 // factors at 448.  The epilogue reads the shared columns first and then lets the next tile's MMAs start, which go to
 // the other accumulator, while it drains the rest.
-// Factors: one 32-bit word per operand row holds four k-blocks' bytes.  Every fourth k-block brings 128 words of A
-// (this CTA's rows) and 256 of B (the pair's) along by TMA, tcgen05.cp takes them to tensor memory, and the
-// instruction descriptor says which byte the MMA uses.  Two sets of them alternate.
+// Factors: one 32-bit word per operand row holds a group of four k-blocks' bytes.  Per group TMA brings 128 words of A
+// (this CTA's rows) and 256 of B (the pair's), tcgen05.cp takes them to tensor memory, and the instruction descriptor
+// says which byte an MMA uses.  A group's factors come with the stage of its first k-block
+// and are copied right before that block's MMAs, into one of five sets in turn: a set must not be written before the
+// MMAs of the group five earlier have finished, at least five k-blocks back, and the stage that the issuing thread has
+// just found full means that the k-block XSTAGES earlier has been multiplied.  (Copies one group ahead, behind
+// another block's MMAs, cost 2 % more time than copies that the group's own MMAs follow; a ring of their own
+// with its own commits cost 9 %.)
 // ---------------------------------------------------------------------------------------------------
 constexpr int XTHREADS = 192;  // TMA warp, MMA warp, 4 epilogue warps
 constexpr int XSTAGES = 5;
 constexpr int XSF_A = 512, XSF_B = 1024;  // bytes of factors per CTA and four k-blocks
 constexpr int XSTAGE_BYTES = PA_BYTES + PB_BYTES;
-constexpr int XACC_STEP = 192, XSF_COL = 448, XSF_SET = 16;
+constexpr int XACC_STEP = 192, XSF_COL = 448, XSF_SET = 12, XSF_SETS = 5;
+constexpr int XSF_BYTES = 2048;  // of shared memory per stage, for the group that comes with it
+static_assert(XSTAGES <= XSF_SETS && XSF_COL + XSF_SETS * XSF_SET <= TMEM_COLS, "see above");
 
 struct __align__(16) ScaledBars {
   uint64_t full[XSTAGES];
   uint64_t empty[XSTAGES];
   uint64_t tmem_full[2];
   uint64_t tmem_shared_free;  // in the leader: 8 arrivals, the shared columns have been read
+  TileRing ring;  // written in both CTAs by the leader's producer thread
   uint32_t tmem_base;
   volatile uint32_t abort_flag;
 };
-constexpr int XSMEM_BYTES = XSTAGES * (XSTAGE_BYTES + 2048) + EPI_STAGING_BYTES + 1024 + (int)sizeof(ScaledBars);
+constexpr int XSMEM_BYTES = XSTAGES * (XSTAGE_BYTES + XSF_BYTES) + EPI_STAGING_BYTES + 1024 + (int)sizeof(ScaledBars);
 
 __device__ __forceinline__ void tc_mma_mx_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
                                                uint32_t tmem_sa, uint32_t tmem_sb, uint32_t accumulate) {
@@ -626,12 +634,12 @@ gemm_block_scaled_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid
                          const __grid_constant__ CUtensorMap tma_ea, const __grid_constant__ CUtensorMap tma_eb,
                          const __grid_constant__ CUtensorMap tma_out, const OutT* __restrict__ bias,
                          OutT* __restrict__ out, int64_t ldo, int m, int n, int k, uint32_t idesc, int out_vec_ok,
-                         int use_tma_store, int raster) {
+                         int use_tma_store, int raster, uint32_t* sched) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* staging = tiles + XSTAGES * XSTAGE_BYTES;
   uint8_t* factors = staging + EPI_STAGING_BYTES;  // per stage: 512 bytes of A's, 1024 of B's
-  ScaledBars* bars = reinterpret_cast<ScaledBars*>(factors + XSTAGES * 2048);
+  ScaledBars* bars = reinterpret_cast<ScaledBars*>(factors + XSTAGES * XSF_BYTES);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -652,6 +660,7 @@ gemm_block_scaled_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid
     mbar_init(&bars->tmem_full[0], 1);
     mbar_init(&bars->tmem_full[1], 1);
     mbar_init(&bars->tmem_shared_free, 8);
+    for (int r = 0; r < RING; ++r) mbar_init(&bars->ring.full[r], 1);
     bars->abort_flag = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -673,18 +682,23 @@ gemm_block_scaled_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int64_t t = cluster_id; ok && t < num_tiles; t += num_clusters) {
+      const int claim_kb = num_kb > 4 ? num_kb - 4 : 0;
+      uint32_t entry = 0;  // ring entries published (leader) or read (partner) so far
+      int64_t t = cluster_id;
+      while (ok && t < num_tiles) {
         const TileCoord tc = tile_coord(t, tiles_m, tiles_n, raster);
         const int row_a = tc.m * PBM + (int)rank * 128;
         const int row_b = tc.n * PBN + (int)rank * 128;
+        int64_t next = t + num_clusters;
         for (int kb = 0; kb < num_kb; ++kb) {
+          if (sched != nullptr && leader && kb == claim_kb) next = num_clusters + (int64_t)atomicAdd(sched, 1u);
           if (!pair_wait(&bars->empty[stage], phase ^ 1u, bars, peer, 1u, 64u)) { ok = false; break; }
           uint8_t* sa = tiles + stage * XSTAGE_BYTES;
-          uint8_t* sf = factors + stage * 2048;
           const bool with_factors = (kb & 3) == 0;
           if (leader) mbar_expect_tx(&bars->full[stage], 2 * (XSTAGE_BYTES + (with_factors ? XSF_A + XSF_B : 0)));
           const uint32_t full_in_leader = mapa_u32(smem_u32(&bars->full[stage]), 0u);
           if (with_factors) {
+            uint8_t* sf = factors + stage * XSF_BYTES;
             tma_load_2d_pair_plain(sf, &tma_ea, row_a, kb >> 2, full_in_leader);
             tma_load_2d_pair_plain(sf + XSF_A, &tma_eb, tc.n * PBN, kb >> 2, full_in_leader);
           }
@@ -693,6 +707,23 @@ gemm_block_scaled_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid
                                  full_in_leader);
           if (++stage == XSTAGES) { stage = 0; phase ^= 1u; }
         }
+        if (!ok) break;
+        if (sched != nullptr) {
+          if (leader) {
+            const uint32_t e = entry & (RING - 1);
+            const int32_t v = next < num_tiles ? (int32_t)next : -1;
+            bars->ring.tile[e] = v;
+            mbar_arrive(&bars->ring.full[e]);
+            st_cluster_u32(mapa_u32(smem_u32(&bars->ring.tile[e]), 1u), (uint32_t)v);
+            mbar_arrive_release_cluster(mapa_u32(smem_u32(&bars->ring.full[e]), 1u));
+          } else {
+            const int32_t v = pair_ring_read(bars, entry, peer, 64u, 32u);
+            if (v == -2) { ok = false; break; }
+            next = v < 0 ? num_tiles : (int64_t)v;
+          }
+          ++entry;
+        }
+        t = next;
       }
       // tail: every release the leader multicast to this CTA's empty barriers has landed
       for (int s = 0; ok && s < XSTAGES; ++s) {
@@ -708,27 +739,29 @@ gemm_block_scaled_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid
     // ---------------- MMA issuer (leader CTA only) ----------------
     if (leader && lane == 0) {
       int stage = 0;
-      uint32_t phase = 0, set = 0;
+      uint32_t phase = 0;
+      int set = 0;
       bool ok = true;
       uint32_t local = 0;
-      for (int64_t t = cluster_id; ok && t < num_tiles; t += num_clusters, ++local) {
+      int64_t t = cluster_id;
+      for (; ok && t < num_tiles; ++local) {
         const uint32_t acc = local & 1u;
+        const uint32_t tmem_d = tmem_base + acc * (uint32_t)XACC_STEP;
         // the columns that this accumulator shares with the previous tile's have been read
         if (local > 0 && !pair_wait(&bars->tmem_shared_free, (local - 1) & 1u, bars, peer, 2u)) { ok = false; break; }
-        tc_fence_after();
-        const uint32_t tmem_d = tmem_base + acc * (uint32_t)XACC_STEP;
+        uint32_t sf = 0;
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!pair_wait(&bars->full[stage], phase, bars, peer, 4u)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t a_addr = smem_u32(tiles + stage * XSTAGE_BYTES);
           if ((kb & 3) == 0) {
-            set ^= 1u;
-            const uint32_t f = smem_u32(factors + stage * 2048), d = tmem_base + XSF_COL + set * XSF_SET;
-            tc_copy_factors_pair(d, f);
-            tc_copy_factors_pair(d + 4, f + XSF_A);
-            tc_copy_factors_pair(d + 8, f + XSF_A + 512);
+            const uint32_t f = smem_u32(factors + stage * XSF_BYTES);
+            sf = tmem_base + XSF_COL + set * XSF_SET;
+            tc_copy_factors_pair(sf, f);
+            tc_copy_factors_pair(sf + 4, f + XSF_A);
+            tc_copy_factors_pair(sf + 8, f + XSF_A + 512);
+            if (++set == XSF_SETS) set = 0;
           }
-          const uint32_t sf = tmem_base + XSF_COL + set * XSF_SET;
+          const uint32_t a_addr = smem_u32(tiles + stage * XSTAGE_BYTES);
           const uint32_t id = idesc | ((uint32_t)(kb & 3) << 4) | ((uint32_t)(kb & 3) << 29);
           const uint64_t da = a_mn ? make_smem_desc_mn(a_addr, PA_BYTES) : make_smem_desc(a_addr);
           const uint64_t db = b_mn ? make_smem_desc_mn(a_addr + PA_BYTES, PB_BYTES) : make_smem_desc(a_addr + PA_BYTES);
@@ -741,6 +774,13 @@ gemm_block_scaled_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid
         }
         if (!ok) break;
         tc_commit_pair(&bars->tmem_full[acc]);
+        if (sched != nullptr) {
+          const int32_t v = pair_ring_read(bars, local, peer, 16u, 0u);
+          if (v == -2) { ok = false; break; }
+          t = v < 0 ? num_tiles : (int64_t)v;
+        } else {
+          t += num_clusters;
+        }
       }
     }
   } else {
@@ -750,14 +790,14 @@ gemm_block_scaled_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid
                                 staging + (warp - 2) * 2 * EPI_BOX_BYTES, 1.0f, 1, nullptr};
     const uint32_t free_in_leader = mapa_u32(smem_u32(&bars->tmem_shared_free), 0u);
     uint32_t boxes = 0, local = 0;
-    bool ok = true;
-    for (int64_t t = cluster_id; ok && t < num_tiles; t += num_clusters, ++local) {
+    int64_t t = cluster_id;
+    for (; t < num_tiles; ++local) {
       const TileCoord tc = tile_coord(t, tiles_m, tiles_n, raster);
       const uint32_t acc = local & 1u;
       int got = 1;
       if (lane == 0) got = pair_wait(&bars->tmem_full[acc], (local >> 1) & 1u, bars, peer, 8u, WAIT_BY_HINT | 1000u) ? 1 : 0;
       got = __shfl_sync(0xFFFFFFFFu, got, 0);
-      if (got == 0) { ok = false; break; }
+      if (got == 0) break;
       tc_fence_after();
       const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * (uint32_t)XACC_STEP;
       const int row0 = tc.m * PBM + (int)rank * 128 + quarter * 32;
@@ -774,6 +814,14 @@ gemm_block_scaled_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid
           if (lane == 0) mbar_arrive_cluster(free_in_leader);
         }
         store_columns<OutT>(ea, r, row0, tc.n * PBN + part * 64, boxes);
+      }
+      if (sched != nullptr) {
+        int v = 0;
+        if (lane == 0) v = pair_ring_read(bars, local, peer, 32u, 64u);
+        v = __shfl_sync(0xFFFFFFFFu, v, 0);
+        t = v < 0 ? num_tiles : (int64_t)v;  // no more tiles, or gave up
+      } else {
+        t += num_clusters;
       }
     }
     if (use_tma_store && lane == 0) bulk_wait_all();
@@ -851,7 +899,7 @@ static int encode_exponent_map(CUtensorMap* map, const void* base, int64_t rows,
 template <typename OutT>
 static int launch_block_scaled(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mea, const CUtensorMap& meb,
                                const CUtensorMap& mo, int use_tma, const void* bias, void* out, int64_t ldo, int m, int n,
-                               int k, uint32_t idesc, int vec_ok, int layouts, cudaStream_t st) {
+                               int k, uint32_t idesc, int vec_ok, int layouts, uint32_t* sched, cudaStream_t st) {
   static PerDeviceOnce setup;
   int max_clusters = 0;
   auto kernel = gemm_block_scaled_kernel<OutT>;
@@ -883,9 +931,14 @@ static int launch_block_scaled(const CUtensorMap& ma, const CUtensorMap& mb, con
   if (persistent_ctas() / 2 < clusters) clusters = persistent_ctas() / 2;
   if (tiles < clusters) clusters = (int)tiles;
   cfg.gridDim = dim3(2 * clusters);
+  sched = usable_sched(sched, tiles, clusters);
+  if (sched != nullptr) {
+    const cudaError_t e = cudaMemsetAsync(sched, 0, sizeof(uint32_t), st);
+    if (e != cudaSuccess) return record_cuda_error(e);
+  }
   return record_cuda_error(cudaLaunchKernelEx(&cfg, kernel, ma, mb, mea, meb, mo, static_cast<const OutT*>(bias),
                                               static_cast<OutT*>(out), ldo, m, n, k, idesc, vec_ok, use_tma,
-                                              choose_raster(m, n, k, PBM, PBN) | layouts));
+                                              choose_raster(m, n, k, PBM, PBN) | layouts, sched));
 }
 
 template <typename OutT, int T>
@@ -937,12 +990,15 @@ extern "C" int f8b200_gemm_blockwise(const void* a, int a_kind, int a_layout, in
                                      const void* exp_a, const void* b,
                                      int b_kind, int b_layout, int64_t ldb, const float* scale_b, int64_t sb_row_stride,
                                      int64_t sb_kb_stride, int b_block_rows, const void* exp_b, const void* bias,
-                                     int out_dtype, void* out, int64_t ldo, int64_t m, int64_t n, int64_t k, void* stream) {
+                                     int out_dtype, void* out, int64_t ldo, int64_t m, int64_t n, int64_t k,
+                                     void* workspace, int64_t workspace_bytes, void* stream) {
   using namespace gemm::block;
   if ((a_block_rows != 1 && a_block_rows != 128) || (b_block_rows != 1 && b_block_rows != 128)) return F8B200_ERR_BAD_ARG;
   const BlockScale sa{scale_a, sa_row_stride, sa_kb_stride, a_block_rows == 128 ? 7 : 0};
   const BlockScale sb{scale_b, sb_row_stride, sb_kb_stride, b_block_rows == 128 ? 7 : 0};
   if (!strides_ok(sa) || !strides_ok(sb)) return F8B200_ERR_BAD_ARG;
+  if (workspace != nullptr && workspace_bytes < F8B200_GEMM_WORKSPACE_BYTES) return F8B200_ERR_BAD_ARG;
+  if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return F8B200_ERR_ALIGNMENT;
   bool empty = false;
   int rc = gemm_fp8_validate(a, a_kind, a_layout, lda, b, b_kind, b_layout, ldb, scale_a, scale_b, bias, out_dtype, out,
                              ldo, m, n, k, &empty);
@@ -988,7 +1044,8 @@ extern "C" int f8b200_gemm_blockwise(const void* a, int a_kind, int a_layout, in
     return dispatch_out_dtype(out_dtype, [&](auto* tag) {
       using OutT = std::remove_pointer_t<decltype(tag)>;
       return launch_block_scaled<OutT>(ma, mb, mea, meb, mo, vec_ok, bias, out, ldo, (int)m, (int)n, (int)k,
-                                       make_idesc_scaled(a_kind, b_kind, a_layout, b_layout), vec_ok, layouts, st);
+                                       make_idesc_scaled(a_kind, b_kind, a_layout, b_layout), vec_ok, layouts,
+                                       static_cast<uint32_t*>(workspace), st);
     });
   }
   const uint32_t idesc = gemm::pair::make_idesc_pair(a_kind, b_kind, a_layout, b_layout);

@@ -439,14 +439,16 @@ int f8b200_uncast_blockwise(const void* q, int fp8_kind, int64_t rows, int64_t c
  * at scale_a[(m / a_block_rows) * sa_row_stride + j * sa_kb_stride], a_block_rows 1 or 128, strides >= 0
  * (elements); B's likewise.  Factors are arbitrary fp32 values.  exp_a and exp_b (each may be NULL) are the exponent
  * bytes that f8b200_cast_blockwise wrote beside those factors; with both given, products of more than a few rows let
- * the tensor cores apply them.  `bias` has out_dtype or is NULL.  Needs no workspace.
+ * the tensor cores apply them.  `bias` has out_dtype or is NULL.  `workspace` (F8B200_GEMM_WORKSPACE_BYTES, 16-byte
+ * aligned, not shared with another launch that may run at the same time) lets those products hand out their tiles
+ * dynamically; it may be NULL.
  */
 int f8b200_gemm_blockwise(const void* a, int a_kind, int a_layout, int64_t lda, const float* scale_a,
                           int64_t sa_row_stride, int64_t sa_kb_stride, int a_block_rows,
                           const void* exp_a, const void* b, int b_kind, int b_layout, int64_t ldb,
                           const float* scale_b, int64_t sb_row_stride, int64_t sb_kb_stride,
                           int b_block_rows, const void* exp_b, const void* bias, int out_dtype, void* out, int64_t ldo, int64_t m, int64_t n,
-                          int64_t k, void* stream);
+                          int64_t k, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Layer norm over the columns of x [rows, cols], T = hp_dtype:

@@ -116,11 +116,12 @@ def test_c_argument_checks_come_before_any_cuda_call():
     assert unc(y=vp(257)) == -2 and unc(rows=0) == 0
     mm = lambda **k: lib.f8b200_gemm_blockwise(*{**dict(  # noqa: E731
         a=P, ak=0, al=0, lda=16, sa=P, sar=1, sak=1, ab=1, ea=None, b=P, bk=0, bl=0, ldb=16, sb=P, sbr=1, sbk=1, bb=128, eb=None, bias=None,
-        dt=0, out=P, ldo=4, m=4, n=4, k=16, st=None), **k}.values())
+        dt=0, out=P, ldo=4, m=4, n=4, k=16, ws=None, wsb=0, st=None), **k}.values())
     assert mm(m=0) == 0 and mm(n=0) == 0 and mm(k=0) == -6
     assert mm(lda=24) == -2 and mm(a=vp(264)) == -2
     assert mm(a=None) == -1 and mm(sa=None) == -1 and mm(ldo=3) == -1 and mm(dt=3) == -1 and mm(k=-1) == -1
     assert mm(ab=2) == -1 and mm(bb=64) == -1 and mm(sar=-1) == -1 and mm(sbk=-1) == -1
+    assert mm(ws=Q, wsb=255) == -1 and mm(ws=vp(4104), wsb=256) == -2
     ln = lambda **k: lib.f8b200_layer_norm(*{**dict(  # noqa: E731
         x=P, dt=0, rows=4, cols=8, ld=8, w=P, b=P, at=0, eps=1e-5, y=P, ldy=8, mean=None, rstd=None, st=None), **k}.values())
     for bad in (dict(x=None), dict(y=None), dict(cols=0), dict(rows=-1), dict(ld=7), dict(ldy=7), dict(at=1), dict(dt=4),
