@@ -171,6 +171,203 @@ ln_fwd_kernel(const T* __restrict__ x, int64_t ld_x, int64_t rows, int64_t cols,
   }
 }
 
+// ---- backward, rows through a ring of private slots -----------------------------------------------------
+// Each thread copies its own 16-byte pieces of the coming rows of x and g to shared memory (cp.async, STAGES - 1 rows
+// ahead) and reads back only those: the memory system is kept busy across the row sums without a barrier for the
+// data.  dw and db gather in registers over all rows of the CTA, which leaves one partial sum per CTA: x and g are read
+// once for all three gradients.
+constexpr int kBwdThreads = 512;
+
+__device__ __forceinline__ void cp_async16(void* smem, const void* gmem) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(smem)), "l"(gmem) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// N affine values held as they lie in memory, so that they cost few registers over the whole loop.
+template <typename W, int N>
+struct Packed {
+  static constexpr int Q = N / Vec<W>::N;
+  uint4 q[Q];
+  __device__ __forceinline__ void load(const W* p, int64_t i) {
+#pragma unroll
+    for (int h = 0; h < Q; ++h) q[h] = __ldg(reinterpret_cast<const uint4*>(p + i) + h);
+  }
+  __device__ __forceinline__ void set_one() {
+    float v[Vec<W>::N];
+#pragma unroll
+    for (int j = 0; j < Vec<W>::N; ++j) v[j] = 1.f;
+#pragma unroll
+    for (int h = 0; h < Q; ++h) q[h] = Vec<W>::narrow(v);
+  }
+  __device__ __forceinline__ void get(float (&v)[N]) const {
+#pragma unroll
+    for (int h = 0; h < Q; ++h) {
+      float t[Vec<W>::N];
+      Vec<W>::widen(q[h], t);
+#pragma unroll
+      for (int j = 0; j < Vec<W>::N; ++j) v[h * Vec<W>::N + j] = t[j];
+    }
+  }
+};
+
+template <typename T, typename W, int ROWT, int CH, int R, int STAGES>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+ln_bwd_kernel(const T* __restrict__ x, int64_t ld_x, const T* __restrict__ g, int64_t ld_g, int64_t rows, int64_t cols,
+              const W* __restrict__ weight, const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
+              T* __restrict__ dx, int64_t ld_dx, float* __restrict__ part) {
+  constexpr int N = Vec<T>::N, GROUPS = kBwdThreads / ROWT, WARPS = ROWT / 32;
+  extern __shared__ uint4 ring[];  // [STAGES][R rows][x, g][CH][thread]
+  __shared__ float sums[2][kBwdThreads / 32][2 * R];
+  const int t = threadIdx.x % ROWT, group = threadIdx.x / ROWT, lane = threadIdx.x & 31;
+  const int chunks = (int)(cols / N);
+  const float inv_c = 1.0f / (float)cols;
+  // a group takes R rows at a time: one exchange of sums serves them all
+  const int64_t sets = (rows + R - 1) / R, step = (int64_t)gridDim.x * GROUPS;
+  auto slot = [&](int stage, int u, int which, int i) {
+    return ring + (((stage * R + u) * 2 + which) * CH + i) * kBwdThreads + threadIdx.x;
+  };
+  auto fetch = [&](int64_t p, int stage) {
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+      const int64_t r = R * p + u;
+      if (r < rows) {
+        const uint4 *xr = reinterpret_cast<const uint4*>(x + r * ld_x), *gr = reinterpret_cast<const uint4*>(g + r * ld_g);
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+          const int c = t + i * ROWT;
+          if (c < chunks) {
+            cp_async16(slot(stage, u, 0, i), xr + c);
+            cp_async16(slot(stage, u, 1, i), gr + c);
+          }
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto stats = [&](int64_t p, float (&mean)[R], float (&rstd)[R]) {
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+      const bool in = R * p + u < rows;
+      mean[u] = in ? __ldg(mean_in + R * p + u) : 0.f;
+      rstd[u] = in ? __ldg(rstd_in + R * p + u) : 0.f;
+    }
+  };
+
+  float dw[CH][N], db[CH][N];
+  Packed<W, N> w[CH];
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    if (weight != nullptr && t + i * ROWT < chunks) w[i].load(weight, (int64_t)(t + i * ROWT) * N);
+    else w[i].set_one();
+#pragma unroll
+    for (int j = 0; j < N; ++j) dw[i][j] = db[i][j] = 0.f;
+  }
+
+  int64_t p = (int64_t)blockIdx.x * GROUPS + group;
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s) fetch(p + s * step, s);
+  float mean[R], rstd[R];
+  stats(p, mean, rstd);
+  int stage = 0, flip = 0;
+  for (; p < sets; p += step) {
+    float mean_next[R], rstd_next[R];
+    stats(p + step, mean_next, rstd_next);  // their latency passes behind this set's work
+    cp_async_wait<STAGES - 2>();
+    float s[2 * R] = {};
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+      const bool row_in = R * p + u < rows;
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const bool in = row_in && t + i * ROWT < chunks;
+        float xv[N], gv[N], wv[N];
+        Vec<T>::widen(in ? *slot(stage, u, 0, i) : make_uint4(0u, 0u, 0u, 0u), xv);
+        Vec<T>::widen(in ? *slot(stage, u, 1, i) : make_uint4(0u, 0u, 0u, 0u), gv);
+        w[i].get(wv);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {  // where there is no element, g is 0 and so is everything below
+          const float n = (xv[j] - mean[u]) * rstd[u], h = gv[j] * wv[j];
+          s[2 * u] += h;
+          s[2 * u + 1] = fmaf(h, n, s[2 * u + 1]);
+          dw[i][j] = fmaf(gv[j], n, dw[i][j]);
+          db[i][j] += gv[j];
+        }
+      }
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1)
+#pragma unroll
+      for (int q = 0; q < 2 * R; ++q) s[q] += __shfl_xor_sync(0xFFFFFFFFu, s[q], off);
+    if constexpr (WARPS > 1) {  // two buffers: the next set's sums may be written while these are read
+      if (lane == 0) {
+#pragma unroll
+        for (int q = 0; q < 2 * R; ++q) sums[flip][threadIdx.x >> 5][q] = s[q];
+      }
+      if constexpr (ROWT == kBwdThreads) __syncthreads();
+      else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(ROWT) : "memory");
+#pragma unroll
+      for (int q = 0; q < 2 * R; ++q) {
+        s[q] = 0.f;
+#pragma unroll
+        for (int v = 0; v < WARPS; ++v) s[q] += sums[flip][group * WARPS + v][q];
+      }
+      flip ^= 1;
+    }
+    fetch(p + (STAGES - 1) * step, stage == 0 ? STAGES - 1 : stage - 1);
+    if (dx != nullptr) {
+#pragma unroll
+      for (int u = 0; u < R; ++u) {
+        if (R * p + u >= rows) continue;
+        const float a = s[2 * u] * inv_c, b = s[2 * u + 1] * inv_c;
+        uint4* out = reinterpret_cast<uint4*>(dx + (R * p + u) * ld_dx);
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+          const int c = t + i * ROWT;
+          if (c < chunks) {
+            float xv[N], gv[N], wv[N];
+            Vec<T>::widen(*slot(stage, u, 0, i), xv);  // still there: held in registers the rows would cost 32 of them
+            Vec<T>::widen(*slot(stage, u, 1, i), gv);
+            w[i].get(wv);
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+              const float n = (xv[j] - mean[u]) * rstd[u];
+              gv[j] = rstd[u] * (fmaf(gv[j], wv[j], -a) - n * b);
+            }
+            __stcs(out + c, Vec<T>::narrow(gv));
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < R; ++u) mean[u] = mean_next[u], rstd[u] = rstd_next[u];
+    if (++stage == STAGES) stage = 0;
+  }
+  if (part == nullptr) return;
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  // the groups' sums over each other, dw and db in turn, through the ring
+  float* sm = reinterpret_cast<float*>(ring);
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+      if (t + i * ROWT < chunks) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) sm[group * cols + (int64_t)(t + i * ROWT) * N + j] = which == 0 ? dw[i][j] : db[i][j];
+      }
+    __syncthreads();
+    for (int c = threadIdx.x; c < (int)cols; c += kBwdThreads) {
+      float v = 0.f;
+#pragma unroll
+      for (int q = 0; q < GROUPS; ++q) v += sm[q * cols + c];
+      part[((int64_t)blockIdx.x * 2 + which) * cols + c] = v;
+    }
+  }
+}
+
 // ---- any width, any alignment -----------------------------------------------------------------------
 template <typename T, typename W>
 __global__ void __launch_bounds__(kThreads)
@@ -309,10 +506,52 @@ int ln_fwd(const void* x, int64_t rows, int64_t cols, int64_t ld_x, const void* 
   return check_launch();
 }
 
+template <typename T, typename W, int ROWT, int CH, int R, int STAGES>
+int ln_bwd_launch(const T* x, int64_t ld_x, const T* g, int64_t ld_g, int64_t rows, int64_t cols, const W* weight,
+                  const float* mean, const float* rstd, T* dx, int64_t ld_dx, float* part, int* parts, cudaStream_t st) {
+  constexpr int kGroups = kBwdThreads / ROWT;
+  constexpr int kSmem = STAGES * R * 2 * CH * kBwdThreads * 16;
+  static_assert(kGroups * ROWT * CH * Vec<T>::N * 4 <= kSmem, "the groups' sums have to fit into the ring");
+  static PerDeviceOnce setup;
+  auto kernel = ln_bwd_kernel<T, W, ROWT, CH, R, STAGES>;
+  const cudaError_t e = setup.run([&](int*) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem); });
+  if (e != cudaSuccess) return record_cuda_error(e);
+  const int64_t need = ((rows + R - 1) / R + kGroups - 1) / kGroups;
+  int64_t grid = sm_count() < kMaxParts ? sm_count() : kMaxParts;
+  if (need < grid) grid = need;
+  kernel<<<(unsigned)grid, kBwdThreads, kSmem, st>>>(x, ld_x, g, ld_g, rows, cols, weight, mean, rstd, dx, ld_dx, part);
+  *parts = (int)grid;
+  return check_launch();
+}
+
 template <typename T, typename W>
 int ln_bwd(const void* x, const void* g, int64_t rows, int64_t cols, int64_t ld_x, int64_t ld_g, const void* weight,
            const float* mean, const float* rstd, void* dx, int64_t ld_dx, void* dw, void* db, float* part, cudaStream_t st) {
   const T *xp = static_cast<const T*>(x), *gp = static_cast<const T*>(g);
+  constexpr int N = Vec<T>::N;
+  const int64_t chunks = cols / N;
+  const bool vec = cols % N == 0 && chunks <= 2048 && ld_x % N == 0 && ld_g % N == 0 && (dx == nullptr || ld_dx % N == 0) &&
+                   aligned16(x) && aligned16(g) && aligned16(dx) && aligned16(weight);
+  if (vec) {
+    int parts = 0, rc = F8B200_OK;
+    float* sums = dw != nullptr || db != nullptr ? part : nullptr;
+#define F8_LN(ROWT, CH, R, STAGES)                                                                                           \
+  rc = ln_bwd_launch<T, W, ROWT, CH, R, STAGES>(xp, ld_x, gp, ld_g, rows, cols, static_cast<const W*>(weight), mean, rstd, \
+                                             static_cast<T*>(dx), ld_dx, sums, &parts, st)
+    // the narrowest group of threads that takes a row in two pieces each: 32 accumulators for 16-bit rows
+    if (chunks <= 64) F8_LN(32, 2, 2, 3);
+    else if (chunks <= 128) F8_LN(64, 2, 2, 3);
+    else if (chunks <= 256) F8_LN(128, 2, 2, 3);
+    else if (chunks <= 512) F8_LN(256, 2, 2, 3);
+    else if (chunks <= 1024) F8_LN(512, 2, 1, 6);
+    else F8_LN(512, 4, 1, 3);
+#undef F8_LN
+    if (rc != F8B200_OK) return rc;
+    if (sums != nullptr)
+      ln_dw_join_kernel<W><<<(unsigned)((cols + 31) / 32), kThreads, 0, st>>>(part, parts, cols, static_cast<W*>(dw),
+                                                                            static_cast<W*>(db));
+    return check_launch();
+  }
   if (dx != nullptr)
     ln_dx_any_kernel<T, W><<<row_grid(rows), kThreads, 0, st>>>(xp, ld_x, gp, ld_g, rows, cols, static_cast<const W*>(weight),
                                                                 mean, rstd, static_cast<T*>(dx), ld_dx);
