@@ -55,51 +55,50 @@ __device__ __forceinline__ void block_scale(uint32_t amax_bits, float& up, float
 }
 
 template <int HP>
-__device__ __forceinline__ uint32_t widen_bits(uint32_t h) {  // |x| bits of T -> fp32 bits
+__device__ __forceinline__ uint32_t widen_bits(uint32_t h) {  // |x| bits of a 16-bit type -> fp32 bits
   if constexpr (HP == F8B200_BF16) return h << 16;
   else return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
 }
 
-// Eight consecutive elements of a row as fp32; `n` of them exist.
-template <int HP, bool VEC>
-__device__ __forceinline__ void load8(const char* p, int n, float (&v)[8]) {
-  if constexpr (HP == F8B200_FP32) {
-    const float* f = reinterpret_cast<const float*>(p);
+// Eight consecutive elements of a row as they lie in memory: 16-bit types stay packed (half the registers, and two
+// maxima per instruction).
+template <int HP>
+struct Eight {
+  static constexpr int W = HP == F8B200_FP32 ? 8 : 4;
+  uint32_t w[W];
+
+  template <bool VEC>
+  __device__ __forceinline__ void load(const char* p, int n) {  // n of them exist
+#pragma unroll
+    for (int j = 0; j < W; ++j) w[j] = 0u;
     if constexpr (VEC) {
       if (n > 0) {
-        const float4 a = __ldcs(reinterpret_cast<const float4*>(f)), b = __ldcs(reinterpret_cast<const float4*>(f) + 1);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        return;
-      }
-    }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < n ? __ldcs(f + j) : 0.f;
-  } else {
-    const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
-    uint32_t w[4] = {0u, 0u, 0u, 0u};
-    if (VEC) {
-      if (n > 0) {
-        const uint4 q = __ldcs(reinterpret_cast<const uint4*>(p));
-        w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
+        for (int h = 0; h < W / 4; ++h) {
+          const uint4 q = __ldcs(reinterpret_cast<const uint4*>(p) + h);
+          w[4 * h] = q.x, w[4 * h + 1] = q.y, w[4 * h + 2] = q.z, w[4 * h + 3] = q.w;
+        }
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j < n) w[j >> 1] |= (uint32_t)__ldcs(h + j) << (16 * (j & 1));
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if constexpr (HP == F8B200_BF16) {
-        v[2 * j] = __uint_as_float(w[j] << 16);
-        v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
-      } else {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-        v[2 * j] = f.x;
-        v[2 * j + 1] = f.y;
+      for (int j = 0; j < 8; ++j) {
+        if (j < n) {
+          if constexpr (HP == F8B200_FP32) w[j] = __ldcs(reinterpret_cast<const uint32_t*>(p) + j);
+          else w[j >> 1] |= (uint32_t)__ldcs(reinterpret_cast<const unsigned short*>(p) + j) << (16 * (j & 1));
+        }
       }
     }
   }
-}
+  // element pair j as fp32
+  __device__ __forceinline__ float2 pair(int j) const {
+    if constexpr (HP == F8B200_FP32) return make_float2(__uint_as_float(w[2 * j]), __uint_as_float(w[2 * j + 1]));
+    else if constexpr (HP == F8B200_BF16) return make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u));
+    else return __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+  }
+  // |x| bits of word j, and the larger of two such words: unsigned order is the order of the values, NaN above infinity
+  __device__ __forceinline__ uint32_t abs_word(int j) const { return w[j] & (HP == F8B200_FP32 ? 0x7FFFFFFFu : 0x7FFF7FFFu); }
+  __device__ __forceinline__ static uint32_t larger(uint32_t a, uint32_t b) { return HP == F8B200_FP32 ? max(a, b) : __vmaxu2(a, b); }
+};
 
 template <bool VEC>
 __device__ __forceinline__ void store8(uint8_t* p, int n, uint32_t lo, uint32_t hi) {
@@ -113,51 +112,59 @@ __device__ __forceinline__ void store8(uint8_t* p, int n, uint32_t lo, uint32_t 
 }
 
 template <int HP, int KIND, int FORMS, bool VEC>
-__global__ void __launch_bounds__(kThreads) cast_block_kernel(const BlockCastArgs p) {
-  __shared__ uint32_t col_max[kThreads / 32][kBlk];
+__global__ void __launch_bounds__(kThreads, HP == F8B200_FP32 ? 2 : (FORMS == kByRow || FORMS == kByCol) ? 4 : 3) cast_block_kernel(const BlockCastArgs p) {
+  __shared__ __align__(16) uint32_t col_max[kThreads / 32][16 * Eight<HP>::W];
   __shared__ uint32_t warp_max[kThreads / 32];
+  __shared__ float factors[2][kBlk];
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t tm = blockIdx.x / p.tiles_k, tk = blockIdx.x - tm * p.tiles_k;
   const int64_t row0 = tm * kBlk, col = tk * kBlk + tx * 8;
   const int n = (int)max((int64_t)0, min((int64_t)8, p.cols - col));
   constexpr int kEs = HP == F8B200_FP32 ? 4 : 2;
 
-  float v[8][8];
+  using V = Eight<HP>;
+  constexpr int W = V::W;
+  V v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int64_t r = row0 + ty + 16 * i;
-    load8<HP, VEC>(p.x + (r * p.ld + col) * kEs, r < p.rows ? n : 0, v[i]);
+    v[i].template load<VEC>(p.x + (r * p.ld + col) * kEs, r < p.rows ? n : 0);
   }
 
-  uint32_t rmax[8];  // |x| bits, fp32: unsigned order is the order of the values, NaN above infinity
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[i][j]) & 0x7FFFFFFFu);
-    rmax[i] = m;
-  }
   if constexpr (FORMS & kByCol) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      uint32_t m = 0;
+    for (int j = 0; j < W; ++j) {
+      uint32_t m = v[0].abs_word(j);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i][j]) & 0x7FFFFFFFu);
-      m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 16));
-      if (lane < 16) col_max[warp][tx * 8 + j] = m;
+      for (int i = 1; i < 8; ++i) m = V::larger(m, v[i].abs_word(j));
+      m = V::larger(m, __shfl_xor_sync(0xFFFFFFFFu, m, 16));
+      if (lane < 16) col_max[warp][tx * W + j] = m;
     }
   }
+  uint32_t rmax[8];  // fp32: |x| bits; 16 bits: of rows 2i and 2i + 1 in rmax[i]
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    uint32_t m = v[i].abs_word(0);
+#pragma unroll
+    for (int j = 1; j < W; ++j) m = V::larger(m, v[i].abs_word(j));
+    if constexpr (HP == F8B200_FP32) {
+      rmax[i] = m;
+    } else {
+      m = max(m & 0xFFFFu, m >> 16);
+      if (i & 1) rmax[i >> 1] |= m << 16;
+      else rmax[i >> 1] = m;
+    }
+  }
+  constexpr int R = HP == F8B200_FP32 ? 8 : 4;
   float up_sq = 0.f;
   if constexpr (FORMS & kBySquare) {
-    uint32_t m = 0;
+    uint32_t m = rmax[0];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, rmax[i]);
+    for (int i = 1; i < R; ++i) m = V::larger(m, rmax[i]);
+    if constexpr (HP != F8B200_FP32) m = widen_bits<HP>(max(m & 0xFFFFu, m >> 16));
     m = warp_max_u32(m);
     if (lane == 0) warp_max[warp] = m;
-  }
-  if constexpr ((FORMS & (kByCol | kBySquare)) != 0) __syncthreads();
-  if constexpr (FORMS & kBySquare) {
-    uint32_t m = 0;
+    __syncthreads();
 #pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) m = max(m, warp_max[w]);
     float down;
@@ -171,39 +178,47 @@ __global__ void __launch_bounds__(kThreads) cast_block_kernel(const BlockCastArg
   }
 
   if constexpr (FORMS & (kByRow | kBySquare)) {
+    if constexpr (FORMS & kByRow) {
+#pragma unroll
+      for (int off = 8; off > 0; off >>= 1)
+#pragma unroll
+        for (int i = 0; i < R; ++i) rmax[i] = V::larger(rmax[i], __shfl_xor_sync(0xFFFFFFFFu, rmax[i], off));
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int64_t r = row0 + ty + 16 * i;
       float up = up_sq;
       if constexpr (FORMS & kByRow) {
-        uint32_t m = rmax[i];
-#pragma unroll
-        for (int off = 8; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, off));
         float down;
+        uint32_t m = rmax[i / (8 / R)];
+        if constexpr (HP != F8B200_FP32) m = widen_bits<HP>((i & 1) ? m >> 16 : m & 0xFFFFu);
         block_scale<KIND>(m, up, down);
-        if (tx == 0 && r < p.rows) {
-          p.scale_r[tk * p.ld_scale_r + r] = down;
-          if (p.exp_r != nullptr) p.exp_r[exponent_at(r, tk, p.exp_pitch_r)] = exponent_of(down);
-        }
+        if (tx == 0) factors[0][ty + 16 * i] = down;
       }
       uint32_t w[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = cvt_pair_raw<KIND>(v[i][2 * j] * up, v[i][2 * j + 1] * up);
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = v[i].pair(j);
+        w[j] = cvt_pair_raw<KIND>(f.x * up, f.y * up);
+      }
       if (r < p.rows) store8<VEC>(p.out_r + r * p.ld_r + col, n, w[0] | (w[1] << 16), w[2] | (w[3] << 16));
     }
   }
   if constexpr (FORMS & kByCol) {
+    __syncthreads();  // behind the rows' work: the column maxima of the other warps have had time to arrive
     float up[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      uint32_t m = 0;
+    for (int j = 0; j < W; ++j) {
+      uint32_t m = col_max[0][tx * W + j];
 #pragma unroll
-      for (int w = 0; w < kThreads / 32; ++w) m = max(m, col_max[w][tx * 8 + j]);
-      float down;
-      block_scale<KIND>(m, up[j], down);
-      if (ty == 0 && j < n) {
-        p.scale_c[tm * p.ld_scale_c + col + j] = down;
-        if (p.exp_c != nullptr) p.exp_c[exponent_at(col + j, tm, p.exp_pitch_c)] = exponent_of(down);
+      for (int w = 1; w < kThreads / 32; ++w) m = V::larger(m, col_max[w][tx * W + j]);
+#pragma unroll
+      for (int h = 0; h < 8 / W; ++h) {
+        const int c = j * (8 / W) + h;
+        float down;
+        if constexpr (HP == F8B200_FP32) block_scale<KIND>(m, up[c], down);
+        else block_scale<KIND>(widen_bits<HP>(h ? m >> 16 : m & 0xFFFFu), up[c], down);
+        if (ty == 0) factors[1][tx * 8 + c] = down;
       }
     }
 #pragma unroll
@@ -211,8 +226,30 @@ __global__ void __launch_bounds__(kThreads) cast_block_kernel(const BlockCastArg
       const int64_t r = row0 + ty + 16 * i;
       uint32_t w[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = cvt_pair_raw<KIND>(v[i][2 * j] * up[2 * j], v[i][2 * j + 1] * up[2 * j + 1]);
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = v[i].pair(j);
+        w[j] = cvt_pair_raw<KIND>(f.x * up[2 * j], f.y * up[2 * j + 1]);
+      }
       if (r < p.rows) store8<VEC>(p.out_c + r * p.ld_c + col, n, w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+    }
+  }
+  if constexpr ((FORMS & (kByRow | kByCol)) != 0) {
+    // the tile's factors leave together, neighbours from neighbouring threads: stored by the threads that found them,
+    // one here and one there, they cost as much as the bytes (330 against 148 us for both forms of 16384 x 8192 bf16)
+    __syncthreads();
+    const int t = threadIdx.x & 127;
+    if (threadIdx.x < 128) {
+      const int64_t r = row0 + t;
+      if ((FORMS & kByRow) && r < p.rows) {
+        p.scale_r[tk * p.ld_scale_r + r] = factors[0][t];
+        if (p.exp_r != nullptr) p.exp_r[exponent_at(r, tk, p.exp_pitch_r)] = exponent_of(factors[0][t]);
+      }
+    } else {
+      const int64_t c = tk * kBlk + t;
+      if ((FORMS & kByCol) && c < p.cols) {
+        p.scale_c[tm * p.ld_scale_c + c] = factors[1][t];
+        if (p.exp_c != nullptr) p.exp_c[exponent_at(c, tm, p.exp_pitch_c)] = exponent_of(factors[1][t]);
+      }
     }
   }
 }
@@ -227,17 +264,17 @@ int launch_forms(const BlockCastArgs& p, int forms, int64_t tiles, cudaStream_t 
   return check_launch();
 }
 
-// fp8 -> T: y = q * scale_inv(block).  16 consecutive columns per thread; they share a factor unless the blocks are
-// one column wide (16 divides 128).
+// fp8 -> T: y = q * scale(block), in the tiles of the cast: 8 columns and 8 rows, 16 apart, per thread, so that
+// column factors are fetched once for eight rows.
 struct BlockUncastArgs {
   const uint8_t* q;
   int64_t rows, cols, ld_q;
   const float* scale;
-  int64_t s_row, s_col;    // strides of the factors
+  int64_t s_row, s_col;      // strides of the factors
   int row_shift, col_shift;  // 7: one factor per 128 rows / columns, 0: per row / column
   char* y;
   int64_t ld_y;
-  int64_t chunks;  // ceil(cols / 16)
+  int64_t tiles_k;
 };
 
 template <int HP>
@@ -250,45 +287,69 @@ __device__ __forceinline__ void store_hp(char* base, int64_t i, float v) {
 template <int HP, int KIND, bool VEC>
 __global__ void __launch_bounds__(kThreads) uncast_block_kernel(const BlockUncastArgs p) {
   constexpr __nv_fp8_interpretation_t kInterp = KIND == F8B200_E4M3 ? __NV_E4M3 : __NV_E5M2;
-  const int64_t total = p.rows * p.chunks;
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
-    const int64_t r = i / p.chunks, c = (i - r * p.chunks) * 16;
-    const int n = (int)min((int64_t)16, p.cols - c);
-    const uint8_t* q = p.q + r * p.ld_q + c;
-    uint32_t w[4] = {0u, 0u, 0u, 0u};
-    if constexpr (VEC) {
-      const uint4 t = __ldcs(reinterpret_cast<const uint4*>(q));
-      w[0] = t.x, w[1] = t.y, w[2] = t.z, w[3] = t.w;
-    } else {
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int64_t tm = blockIdx.x / p.tiles_k, tk = blockIdx.x - tm * p.tiles_k;
+  const int64_t row0 = tm * kBlk, col = tk * kBlk + tx * 8;
+  const int n = (int)max((int64_t)0, min((int64_t)8, p.cols - col));
+  if (n == 0) return;
+  uint32_t w[8][2];
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (j < n) w[j >> 2] |= (uint32_t)q[j] << (8 * (j & 3));
-    }
-    const float* sp = p.scale + (r >> p.row_shift) * p.s_row;
-    float y[16];
-    const float s0 = __ldg(sp + (c >> p.col_shift) * p.s_col);
+  for (int i = 0; i < 8; ++i) {
+    const int64_t r = row0 + ty + 16 * i;
+    const uint8_t* q = p.q + r * p.ld_q + col;
+    w[i][0] = w[i][1] = 0u;
+    if (r < p.rows) {
+      if constexpr (VEC) {
+        const uint2 t = __ldcs(reinterpret_cast<const uint2*>(q));
+        w[i][0] = t.x, w[i][1] = t.y;
+      } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((w[j >> 1] >> (16 * (j & 1))) & 0xFFFFu), kInterp);
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-      float sa = s0, sb = s0;
-      if (p.col_shift == 0) {
-        sa = 2 * j < n ? __ldg(sp + (c + 2 * j) * p.s_col) : 0.f;
-        sb = 2 * j + 1 < n ? __ldg(sp + (c + 2 * j + 1) * p.s_col) : 0.f;
+        for (int j = 0; j < 8; ++j)
+          if (j < n) w[i][j >> 2] |= (uint32_t)q[j] << (8 * (j & 3));
       }
-      y[2 * j] = f.x * sa;
-      y[2 * j + 1] = f.y * sb;
+    }
+  }
+  float sc[8], sr[8];  // factors of the columns, or, where blocks are 128 columns wide, of the rows
+  const bool per_col = p.col_shift == 0, per_row = p.row_shift == 0;
+  if (per_col) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sc[j] = j < n ? __ldg(p.scale + (row0 >> p.row_shift) * p.s_row + (col + j) * p.s_col) : 0.f;
+  }
+  if (!per_col) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int64_t r = row0 + ty + 16 * i;
+      sr[i] = r < p.rows ? __ldg(p.scale + (r >> p.row_shift) * p.s_row + (col >> p.col_shift) * p.s_col) : 0.f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t r = row0 + ty + 16 * i;
+    if (r >= p.rows) continue;
+    if (!per_col) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sc[j] = sr[i];
+    } else if (per_row) {  // one factor per element
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sc[j] = j < n ? __ldg(p.scale + r * p.s_row + (col + j) * p.s_col) : 0.f;
+    }
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((w[i][j >> 1] >> (16 * (j & 1))) & 0xFFFFu), kInterp);
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+      y[2 * j] = f.x * sc[2 * j];
+      y[2 * j + 1] = f.y * sc[2 * j + 1];
     }
     if constexpr (VEC) {
       if constexpr (HP == F8B200_FP32) {
-        float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.y) + r * p.ld_y + c);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) __stcs(o + j, make_float4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]));
+        float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.y) + r * p.ld_y + col);
+        __stcs(o, make_float4(y[0], y[1], y[2], y[3]));
+        __stcs(o + 1, make_float4(y[4], y[5], y[6], y[7]));
       } else {
-        uint4* o = reinterpret_cast<uint4*>(p.y + (r * p.ld_y + c) * 2);
-        uint32_t h[8];
+        uint32_t h[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < 4; ++j) {
           if constexpr (HP == F8B200_BF16) {
             const __nv_bfloat162 t = __floats2bfloat162_rn(y[2 * j], y[2 * j + 1]);
             h[j] = *reinterpret_cast<const uint32_t*>(&t);
@@ -297,13 +358,12 @@ __global__ void __launch_bounds__(kThreads) uncast_block_kernel(const BlockUncas
             h[j] = *reinterpret_cast<const uint32_t*>(&t);
           }
         }
-        __stcs(o, make_uint4(h[0], h[1], h[2], h[3]));
-        __stcs(o + 1, make_uint4(h[4], h[5], h[6], h[7]));
+        __stcs(reinterpret_cast<uint4*>(p.y + (r * p.ld_y + col) * 2), make_uint4(h[0], h[1], h[2], h[3]));
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (j < n) store_hp<HP>(p.y, r * p.ld_y + c + j, y[j]);
+      for (int j = 0; j < 8; ++j)
+        if (j < n) store_hp<HP>(p.y, r * p.ld_y + col + j, y[j]);
     }
   }
 }
@@ -385,10 +445,11 @@ extern "C" int f8b200_uncast_blockwise(const void* q, int fp8_kind, int64_t rows
   p.scale = scale, p.s_row = scale_row_stride, p.s_col = scale_col_stride;
   p.row_shift = block_rows == kBlk ? 7 : 0, p.col_shift = block_cols == kBlk ? 7 : 0;
   p.y = static_cast<char*>(y), p.ld_y = ld_y;
-  p.chunks = (cols + 15) / 16;
-  const bool vec = cols % 16 == 0 && ld_q % 16 == 0 && aligned(q, 16) && aligned(y, 16) && (ld_y * es) % 16 == 0;
-  const int64_t work = (rows * p.chunks + kThreads - 1) / kThreads, cap = (int64_t)sm_count() * 16;
-  const unsigned grid = (unsigned)(work < cap ? work : cap);
+  p.tiles_k = (cols + kBlk - 1) / kBlk;
+  const int64_t tiles_m = (rows + kBlk - 1) / kBlk;
+  if (tiles_m > 0x7FFFFFFFLL / p.tiles_k) return F8B200_ERR_UNSUPPORTED;
+  const bool vec = cols % 8 == 0 && ld_q % 8 == 0 && aligned(q, 8) && aligned(y, 16) && (ld_y * es) % 16 == 0;
+  const unsigned grid = (unsigned)(tiles_m * p.tiles_k);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
 #define F8_UNCAST(HP, KIND)                                                                   \
   (vec ? (void)(uncast_block_kernel<HP, KIND, true><<<grid, kThreads, 0, st>>>(p))            \
