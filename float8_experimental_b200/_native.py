@@ -664,33 +664,39 @@ def layer_norm_bwd(x: torch.Tensor, g: torch.Tensor, rows: int, cols: int, ld_x:
         )
 
 
-def _tensor_arrays(xs: Sequence[torch.Tensor]):
-    n = len(xs)
-    return ((ctypes.c_void_p * n)(*[t.data_ptr() for t in xs]), (ctypes.c_int64 * n)(*[t.numel() for t in xs]),
-            (ctypes.c_int * n)(*[hp_code(t.dtype) for t in xs]))
+class TensorArrays:
+    """Addresses, sizes and types of dense CUDA tensors of one device as the multi-tensor entry points take them."""
+
+    __slots__ = ("n", "ptrs", "numels", "codes", "device")
+
+    def __init__(self, xs: Sequence[torch.Tensor]):
+        n = self.n = len(xs)
+        self.device = xs[0].device if n else None
+        _require_cuda(*xs)
+        self.ptrs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in xs])
+        self.numels = (ctypes.c_int64 * n)(*[t.numel() for t in xs])
+        self.codes = (ctypes.c_int * n)(*[hp_code(t.dtype) for t in xs])
 
 
 MULTI_TENSORS_PER_LAUNCH = 1024  # tensors whose addresses fit one launch's parameters (csrc/grad_clip.cu)
 
 
-def multi_norm(xs: Sequence[torch.Tensor], kind: int, root: bool, out: torch.Tensor) -> None:
+def multi_norm(xs: TensorArrays, kind: int, root: bool, out: torch.Tensor) -> None:
     """`f8b200_multi_norm` over dense tensors of one device, each taken as its storage lies."""
-    n = len(xs)
-    _require_cuda(out, *xs)
-    ptrs, numels, codes = _tensor_arrays(xs)
-    nbytes = int(load().f8b200_multi_norm_workspace_bytes(numels, n))
+    n = xs.n
+    _require_cuda(out)
+    nbytes = int(load().f8b200_multi_norm_workspace_bytes(xs.numels, n))
     ws = torch.empty(nbytes, dtype=torch.uint8, device=out.device) if nbytes else None
     with _Launch("multi_norm", out.device, 1 + -(-n // MULTI_TENSORS_PER_LAUNCH)):
-        _check(load().f8b200_multi_norm(ptrs, numels, codes, n, kind, int(root), out.data_ptr(), _ptr(ws), nbytes,
+        _check(load().f8b200_multi_norm(xs.ptrs, xs.numels, xs.codes, n, kind, int(root), out.data_ptr(), _ptr(ws), nbytes,
                                         _stream(out)), "f8b200_multi_norm")
 
 
-def multi_clip(xs: Sequence[torch.Tensor], total_norm: torch.Tensor, max_norm: float) -> None:
-    n = len(xs)
-    _require_cuda(total_norm, *xs)
-    ptrs, numels, codes = _tensor_arrays(xs)
+def multi_clip(xs: TensorArrays, total_norm: torch.Tensor, max_norm: float) -> None:
+    n = xs.n
+    _require_cuda(total_norm)
     with _Launch("multi_clip", total_norm.device, -(-n // MULTI_TENSORS_PER_LAUNCH)):
-        _check(load().f8b200_multi_clip(ptrs, numels, codes, n, total_norm.data_ptr(), float(max_norm),
+        _check(load().f8b200_multi_clip(xs.ptrs, xs.numels, xs.codes, n, total_norm.data_ptr(), float(max_norm),
                                         _stream(total_norm)), "f8b200_multi_clip")
 
 

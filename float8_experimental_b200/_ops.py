@@ -293,10 +293,11 @@ def _swiglu_bwd_cuda(a, b, grad_y, approx: bool = False):
     return da, db
 
 
-def _one_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) > 1:
-        raise RuntimeError(f"{what}: tensors on different devices ({', '.join(sorted(map(str, devices)))})")
+def _one_device(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    device = first.device
+    for t in others:
+        if t is not None and t.device != device:
+            raise RuntimeError(f"{what}: tensors on different devices ({device} and {t.device})")
 
 
 def _blocks(size: int) -> int:
@@ -313,25 +314,37 @@ def _exponent_bytes(rows: int, k: int) -> int:
     return -(-rows // 256) * 1024 * -(-k // 512)
 
 
-def _cast_blockwise_cuda(x, fp8_kind: int, by_row: bool, by_col: bool):
+def _cast_blockwise_some(x, fp8_kind: int, by_row: bool, by_col: bool, exponents: bool = True):
+    """The forms asked for as (data, scale_inv, exps), None for the others."""
     if x.dim() != 2 or not (by_row or by_col):
         raise RuntimeError("cast_blockwise: takes a matrix and at least one of by_row, by_col")
     xm, _, _, ld = _as_matrix(x)
     rows, cols = x.shape
-    none8 = torch.empty((0, 0), dtype=N.FP8_DTYPE[fp8_kind], device=x.device)
-    none32 = torch.empty((0, 0), dtype=torch.float32, device=x.device)
-    data = _empty_fp8_matrix(rows, cols, fp8_kind, x.device) if by_row else none8
-    data_c = _empty_fp8_matrix(rows, cols, fp8_kind, x.device) if by_col else none8
-    # one factor per (block, row) resp. (block, column): the GEMM's lanes read neighbouring rows
-    scale = torch.empty((_blocks(cols), rows), dtype=torch.float32, device=x.device) if by_row else none32
-    scale_c = torch.empty((_blocks(rows), cols), dtype=torch.float32, device=x.device) if by_col else none32
-    exps = torch.empty(_exponent_bytes(rows, cols) if by_row else 0, dtype=torch.uint8, device=x.device)
-    exps_c = torch.empty(_exponent_bytes(cols, rows) if by_col else 0, dtype=torch.uint8, device=x.device)
-    if x.numel():
-        r = (data, data.stride(0), scale, rows, exps) if by_row else (None, 0, None, 0, None)
-        c = (data_c, data_c.stride(0), scale_c, cols, exps_c) if by_col else (None, 0, None, 0, None)
-        N.cast_blockwise(xm, rows, cols, ld, fp8_kind, False, *r, *c)
-    return data, scale.t(), exps, data_c, scale_c, exps_c
+    device = x.device
+
+    def form(n, k):  # one factor per (block, row) resp. (block, column): the GEMM's lanes read neighbouring rows
+        data = _empty_fp8_matrix(rows, cols, fp8_kind, device)
+        scale = torch.empty((_blocks(k), n), dtype=torch.float32, device=device)
+        return data, scale, torch.empty(_exponent_bytes(n, k), dtype=torch.uint8, device=device) if exponents else None
+
+    r = form(rows, cols) if by_row else None
+    c = form(cols, rows) if by_col else None
+    if rows and cols:
+        N.cast_blockwise(xm, rows, cols, ld, fp8_kind, False,
+                         *((r[0], r[0].stride(0), r[1], rows, r[2]) if by_row else (None, 0, None, 0, None)),
+                         *((c[0], c[0].stride(0), c[1], cols, c[2]) if by_col else (None, 0, None, 0, None)))
+    return (r[0], r[1].t(), r[2]) if by_row else (None, None, None), c if by_col else (None, None, None)
+
+
+def _cast_blockwise_cuda(x, fp8_kind: int, by_row: bool, by_col: bool):
+    r, c = _cast_blockwise_some(x, fp8_kind, by_row, by_col)
+
+    def none():
+        return (torch.empty((0, 0), dtype=N.FP8_DTYPE[fp8_kind], device=x.device),
+                torch.empty((0, 0), dtype=torch.float32, device=x.device),
+                torch.empty((0,), dtype=torch.uint8, device=x.device))
+
+    return (*(r if by_row else none()), *(c if by_col else none()))
 
 
 def _cast_blockwise_square_cuda(x, fp8_kind: int):
@@ -446,17 +459,26 @@ def _check_dense(what: str, xs: List[torch.Tensor]) -> None:
             step *= size
 
 
+class TensorList(N.TensorArrays):
+    """Checked arguments of the multi-tensor kernels, made once for the calls that share the tensors."""
+
+    def __init__(self, what: str, xs: List[torch.Tensor]):
+        if xs:
+            _one_device(what, *xs)
+        _check_dense(what, xs)
+        super().__init__(xs)
+
+
 def _multi_norm_cuda(xs: List[torch.Tensor], kind: int, root: bool):
-    _one_device("multi_norm", *xs)
-    _check_dense("multi_norm", xs)
     out = torch.empty((), dtype=torch.float32, device=xs[0].device if xs else torch.device("cuda"))
-    N.multi_norm(xs, kind, root, out)
+    N.multi_norm(TensorList("multi_norm", xs), kind, root, out)
     return out
 
 
 def _multi_clip_cuda(xs: List[torch.Tensor], total_norm, max_norm: float) -> None:
-    _one_device("multi_clip_", total_norm, *xs)
-    _check_dense("multi_clip_", xs)
+    xs = TensorList("multi_clip_", xs)
+    if xs.device not in (None, total_norm.device):
+        raise RuntimeError(f"multi_clip_: tensors on different devices ({xs.device} and {total_norm.device})")
     if total_norm.numel() != 1 or total_norm.dtype != torch.float32:
         raise RuntimeError("multi_clip_: total_norm must be one float32 value")
     N.multi_clip(xs, total_norm, max_norm)
@@ -486,6 +508,16 @@ _lib.impl("multi_cast_with_scales", _multi_cast_with_scales_cuda, "CUDA")
 _lib.impl("cast_dynamic", _cast_dynamic_cuda, "CUDA")
 _lib.impl("delayed_sync", _delayed_sync_cuda, "CUDA")
 _lib.impl("scaled_mm", _scaled_mm_cuda, "CUDA")
+
+
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+
+
+def eager_cuda(t: torch.Tensor) -> bool:
+    """Whether an op on `t` would come straight to its CUDA implementation here: a plain CUDA tensor, nothing tracing.
+    Callers that run without autograd (inside an autograd function, or with nothing to differentiate) then call
+    the implementation themselves: a trip through the dispatcher costs more host time than a small launch."""
+    return type(t) in _PLAIN and t.is_cuda and not torch.compiler.is_compiling()
 
 
 # ---------------------------------------------------------------------------

@@ -18,7 +18,9 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native as N
-from ._ops import _blocks, ops
+from ._ops import (
+    _blocks, _blockwise_mm_cuda, _cast_blockwise_some, _cast_blockwise_square_cuda, _uncast_blockwise_cuda, eager_cuda, ops,
+)
 from .float8_utils import _kind, e4m3_dtype, e5m2_dtype
 
 __all__ = ["BLOCK", "Float8BlockTensor", "cast_to_float8_blockwise", "cast_to_float8_blockwise_both", "blockwise_mm"]
@@ -82,10 +84,28 @@ class Float8BlockTensor:
         return out
 
     def to_original_precision(self, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-        return ops.uncast_blockwise(self.data, self.scale_inv, *self.block, dtype or self.orig_dtype)
+        args = (self.data, self.scale_inv, *self.block, dtype or self.orig_dtype)
+        return _uncast_blockwise_cuda(*args) if eager_cuda(self.data) else ops.uncast_blockwise(*args)
 
     def __repr__(self):
         return f"Float8BlockTensor({self.data.dtype}, shape={tuple(self.shape)}, block={self.block})"
+
+
+def _cast(x, kind: int, by_row: bool, by_col: bool, exponents: bool = True):
+    """((data, scale_inv, exps) by rows, the same by columns); a form not asked for is three None."""
+    if eager_cuda(x):
+        return _cast_blockwise_some(x, kind, by_row, by_col, exponents)
+    out = ops.cast_blockwise(x, kind, by_row, by_col)
+    none = (None, None, None)
+    return out[:3] if by_row else none, out[3:] if by_col else none
+
+
+def _cast_square(x, kind: int):
+    return _cast_blockwise_square_cuda(x, kind) if eager_cuda(x) else ops.cast_blockwise_square(x, kind)
+
+
+def _mm(a, *args):
+    return _blockwise_mm_cuda(a, *args) if eager_cuda(a) else ops.blockwise_mm(a, *args)
 
 
 def _matrix(x: torch.Tensor, what: str) -> torch.Tensor:
@@ -103,12 +123,12 @@ def cast_to_float8_blockwise(x: torch.Tensor, block: Tuple[int, int] = (1, BLOCK
         raise ValueError(f"cast_to_float8_blockwise: block must be one of {_BLOCKS}, got {block}")
     x, kind = _matrix(x, "cast_to_float8_blockwise"), _kind(float8_dtype)
     if block == (BLOCK, BLOCK):
-        data, scale, exps, exps_t = ops.cast_blockwise_square(x, kind)
+        data, scale, exps, exps_t = _cast_square(x, kind)
     elif block == (1, BLOCK):
-        data, scale, exps, _, _, _ = ops.cast_blockwise(x, kind, True, False)
+        (data, scale, exps), _ = _cast(x, kind, True, False)
         exps_t = None
     else:
-        _, _, _, data, scale, exps_t = ops.cast_blockwise(x, kind, False, True)
+        _, (data, scale, exps_t) = _cast(x, kind, False, True)
         exps = None
     return Float8BlockTensor(data, scale, block, x.dtype)._with_exponents(exps, exps_t)
 
@@ -117,7 +137,7 @@ def cast_to_float8_blockwise_both(x: torch.Tensor, float8_dtype: torch.dtype = e
                                   ) -> Tuple[Float8BlockTensor, Float8BlockTensor]:
     """`x` cast by rows (1 x 128 blocks) and by columns (128 x 1), from one read of it."""
     x = _matrix(x, "cast_to_float8_blockwise_both")
-    data, scale, exps, data_c, scale_c, exps_c = ops.cast_blockwise(x, _kind(float8_dtype), True, True)
+    (data, scale, exps), (data_c, scale_c, exps_c) = _cast(x, _kind(float8_dtype), True, True)
     return (Float8BlockTensor(data, scale, (1, BLOCK), x.dtype)._with_exponents(exps, None),
             Float8BlockTensor(data_c, scale_c, (BLOCK, 1), x.dtype)._with_exponents(None, exps_c))
 
@@ -136,8 +156,19 @@ def blockwise_mm(a: Float8BlockTensor, b: Float8BlockTensor, out_dtype: torch.dt
     if a.shape[1] != b.shape[0]:
         raise ValueError(f"blockwise_mm: inner dimensions differ ({a.shape[1]} vs {b.shape[0]})")
     N.hp_code(out_dtype)
-    return ops.blockwise_mm(a.data, b.data.t(), a.scale_inv, b.scale_inv.t(), a.block[0], b.block[1],
-                            a._exponents(), b._exponents(transposed=True), bias, out_dtype)
+    return _mm(a.data, b.data.t(), a.scale_inv, b.scale_inv.t(), a.block[0], b.block[1], a._exponents(),
+               b._exponents(transposed=True), None if bias is None else bias.detach(), out_dtype)
+
+
+def linear_by_rows(x: torch.Tensor, weight: torch.Tensor, weight_scale_inv: torch.Tensor,
+                   bias: Optional[torch.Tensor]) -> torch.Tensor:
+    """x [..., K] cast by rows, times the transpose of an fp8 weight [N, K] with factors per 128 x 128 square, plus bias.
+    Not differentiable."""
+    x2 = x.detach().reshape(-1, x.shape[-1])
+    N.hp_code(x.dtype)
+    (x8, sx, _), _ = _cast(x2, N.E4M3, True, False, exponents=False)
+    y = _mm(x8, weight.detach(), sx, weight_scale_inv, 1, BLOCK, None, None, None if bias is None else bias.detach(), x.dtype)
+    return y if x.dim() == 2 else y.reshape(*x.shape[:-1], y.shape[-1])
 
 
 @torch._dynamo.allow_in_graph
@@ -150,10 +181,10 @@ class _float8_linear_blockwise(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, need_dw: bool):
         x2 = x.reshape(-1, x.shape[-1])
-        x8, sx, ex, x8c, sxc, exc = ops.cast_blockwise(x2, N.E4M3, True, need_dw)
-        w8, sw, ew, ewt = ops.cast_blockwise_square(weight, N.E4M3)
-        y = ops.blockwise_mm(x8, w8, sx, sw, 1, BLOCK, ex, ew, bias, x.dtype)
-        ctx.save_for_backward(x8c, sxc, exc, w8, sw, ewt)
+        (x8, sx, ex), by_col = _cast(x2, N.E4M3, True, need_dw)
+        w8, sw, ew, ewt = _cast_square(weight, N.E4M3)
+        y = _mm(x8, w8, sx, sw, 1, BLOCK, ex, ew, bias, x.dtype)
+        ctx.save_for_backward(*by_col, w8, sw, ewt)
         ctx.dtypes = (weight.dtype, bias.dtype if bias is not None else None)
         return y.reshape(*x.shape[:-1], y.shape[-1])
 
@@ -165,12 +196,12 @@ class _float8_linear_blockwise(torch.autograd.Function):
         go2 = go.reshape(-1, go.shape[-1])
         dx = dw = db = None
         if need_dx or need_dw:
-            g8, sg, eg, g8c, sgc, egc = ops.cast_blockwise(go2, N.E4M3, need_dx, need_dw)
+            (g8, sg, eg), (g8c, sgc, egc) = _cast(go2, N.E4M3, need_dx, need_dw)
         if need_dx:  # dX = dY @ W: the weight's bytes and factors read transposed
-            dx = ops.blockwise_mm(g8, w8.t(), sg, sw.t(), 1, BLOCK, eg, ewt, None, go.dtype)
+            dx = _mm(g8, w8.t(), sg, sw.t(), 1, BLOCK, eg, ewt, None, go.dtype)
             dx = dx.reshape(*go.shape[:-1], dx.shape[-1])
         if need_dw:  # dW = dY^T @ X, summed over rows: both by columns
-            dw = ops.blockwise_mm(g8c.t(), x8c.t(), sgc.t(), sxc.t(), 1, 1, egc, exc, None, ctx.dtypes[0])
+            dw = _mm(g8c.t(), x8c.t(), sgc.t(), sxc.t(), 1, 1, egc, exc, None, ctx.dtypes[0])
         if need_db:
             db = go2.sum(0, dtype=torch.float32).to(ctx.dtypes[1])
         return dx, dw, db, None

@@ -15,7 +15,8 @@ import torch
 import torch.distributed as dist
 from torch.distributed._tensor import DTensor
 
-from ._ops import ops
+from . import _native as N
+from ._ops import eager_cuda, ops, TensorList
 
 __all__ = ["get_total_norm", "clip_grads_with_norm_", "clip_grad_norm_"]
 
@@ -54,6 +55,32 @@ def _sharded_groups(t: DTensor):
     return tuple(groups)
 
 
+def _total_norm(tensors: List[torch.Tensor], kind: int) -> torch.Tensor:
+    if not tensors:
+        return torch.tensor(0.0)
+    if not any(isinstance(t, DTensor) for t in tensors):
+        return ops.multi_norm(tensors, kind, True)
+    by_groups: Dict[tuple, List[torch.Tensor]] = {}
+    for t in tensors:
+        by_groups.setdefault(_sharded_groups(t) if isinstance(t, DTensor) else (), []).append(_local(t))
+    parts = []
+    for groups, local in by_groups.items():
+        part = ops.multi_norm(local, kind, False)
+        for group in groups:
+            dist.all_reduce(part, op=dist.ReduceOp.MAX if kind == 0 else dist.ReduceOp.SUM, group=group)
+        parts.append(part)
+    both = torch.stack(parts)
+    return both.max() if kind == 0 else both.sum().sqrt() if kind == 2 else both.sum()
+
+
+def _check_finite(total: torch.Tensor, norm_type: float) -> None:
+    if not bool(torch.isfinite(total)):
+        raise RuntimeError(
+            f"The total norm of order {norm_type} for gradients is non-finite, so it cannot be clipped. "
+            "To disable this error and scale the gradients by the non-finite norm anyway, set `error_if_nonfinite=False`"
+        )
+
+
 @torch.no_grad()
 def get_total_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: float = 2.0,
                    error_if_nonfinite: bool = False) -> torch.Tensor:
@@ -61,28 +88,9 @@ def get_total_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], norm_ty
 
     Squares are formed in fp32 as in torch: an element beyond 1.8e19 makes the 2-norm infinite."""
     kind = _kind_of(norm_type)
-    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    if not tensors:
-        return torch.tensor(0.0)
-    by_groups: Dict[tuple, List[torch.Tensor]] = {}
-    for t in tensors:
-        by_groups.setdefault(_sharded_groups(t) if isinstance(t, DTensor) else (), []).append(_local(t))
-    if set(by_groups) == {()}:
-        total = ops.multi_norm(by_groups[()], kind, True)
-    else:
-        parts = []
-        for groups, local in by_groups.items():
-            part = ops.multi_norm(local, kind, False)
-            for group in groups:
-                dist.all_reduce(part, op=dist.ReduceOp.MAX if kind == 0 else dist.ReduceOp.SUM, group=group)
-            parts.append(part)
-        both = torch.stack(parts)
-        total = both.max() if kind == 0 else both.sum().sqrt() if kind == 2 else both.sum()
-    if error_if_nonfinite and not bool(torch.isfinite(total)):
-        raise RuntimeError(
-            f"The total norm of order {norm_type} for gradients is non-finite, so it cannot be clipped. "
-            "To disable this error and scale the gradients by the non-finite norm anyway, set `error_if_nonfinite=False`"
-        )
+    total = _total_norm([tensors] if isinstance(tensors, torch.Tensor) else list(tensors), kind)
+    if error_if_nonfinite:
+        _check_finite(total, norm_type)
     return total
 
 
@@ -100,7 +108,21 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
                     error_if_nonfinite: bool = False) -> torch.Tensor:
     """Clips the gradients of `parameters` to a total norm of at most `max_norm`, in place, and returns the norm they had
     (fp32, 0-dim, on their device).  `error_if_nonfinite=True` reads it back and synchronises."""
-    params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
-    total = get_total_norm(_gradients(params), norm_type, error_if_nonfinite)
-    clip_grads_with_norm_(params, max_norm, total)
+    kind = _kind_of(norm_type)
+    grads = _gradients(parameters)
+    if grads and all(map(eager_cuda, grads)):
+        # the usual case: the tensors' addresses are gathered once for both launches
+        tensors = TensorList("clip_grad_norm_", grads)
+        total = torch.empty((), dtype=torch.float32, device=tensors.device)
+        N.multi_norm(tensors, kind, True, total)
+        if error_if_nonfinite:
+            _check_finite(total, norm_type)
+        N.multi_clip(tensors, total, float(max_norm))
+        return total
+    total = _total_norm(grads, kind)
+    if error_if_nonfinite:
+        _check_finite(total, norm_type)
+    local = [_local(g) for g in grads]
+    if local:
+        ops.multi_clip_(local, total, float(max_norm))
     return total

@@ -11,8 +11,7 @@ from typing import Callable, Optional
 import torch
 import torch.nn as nn
 
-from ._ops import ops
-from .float8_blockwise import BLOCK, cast_to_float8_blockwise
+from .float8_blockwise import BLOCK, cast_to_float8_blockwise, linear_by_rows
 from .float8_linear_utils import swap_linear_layers
 from .float8_tensor import (
     Float8Tensor,
@@ -103,9 +102,7 @@ class Float8InferenceLinear(torch.nn.Linear):
     def _forward_blockwise(self, input: torch.Tensor) -> torch.Tensor:
         if type(input) not in (torch.Tensor, nn.Parameter):
             raise RuntimeError(f"ActivationCasting.BLOCKWISE takes plain tensors, got a {type(input).__name__}")
-        x8 = cast_to_float8_blockwise(input.reshape(-1, input.shape[-1]))
-        y = ops.blockwise_mm(x8.data, self.weight, x8.scale_inv, self.weight_scale_inv, 1, BLOCK, None, None, self.bias, input.dtype)
-        return y.reshape(*input.shape[:-1], y.shape[-1])
+        return linear_by_rows(input, self.weight, self.weight_scale_inv, self.bias)
 
     def quantize_weight(self, dtype: torch.dtype = e4m3_dtype) -> None:
         """Replaces the weight by its `Float8Tensor` (dynamic scale), frozen; with ActivationCasting.BLOCKWISE by its

@@ -13,18 +13,21 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native as N
-from ._ops import ops
+from ._ops import _layer_norm_bwd_cuda, _layer_norm_cuda, eager_cuda, ops
 
 __all__ = ["layer_norm", "LayerNorm"]
 
 
+def _forward(x, *args):
+    return _layer_norm_cuda(x, *args) if eager_cuda(x) else ops.layer_norm(x, *args)
+
+
 class _LayerNormFunc(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, eps, keep):
-        y, mean, rstd = ops.layer_norm(x, weight, bias, eps, keep)
-        if keep:
-            ctx.save_for_backward(x, weight, mean, rstd)
-            ctx.affine_dtype = next((t.dtype for t in (weight, bias) if t is not None), x.dtype)
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = _forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.affine_dtype = next((t.dtype for t in (weight, bias) if t is not None), x.dtype)
         return y
 
     @staticmethod
@@ -32,8 +35,9 @@ class _LayerNormFunc(torch.autograd.Function):
     def backward(ctx, g):
         x, weight, mean, rstd = ctx.saved_tensors
         need = ctx.needs_input_grad[:3]
-        grads = ops.layer_norm_bwd(x, g, weight, mean, rstd, ctx.affine_dtype, *need)
-        return (*[t if n else None for t, n in zip(grads, need)], None, None)
+        backward = _layer_norm_bwd_cuda if eager_cuda(x) else ops.layer_norm_bwd
+        grads = backward(x, g, weight, mean, rstd, ctx.affine_dtype, *need)
+        return (*[t if n else None for t, n in zip(grads, need)], None)
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -43,8 +47,9 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     `x` is bf16, fp16 or fp32; `weight` and `bias` [D] are optional and share x's dtype or are both float32.
     The result has x's dtype.  Differentiable once in x, weight and bias."""
     N.hp_code(x.dtype)
-    keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias))
-    return _LayerNormFunc.apply(x, weight, bias, float(eps), keep)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return _LayerNormFunc.apply(x, weight, bias, float(eps))
+    return _forward(x, weight, bias, float(eps), False)[0]
 
 
 class LayerNorm(torch.nn.LayerNorm):
