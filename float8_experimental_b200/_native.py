@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+from array import array
 from typing import Optional, Sequence
 
 import torch
@@ -168,7 +169,8 @@ def fp8_code(dtype: torch.dtype) -> int:
 
 
 def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    # the handle alone: torch.cuda.current_stream builds a Stream object around it, 3 us of host time per launch
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def _require_cuda(*tensors: Optional[torch.Tensor]) -> None:
@@ -636,6 +638,28 @@ def gemm_blockwise(a: torch.Tensor, lda: int, a_mn_major: bool, scale_a: torch.T
         )
 
 
+def linear_blockwise(x: torch.Tensor, m: int, k: int, ld_x: int, weight: torch.Tensor, ldw: int, w_mn_major: bool,
+                     weight_scale: torch.Tensor, bias: Optional[torch.Tensor], out: torch.Tensor, n: int) -> None:
+    """out [m, n] = x [m, k] cast by rows, times the transpose of an fp8 weight with one factor per 128 x 128: the cast
+    and the product (`f8b200_cast_blockwise`, `f8b200_gemm_blockwise`) with the cast's bytes and factors in one
+    scratch buffer.  Few rows leave the GPU waiting for the host, so this is as little host work as the two need."""
+    _require_cuda(x, weight, weight_scale, bias, out)
+    pitch = -(-k // 16) * 16
+    data_bytes = -(-m * pitch // 16) * 16
+    scratch = torch.empty(data_bytes + 4 * m * -(-k // 128), dtype=torch.uint8, device=x.device)
+    data, stream = scratch.data_ptr(), _stream(x)
+    scale = data + data_bytes  # [k-block][row]
+    lib = load()
+    with _Launch("gemm_block", x.device, 2):
+        _check(lib.f8b200_cast_blockwise(x.data_ptr(), hp_code(x.dtype), m, k, ld_x, E4M3, 0, data, pitch, scale, m, None,
+                                         None, 0, None, 0, None, stream), "f8b200_cast_blockwise")
+        _check(lib.f8b200_gemm_blockwise(data, E4M3, 0, pitch, scale, 1, m, 1, None, weight.data_ptr(),
+                                         fp8_code(weight.dtype), int(w_mn_major), ldw, weight_scale.data_ptr(),
+                                         weight_scale.stride(0), weight_scale.stride(1), 128, None, _ptr(bias),
+                                         hp_code(out.dtype), out.data_ptr(), n, m, n, k, None, 0, stream),
+               "f8b200_gemm_blockwise")
+
+
 def layer_norm(x: torch.Tensor, rows: int, cols: int, ld_x: int, weight: Optional[torch.Tensor],
                bias: Optional[torch.Tensor], affine_dtype: torch.dtype, eps: float, y: torch.Tensor,
                mean: Optional[torch.Tensor], rstd: Optional[torch.Tensor]) -> None:
@@ -670,12 +694,20 @@ class TensorArrays:
     __slots__ = ("n", "ptrs", "numels", "codes", "device")
 
     def __init__(self, xs: Sequence[torch.Tensor]):
+        # hundreds of tensors per call: every pass over them is a C-level map
         n = self.n = len(xs)
+        T = torch.Tensor
+        devices = set(map(T.get_device, xs))
+        if len(devices) > 1:
+            raise F8B200Error(f"tensors on different devices ({', '.join(sorted({str(t.device) for t in xs}))})")
+        if -1 in devices:
+            raise F8B200Error("f8b200 kernels run on CUDA tensors only (no CPU path exists)")
         self.device = xs[0].device if n else None
-        _require_cuda(*xs)
-        self.ptrs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in xs])
-        self.numels = (ctypes.c_int64 * n)(*[t.numel() for t in xs])
-        self.codes = (ctypes.c_int * n)(*[hp_code(t.dtype) for t in xs])
+        dtypes = [t.dtype for t in xs]
+        codes = {dtype: hp_code(dtype) for dtype in set(dtypes)}
+        self.ptrs = (ctypes.c_void_p * n).from_buffer(array("Q", map(T.data_ptr, xs))) if n else None
+        self.numels = (ctypes.c_int64 * n).from_buffer(array("q", map(T.numel, xs))) if n else None
+        self.codes = (ctypes.c_int * n).from_buffer(array("i", map(codes.__getitem__, dtypes))) if n else None
 
 
 MULTI_TENSORS_PER_LAUNCH = 1024  # tensors whose addresses fit one launch's parameters (csrc/grad_clip.cu)

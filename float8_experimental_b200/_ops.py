@@ -306,7 +306,8 @@ def _blocks(size: int) -> int:
 
 def _empty_fp8_matrix(rows: int, cols: int, fp8_kind: int, device) -> torch.Tensor:
     """[rows, cols] fp8 whose rows start on 16-byte boundaries, so that the GEMM reads it where it lies."""
-    return torch.empty((rows, _pitch16(cols)), dtype=N.FP8_DTYPE[fp8_kind], device=device)[:, :cols]
+    out = torch.empty((rows, _pitch16(cols)), dtype=N.FP8_DTYPE[fp8_kind], device=device)
+    return out if cols % 16 == 0 else out[:, :cols]
 
 
 def _exponent_bytes(rows: int, k: int) -> int:
@@ -314,7 +315,7 @@ def _exponent_bytes(rows: int, k: int) -> int:
     return -(-rows // 256) * 1024 * -(-k // 512)
 
 
-def _cast_blockwise_some(x, fp8_kind: int, by_row: bool, by_col: bool, exponents: bool = True):
+def _cast_blockwise_some(x, fp8_kind: int, by_row: bool, by_col: bool):
     """The forms asked for as (data, scale_inv, exps), None for the others."""
     if x.dim() != 2 or not (by_row or by_col):
         raise RuntimeError("cast_blockwise: takes a matrix and at least one of by_row, by_col")
@@ -325,7 +326,7 @@ def _cast_blockwise_some(x, fp8_kind: int, by_row: bool, by_col: bool, exponents
     def form(n, k):  # one factor per (block, row) resp. (block, column): the GEMM's lanes read neighbouring rows
         data = _empty_fp8_matrix(rows, cols, fp8_kind, device)
         scale = torch.empty((_blocks(k), n), dtype=torch.float32, device=device)
-        return data, scale, torch.empty(_exponent_bytes(n, k), dtype=torch.uint8, device=device) if exponents else None
+        return data, scale, torch.empty(_exponent_bytes(n, k), dtype=torch.uint8, device=device)
 
     r = form(rows, cols) if by_row else None
     c = form(cols, rows) if by_col else None
@@ -404,15 +405,43 @@ def _blockwise_mm_cuda(a, b_t, scale_a, scale_b, a_block_rows: int, b_block_rows
     return out
 
 
+def linear_blockwise(x, weight, weight_scale, bias):
+    """x [m, k] cast by rows times the transpose of `weight` [n, k] (fp8, `weight_scale` per 128 x 128), plus bias: eager
+    CUDA tensors, without autograd."""
+    m, k = x.shape
+    n, k2 = weight.shape
+    if k != k2:
+        raise RuntimeError(f"blockwise_mm: inner dimensions differ ({k} vs {k2})")
+    if weight_scale.dtype != torch.float32 or tuple(weight_scale.shape) != (_blocks(n), _blocks(k)):
+        raise RuntimeError(f"blockwise_mm: scale_b must be float32 {(_blocks(n), _blocks(k))}, got {weight_scale.dtype} "
+                           f"{tuple(weight_scale.shape)}")
+    _one_device("blockwise_mm", x, weight, weight_scale, bias)
+    if bias is not None:
+        if tuple(bias.shape) != (n,):
+            raise RuntimeError(f"blockwise_mm: the bias must have {n} elements, got {tuple(bias.shape)}")
+        bias = bias.to(x.dtype).contiguous()
+    out = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    if m == 0 or n == 0:
+        return out
+    if k == 0:
+        return out.zero_() if bias is None else out.copy_(bias)
+    xm, _, _, ld = _as_matrix(x)
+    weight, ldw, w_mn = _gemm_operand(weight)
+    N.linear_blockwise(xm, m, k, ld, weight, ldw, w_mn, weight_scale, bias, out, n)
+    return out
+
+
 def _affine_dtype(x, weight, bias) -> torch.dtype:
     """The type of the norm's weight and bias: x's or fp32, the same for both."""
-    cols = x.shape[-1]
-    kinds = {t.dtype for t in (weight, bias) if t is not None}
-    if len(kinds) > 1 or not kinds <= {x.dtype, torch.float32}:
+    first = weight if weight is not None else bias
+    if first is None:
+        return x.dtype
+    affine, want = first.dtype, x.shape[-1:]
+    if (affine != x.dtype and affine != torch.float32) or (bias is not None and bias.dtype != affine):
         raise RuntimeError(f"layer_norm: weight and bias must both have x's dtype {x.dtype} or both float32")
-    if any(tuple(t.shape) != (cols,) for t in (weight, bias) if t is not None):
-        raise RuntimeError(f"layer_norm: weight and bias must have one element per column ({cols})")
-    return kinds.pop() if kinds else x.dtype
+    if first.shape != want or (bias is not None and bias.shape != want):
+        raise RuntimeError(f"layer_norm: weight and bias must have one element per column ({want[0]})")
+    return affine
 
 
 def _layer_norm_cuda(x, weight, bias, eps: float, save_stats: bool):
@@ -422,12 +451,14 @@ def _layer_norm_cuda(x, weight, bias, eps: float, save_stats: bool):
     affine = _affine_dtype(x, weight, bias)
     xm, rows, cols, ld = _as_matrix(x)
     y = _empty_like_shape(x, x.dtype)
-    stats = torch.empty((2, rows if save_stats else 0), dtype=torch.float32, device=x.device)
+    # two tensors of their own: views of one would share its version counter and outlive it together
+    mean = torch.empty(rows if save_stats else 0, dtype=torch.float32, device=x.device)
+    rstd = torch.empty(rows if save_stats else 0, dtype=torch.float32, device=x.device)
     if rows:
         N.layer_norm(xm, rows, cols, ld, None if weight is None else weight.contiguous(),
-                     None if bias is None else bias.contiguous(), affine, eps, y,
-                     stats[0] if save_stats else None, stats[1] if save_stats else None)
-    return y, stats[0], stats[1]
+                     None if bias is None else bias.contiguous(), affine, eps, y, mean if save_stats else None,
+                     rstd if save_stats else None)
+    return y, mean, rstd
 
 
 def _layer_norm_bwd_cuda(x, grad_y, weight, mean, rstd, affine_dtype, need_dx: bool, need_dw: bool, need_db: bool):
@@ -447,6 +478,8 @@ def _layer_norm_bwd_cuda(x, grad_y, weight, mean, rstd, affine_dtype, need_dx: b
 
 def _check_dense(what: str, xs: List[torch.Tensor]) -> None:
     """The kernels walk a tensor's storage: its elements must fill a range of it, each once, in any order."""
+    if all(map(torch.Tensor.is_contiguous, xs)):
+        return
     for t in xs:
         if t.is_contiguous():
             continue
@@ -463,10 +496,8 @@ class TensorList(N.TensorArrays):
     """Checked arguments of the multi-tensor kernels, made once for the calls that share the tensors."""
 
     def __init__(self, what: str, xs: List[torch.Tensor]):
-        if xs:
-            _one_device(what, *xs)
-        _check_dense(what, xs)
         super().__init__(xs)
+        _check_dense(what, xs)
 
 
 def _multi_norm_cuda(xs: List[torch.Tensor], kind: int, root: bool):

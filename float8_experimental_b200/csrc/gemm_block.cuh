@@ -290,24 +290,32 @@ gemm_block_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_c
 // ---------------------------------------------------------------------------------------------------
 // Few rows of A.  D[128 rows of B, T rows of A] per CTA, K split over the CTAs of a cluster.
 // ---------------------------------------------------------------------------------------------------
-constexpr int FTHREADS = 192;  // TMA warp, MMA warp, 4 epilogue warps
-
+// Per CTA and k-block: 16 KB of B, T x 128 bytes of A.  With up to 64 rows two CTAs share an SM, so that one's join
+// and start-up lie beside the other's loads; four epilogue warps add up 64 columns each thread, and twice as many do
+// for 128 rows.
 template <int T>
 struct FewCfg {
+  static constexpr int kCols = T < 64 ? T : 64;              // accumulator columns per epilogue warp
+  static constexpr int kEpiWarps = 4 * (T / kCols);
+  static constexpr int kThreads = 64 + 32 * kEpiWarps;       // TMA warp, MMA warp, epilogue
+  static constexpr int kCtas = T <= 64 ? 2 : 1;              // per SM
   static constexpr int kXBytes = T * BK;
   static constexpr int kStageBytes = 128 * BK + kXBytes;
-  static constexpr int kStages = T <= 32 ? 5 : T <= 64 ? 4 : 3;  // about 100 KB, so that two CTAs share an SM
-  static constexpr int kTmemCols = 2 * T < 32 ? 32 : 2 * T;
-  static constexpr int kJoinBytes = T * 128 * 4;   // fp32 sums handed over at the end, over the stages
+  static constexpr int kStages = T <= 32 ? 5 : T <= 64 ? 4 : 6;
+  static constexpr int kBufs = 512 / kCtas / T < 4 ? 512 / kCtas / T : 4;  // accumulators that alternate
+  static constexpr int kTmemCols = kBufs * T < 32 ? 32 : kBufs * T;
+  static constexpr int kJoinBytes = T * 128 * 4;             // fp32 sums handed over at the end, over the stages
   static_assert(kJoinBytes <= kStages * kStageBytes, "the sums have to fit into the stages");
+  static_assert((kBufs & (kBufs - 1)) == 0 && kBufs >= 2, "buffers are chosen by the low bits of a counter");
 };
 template <int T>
 struct __align__(16) FewBars {
-  float x_scale[4][2][T];  // per epilogue warp, two k-blocks: the factors of A's rows
-  uint64_t full[FewCfg<T>::kStages];
-  uint64_t empty[FewCfg<T>::kStages];
-  uint64_t tmem_full[2];
-  uint64_t tmem_empty[2];
+  using Cfg = FewCfg<T>;
+  float x_scale[Cfg::kEpiWarps][2][Cfg::kCols];  // per epilogue warp, two k-blocks: the factors of its columns (A's rows)
+  uint64_t full[Cfg::kStages];
+  uint64_t empty[Cfg::kStages];
+  uint64_t tmem_full[Cfg::kBufs];
+  uint64_t tmem_empty[Cfg::kBufs];
   uint32_t tmem_base;
   volatile uint32_t abort_flag;
 };
@@ -330,20 +338,23 @@ __device__ __forceinline__ bool few_wait(uint64_t* bar, uint32_t parity, Bars* b
   atomicOr(&g_device_error, who | 0x200u);
   return false;
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t cluster_addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr) : "memory");
   return v;
 }
 
-// grid: x = K split (the cluster), y = tiles of 128 rows of B, z = tiles of T rows of A
+constexpr int FEW_MAX_SPLIT = 8;  // the portable cluster size
+
+// grid: x = K split (the cluster), y = tiles of 128 rows of B, z = tiles of T rows of A.  `uniform`: B has one factor
+// per 128 rows, i.e. one per CTA and k-block, which then goes into A's factors once per block instead of into every FMA.
 template <typename OutT, int T>
-__global__ void __launch_bounds__(FTHREADS)
+__global__ void __launch_bounds__(FewCfg<T>::kThreads, FewCfg<T>::kCtas)
 gemm_block_few_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_constant__ CUtensorMap tma_x,
                       const BlockScale scale_w, const BlockScale scale_x, const OutT* __restrict__ bias,
-                      OutT* __restrict__ out, int64_t ldo, int m, int n, int k, uint32_t idesc, int w_mn) {
+                      OutT* __restrict__ out, int64_t ldo, int m, int n, int k, uint32_t idesc, int w_mn, int out_vec_ok) {
   using Cfg = FewCfg<T>;
-  constexpr int S = Cfg::kStages;
+  constexpr int S = Cfg::kStages, C = Cfg::kCols, BUFS = Cfg::kBufs;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   FewBars<T>* bars = reinterpret_cast<FewBars<T>*>(tiles + S * Cfg::kStageBytes);
@@ -361,9 +372,9 @@ gemm_block_few_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
       mbar_init(&bars->full[s], 1);
       mbar_init(&bars->empty[s], 1);
     }
-    for (int a = 0; a < 2; ++a) {
+    for (int a = 0; a < BUFS; ++a) {
       mbar_init(&bars->tmem_full[a], 1);
-      mbar_init(&bars->tmem_empty[a], 4);
+      mbar_init(&bars->tmem_empty[a], Cfg::kEpiWarps);
     }
     bars->abort_flag = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -380,7 +391,7 @@ gemm_block_few_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
   const uint32_t tmem_base = bars->tmem_base;
 
   bool good = true;
-  float acc[T];
+  uint64_t acc[C / 2];
   if (warp == 0) {
     if (lane == 0) {
       int stage = 0;
@@ -399,7 +410,7 @@ gemm_block_few_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
         if (!few_wait(&bars->empty[stage], phase ^ 1u, bars, 1u)) { ok = false; break; }
         if (++stage == S) { stage = 0; phase ^= 1u; }
       }
-      if (!ok) {
+      if (!ok) {  // give the loads in flight time to land before the CTA leaves
         const long long t0 = clock64();
         while (clock64() - t0 < 2000000LL) {}
       }
@@ -409,9 +420,9 @@ gemm_block_few_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
       int stage = 0;
       uint32_t phase = 0, g = 0;
       for (int kb = kb0; kb < kb1; ++kb, ++g) {
-        const uint32_t buf = g & 1u;
+        const uint32_t buf = g & (BUFS - 1);
         if (!few_wait(&bars->full[stage], phase, bars, 4u)) break;
-        if (!few_wait(&bars->tmem_empty[buf], ((g >> 1) & 1u) ^ 1u, bars, 2u)) break;
+        if (!few_wait(&bars->tmem_empty[buf], ((g / BUFS) & 1u) ^ 1u, bars, 2u)) break;
         tc_fence_after();
         const uint32_t w_addr = smem_u32(tiles + stage * Cfg::kStageBytes);
         const uint64_t dw = w_mn ? make_smem_desc_mn(w_addr, 128 * BK) : make_smem_desc(w_addr);
@@ -425,48 +436,66 @@ gemm_block_few_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
       }
     }
   } else {
-    const int quarter = warp & 3;
+    const int quarter = warp & 3, part = (warp - 2) >> 2;  // 32 rows of B, C rows of A
     const int row = row_w + quarter * 32 + lane;
     const bool row_in = row < n;
-    const float* pw = scale_w.p + (int64_t)((row_in ? row : 0) >> scale_w.shift) * scale_w.row_stride;
-    constexpr int XL = (T + 31) / 32;  // factors of A's rows that one lane fetches per k-block
+    const bool uniform = scale_w.shift == 7;
+    const float* pw = scale_w.p + (int64_t)((row_in ? row : row_w) >> scale_w.shift) * scale_w.row_stride;
+    constexpr int XL = (C + 31) / 32;  // factors of A's rows that one lane fetches per k-block
+    const float* px[XL];
+    bool px_in[XL];
+#pragma unroll
+    for (int j = 0; j < XL; ++j) {
+      const int r = row_x + part * C + lane + 32 * j;
+      px_in[j] = lane + 32 * j < C && r < m;
+      px[j] = scale_x.p + (int64_t)((px_in[j] ? r : 0) >> scale_x.shift) * scale_x.row_stride;
+    }
     float sx[XL], sw = 0.f;
     auto fetch = [&](int kb) {
-      sw = row_in ? __ldg(pw + (int64_t)kb * scale_w.kb_stride) : 0.f;
+      sw = __ldg(pw + (int64_t)kb * scale_w.kb_stride);
 #pragma unroll
-      for (int j = 0; j < XL; ++j) {
-        const int r = row_x + lane + 32 * j;
-        sx[j] = (lane + 32 * j < T && r < m) ? __ldg(scale_x.p + (int64_t)(r >> scale_x.shift) * scale_x.row_stride +
-                                                     (int64_t)kb * scale_x.kb_stride) : 0.f;
-      }
+      for (int j = 0; j < XL; ++j) sx[j] = px_in[j] ? __ldg(px[j] + (int64_t)kb * scale_x.kb_stride) : 0.f;
     };
 #pragma unroll
-    for (int i = 0; i < T; ++i) acc[i] = 0.f;
+    for (int i = 0; i < C / 2; ++i) acc[i] = 0ull;
     if (kb0 < kb1) fetch(kb0);
     uint32_t g = 0;
+    const uint32_t taddr0 = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(part * C);
     for (int kb = kb0; kb < kb1; ++kb, ++g) {
-      const uint32_t buf = g & 1u;
-      float* xs = bars->x_scale[warp - 2][buf];
+      const uint32_t buf = g & (BUFS - 1);
+      float* xs = bars->x_scale[warp - 2][kb & 1];
 #pragma unroll
       for (int j = 0; j < XL; ++j)
-        if (lane + 32 * j < T) xs[lane + 32 * j] = sx[j];
+        if (lane + 32 * j < C) xs[lane + 32 * j] = uniform ? sx[j] * sw : sx[j];
       __syncwarp();
       const float s = sw;
       if (kb + 1 < kb1) fetch(kb + 1);
-      if (!few_wait(&bars->tmem_full[buf], (g >> 1) & 1u, bars, 8u)) { good = false; break; }
+      if (!few_wait(&bars->tmem_full[buf], (g / BUFS) & 1u, bars, 8u)) { good = false; break; }
       __syncwarp();
       tc_fence_after();
+      uint32_t r[C / 16][16];
 #pragma unroll
-      for (int c = 0; c < T / 16; ++c) {
-        uint32_t r[16];
-        tc_ld_32x32b_x16(tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * T + c * 16, r);
-        tc_wait_ld();
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[c * 16 + i] = fmaf(__uint_as_float(r[i]), s * xs[c * 16 + i], acc[c * 16 + i]);
-      }
+      for (int c = 0; c < C / 16; ++c) tc_ld_32x32b_x16(taddr0 + buf * T + c * 16, r[c]);
+      tc_wait_ld();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->tmem_empty[buf]);
+      if (uniform) {
+#pragma unroll
+        for (int c = 0; c < C / 4; ++c) {
+          const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(xs + 4 * c);
+          acc[2 * c] = fma2(pack2(r[c / 4][(4 * c) & 15], r[c / 4][(4 * c + 1) & 15]), f.x, acc[2 * c]);
+          acc[2 * c + 1] = fma2(pack2(r[c / 4][(4 * c + 2) & 15], r[c / 4][(4 * c + 3) & 15]), f.y, acc[2 * c + 1]);
+        }
+      } else {
+        const uint64_t s2 = pack2(s, s);
+#pragma unroll
+        for (int c = 0; c < C / 4; ++c) {
+          const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(xs + 4 * c);
+          acc[2 * c] = fma2(pack2(r[c / 4][(4 * c) & 15], r[c / 4][(4 * c + 1) & 15]), mul2f(f.x, s2), acc[2 * c]);
+          acc[2 * c + 1] = fma2(pack2(r[c / 4][(4 * c + 2) & 15], r[c / 4][(4 * c + 3) & 15]), mul2f(f.y, s2), acc[2 * c + 1]);
+        }
+      }
     }
   }
   tc_fence_before();
@@ -477,29 +506,56 @@ gemm_block_few_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
                  : "memory");
   }
 
-  // join: the sums lie as [token][128] in every CTA of the cluster; CTA r adds up and stores tokens r, r + split, ...
+  // join: the sums lie as [A's row][128] in every CTA of the cluster; CTA r adds up and stores rows r, r + split, ...
   float* mine = reinterpret_cast<float*>(tiles);
   if (warp >= 2 && good) {
-    const int r = (warp & 3) * 32 + lane;
+    const int r = (warp & 3) * 32 + lane, first = ((warp - 2) >> 2) * C;
 #pragma unroll
-    for (int i = 0; i < T; ++i) mine[i * 128 + r] = acc[i];
+    for (int i = 0; i < C / 2; ++i) {
+      float lo, hi;
+      unpack2(acc[i], lo, hi);
+      mine[(first + 2 * i) * 128 + r] = lo;
+      mine[(first + 2 * i + 1) * 128 + r] = hi;
+    }
   }
   const bool failed = bars->abort_flag != 0u;
   if (split > 1) cluster_sync_all(); else __syncthreads();
   if (!failed) {
-    const int ntok = min(T, m - row_x);
-    for (int e = (int)threadIdx.x; e < ntok * 128; e += FTHREADS) {
-      const int i = e >> 7, c = e & 127, col = row_w + c;
-      if (i % split != (int)rank || col >= n) continue;
-      float v = 0.f;
+    const int rows_x = min(T, m - row_x);
+    for (int e = (int)threadIdx.x; ; e += Cfg::kThreads) {
+      const int i = (e >> 5) * split + (int)rank, c = (e & 31) * 4, col = row_w + c;
+      if (i >= rows_x) break;
+      if (col >= n) continue;
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
       if (split > 1) {
         const uint32_t addr = smem_u32(mine + i * 128 + c);
-        for (int q = 0; q < split; ++q) v += ld_cluster_f32(mapa_u32(addr, (uint32_t)q));
+        float4 p[FEW_MAX_SPLIT];
+#pragma unroll
+        for (int q = 0; q < FEW_MAX_SPLIT; ++q)
+          if (q < split) p[q] = ld_cluster_f32x4(mapa_u32(addr, (uint32_t)q));
+#pragma unroll
+        for (int q = 0; q < FEW_MAX_SPLIT; ++q)
+          if (q < split) v[0] += p[q].x, v[1] += p[q].y, v[2] += p[q].z, v[3] += p[q].w;
       } else {
-        v = mine[i * 128 + c];
+        const float4 p = *reinterpret_cast<const float4*>(mine + i * 128 + c);
+        v[0] = p.x, v[1] = p.y, v[2] = p.z, v[3] = p.w;
       }
-      if (bias != nullptr) v += static_cast<float>(bias[col]);
-      out[(int64_t)(row_x + i) * ldo + col] = static_cast<OutT>(v);
+      const int ncols = min(4, n - col);
+      __align__(16) OutT o[4];
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        if (bias != nullptr && h < ncols) v[h] += static_cast<float>(bias[col + h]);
+        o[h] = static_cast<OutT>(v[h]);
+      }
+      OutT* dst = out + (int64_t)(row_x + i) * ldo + col;
+      if (out_vec_ok && ncols == 4) {  // rows start on 16-byte boundaries, columns on multiples of four
+        if constexpr (sizeof(OutT) == 2) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(o);
+        else *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+      } else {
+#pragma unroll
+        for (int h = 0; h < 4; ++h)
+          if (h < ncols) dst[h] = o[h];
+      }
     }
   }
   if (split > 1) cluster_sync_all();  // no CTA leaves while another may still read its sums
@@ -944,7 +1000,7 @@ static int launch_block_scaled(const CUtensorMap& ma, const CUtensorMap& mb, con
 template <typename OutT, int T>
 static int launch_block_few(const CUtensorMap& mw, const CUtensorMap& mx, const BlockScale& sw, const BlockScale& sx,
                             const void* bias, void* out, int64_t ldo, int m, int n, int k, uint32_t idesc, int w_mn,
-                            int split, cudaStream_t st) {
+                            int vec_ok, int split, cudaStream_t st) {
   static PerDeviceOnce setup;
   auto kernel = gemm_block_few_kernel<OutT, T>;
   const cudaError_t attr_err = setup.run([&](int*) {
@@ -957,14 +1013,14 @@ static int launch_block_few(const CUtensorMap& mw, const CUtensorMap& mx, const 
   attr[0].val.clusterDim.x = split;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  cfg.blockDim = dim3(FTHREADS);
+  cfg.blockDim = dim3(FewCfg<T>::kThreads);
   cfg.dynamicSmemBytes = few_smem_bytes<T>();
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = split > 1 ? 1 : 0;
   cfg.gridDim = dim3(split, (n + 127) / 128, (m + T - 1) / T);
   return record_cuda_error(cudaLaunchKernelEx(&cfg, kernel, mw, mx, sw, sx, static_cast<const OutT*>(bias),
-                                              static_cast<OutT*>(out), ldo, m, n, k, idesc, w_mn));
+                                              static_cast<OutT*>(out), ldo, m, n, k, idesc, w_mn, vec_ok));
 }
 
 // instruction descriptor of one CTA: 128 rows of B's side, `cols` rows of A's side
@@ -1021,7 +1077,7 @@ extern "C" int f8b200_gemm_blockwise(const void* a, int a_kind, int a_layout, in
       using OutT = std::remove_pointer_t<decltype(tag)>;
       auto go = [&](auto t_const) {
         return launch_block_few<OutT, decltype(t_const)::value>(mb, ma, sb, sa, bias, out, ldo, (int)m, (int)n, (int)k,
-                                                                idesc, b_layout, split, st);
+                                                                idesc, b_layout, vec_ok, split, st);
       };
       if (t == 16) return go(std::integral_constant<int, 16>{});
       if (t == 32) return go(std::integral_constant<int, 32>{});

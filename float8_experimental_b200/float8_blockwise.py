@@ -19,7 +19,8 @@ from torch.autograd.function import once_differentiable
 
 from . import _native as N
 from ._ops import (
-    _blocks, _blockwise_mm_cuda, _cast_blockwise_some, _cast_blockwise_square_cuda, _uncast_blockwise_cuda, eager_cuda, ops,
+    _blocks, _blockwise_mm_cuda, _cast_blockwise_some, _cast_blockwise_square_cuda, _uncast_blockwise_cuda, eager_cuda,
+    linear_blockwise, ops,
 )
 from .float8_utils import _kind, e4m3_dtype, e5m2_dtype
 
@@ -91,10 +92,10 @@ class Float8BlockTensor:
         return f"Float8BlockTensor({self.data.dtype}, shape={tuple(self.shape)}, block={self.block})"
 
 
-def _cast(x, kind: int, by_row: bool, by_col: bool, exponents: bool = True):
+def _cast(x, kind: int, by_row: bool, by_col: bool):
     """((data, scale_inv, exps) by rows, the same by columns); a form not asked for is three None."""
     if eager_cuda(x):
-        return _cast_blockwise_some(x, kind, by_row, by_col, exponents)
+        return _cast_blockwise_some(x, kind, by_row, by_col)
     out = ops.cast_blockwise(x, kind, by_row, by_col)
     none = (None, None, None)
     return out[:3] if by_row else none, out[3:] if by_col else none
@@ -164,11 +165,15 @@ def linear_by_rows(x: torch.Tensor, weight: torch.Tensor, weight_scale_inv: torc
                    bias: Optional[torch.Tensor]) -> torch.Tensor:
     """x [..., K] cast by rows, times the transpose of an fp8 weight [N, K] with factors per 128 x 128 square, plus bias.
     Not differentiable."""
-    x2 = x.detach().reshape(-1, x.shape[-1])
     N.hp_code(x.dtype)
-    (x8, sx, _), _ = _cast(x2, N.E4M3, True, False, exponents=False)
-    y = _mm(x8, weight.detach(), sx, weight_scale_inv, 1, BLOCK, None, None, None if bias is None else bias.detach(), x.dtype)
-    return y if x.dim() == 2 else y.reshape(*x.shape[:-1], y.shape[-1])
+    with torch.no_grad():
+        x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+        if eager_cuda(x2):
+            y = linear_blockwise(x2, weight, weight_scale_inv, bias)
+        else:
+            (x8, sx, _), _ = _cast(x2, N.E4M3, True, False)
+            y = _mm(x8, weight, sx, weight_scale_inv, 1, BLOCK, None, None, bias, x.dtype)
+        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], y.shape[-1])
 
 
 @torch._dynamo.allow_in_graph

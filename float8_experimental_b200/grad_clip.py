@@ -16,10 +16,11 @@ import torch.distributed as dist
 from torch.distributed._tensor import DTensor
 
 from . import _native as N
-from ._ops import eager_cuda, ops, TensorList
+from ._ops import _PLAIN as _PLAIN_TYPES, eager_cuda, ops, TensorList
 
 __all__ = ["get_total_norm", "clip_grads_with_norm_", "clip_grad_norm_"]
 
+_PLAIN = set(_PLAIN_TYPES)
 _KINDS = {math.inf: 0, 1.0: 1, 2.0: 2}
 
 
@@ -36,12 +37,10 @@ def _local(t: torch.Tensor) -> torch.Tensor:
 
 def _gradients(parameters: Union[torch.Tensor, Iterable[torch.Tensor]]) -> List[torch.Tensor]:
     """The gradients of `parameters`, each once however often its parameter is listed."""
-    params = [parameters] if isinstance(parameters, torch.Tensor) else parameters
-    found: Dict[int, torch.Tensor] = {}
-    for p in params:
-        if p.grad is not None:
-            found.setdefault(id(p), p.grad)
-    return list(found.values())
+    params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    if len(set(map(id, params))) != len(params):
+        params = list({id(p): p for p in params}.values())
+    return [g for p in params if (g := p.grad) is not None]
 
 
 def _sharded_groups(t: DTensor):
@@ -110,7 +109,7 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     (fp32, 0-dim, on their device).  `error_if_nonfinite=True` reads it back and synchronises."""
     kind = _kind_of(norm_type)
     grads = _gradients(parameters)
-    if grads and all(map(eager_cuda, grads)):
+    if grads and set(map(type, grads)) <= _PLAIN and eager_cuda(grads[0]):
         # the usual case: the tensors' addresses are gathered once for both launches
         tensors = TensorList("clip_grad_norm_", grads)
         total = torch.empty((), dtype=torch.float32, device=tensors.device)
