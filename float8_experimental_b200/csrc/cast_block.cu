@@ -71,13 +71,11 @@ struct Eight {
   __device__ __forceinline__ void load(const char* p, int n) {  // n of them exist
 #pragma unroll
     for (int j = 0; j < W; ++j) w[j] = 0u;
-    if constexpr (VEC) {
-      if (n > 0) {
+    if (VEC && n == 8) {
 #pragma unroll
-        for (int h = 0; h < W / 4; ++h) {
-          const uint4 q = __ldcs(reinterpret_cast<const uint4*>(p) + h);
-          w[4 * h] = q.x, w[4 * h + 1] = q.y, w[4 * h + 2] = q.z, w[4 * h + 3] = q.w;
-        }
+      for (int h = 0; h < W / 4; ++h) {
+        const uint4 q = __ldcs(reinterpret_cast<const uint4*>(p) + h);
+        w[4 * h] = q.x, w[4 * h + 1] = q.y, w[4 * h + 2] = q.z, w[4 * h + 3] = q.w;
       }
     } else {
 #pragma unroll
@@ -102,8 +100,8 @@ struct Eight {
 
 template <bool VEC>
 __device__ __forceinline__ void store8(uint8_t* p, int n, uint32_t lo, uint32_t hi) {
-  if constexpr (VEC) {
-    if (n > 0) *reinterpret_cast<uint2*>(p) = make_uint2(lo, hi);
+  if (VEC && n == 8) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(lo, hi);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -299,7 +297,7 @@ __global__ void __launch_bounds__(kThreads) uncast_block_kernel(const BlockUncas
     const uint8_t* q = p.q + r * p.ld_q + col;
     w[i][0] = w[i][1] = 0u;
     if (r < p.rows) {
-      if constexpr (VEC) {
+      if (VEC && n == 8) {
         const uint2 t = __ldcs(reinterpret_cast<const uint2*>(q));
         w[i][0] = t.x, w[i][1] = t.y;
       } else {
@@ -341,7 +339,7 @@ __global__ void __launch_bounds__(kThreads) uncast_block_kernel(const BlockUncas
       y[2 * j] = f.x * sc[2 * j];
       y[2 * j + 1] = f.y * sc[2 * j + 1];
     }
-    if constexpr (VEC) {
+    if (VEC && n == 8) {
       if constexpr (HP == F8B200_FP32) {
         float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.y) + r * p.ld_y + col);
         __stcs(o, make_float4(y[0], y[1], y[2], y[3]));
@@ -410,8 +408,8 @@ extern "C" int f8b200_cast_blockwise(const void* x, int hp_dtype, int64_t rows, 
   p.exp_pitch_r = exponent_pitch(rows), p.exp_pitch_c = exponent_pitch(cols);
   p.tiles_k = tiles_k;
   const int forms = by_square ? kBySquare : (out_r != nullptr ? kByRow : 0) | (out_c != nullptr ? kByCol : 0);
-  // whole 8-element chunks, loaded in 16-byte words and stored in 8-byte ones
-  const bool vec = cols % 8 == 0 && (ld_x * es) % 16 == 0 && aligned(x, 16) && aligned(out_r, 8) && aligned(out_c, 8) &&
+  // rows that allow 16-byte loads and 8-byte stores; the last chunk of a row may be shorter
+  const bool vec = (ld_x * es) % 16 == 0 && aligned(x, 16) && aligned(out_r, 8) && aligned(out_c, 8) &&
                    (out_r == nullptr || ld_r % 8 == 0) && (out_c == nullptr || ld_c % 8 == 0);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int64_t tiles = tiles_m * tiles_k;
@@ -448,7 +446,7 @@ extern "C" int f8b200_uncast_blockwise(const void* q, int fp8_kind, int64_t rows
   p.tiles_k = (cols + kBlk - 1) / kBlk;
   const int64_t tiles_m = (rows + kBlk - 1) / kBlk;
   if (tiles_m > 0x7FFFFFFFLL / p.tiles_k) return F8B200_ERR_UNSUPPORTED;
-  const bool vec = cols % 8 == 0 && ld_q % 8 == 0 && aligned(q, 8) && aligned(y, 16) && (ld_y * es) % 16 == 0;
+  const bool vec = ld_q % 8 == 0 && aligned(q, 8) && aligned(y, 16) && (ld_y * es) % 16 == 0;
   const unsigned grid = (unsigned)(tiles_m * p.tiles_k);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
 #define F8_UNCAST(HP, KIND)                                                                   \
