@@ -7,7 +7,8 @@
 // own: every block's MMAs start a fresh tensor-memory accumulator, and the epilogue warps add it, multiplied by
 // its scale, to fp32 sums that stay in registers for the whole tile.  Per block that costs a 128x256 tile's
 // CTA 32768 fp32 FMAs (256 cycles of its FMA pipes) and as many tensor-memory words against the 512 cycles of the
-// MMAs, and it runs beside them: two accumulators alternate.
+// MMAs, and it runs beside them: two accumulators alternate.  16384 x 8192 x 8192: 1.07 ms, 2.06 PFLOP/s; with a factor
+// per row on both sides one more multiplication per element, 2.07 ms.
 //
 // Two kernels:
 //   block pair kernel   two CTAs per 256x256 tile, tcgen05.mma.cta_group::2 as in the pair kernel of gemm.cu;
@@ -65,7 +66,11 @@ __device__ __forceinline__ uint64_t mul2f(uint64_t a, uint64_t b) {
   return d;
 }
 
-constexpr int BTHREADS = 320;  // TMA warp, MMA warp, 8 epilogue warps
+// TMA warp, MMA warp, two that only make their group whole, 8 epilogue warps.  A thread of the epilogue holds 128 sums,
+// more than the 168 registers that 12 warps get each leave room for: the first group hands 128 of its own over
+// (40 + 2 * 232 = 3 * 168).
+constexpr int BTHREADS = 384;
+constexpr int BREGS_FEW = 40, BREGS_MANY = 232;
 constexpr int BSTAGES = 6;
 constexpr int BSTAGE_BYTES = PA_BYTES + PB_BYTES;
 
@@ -127,66 +132,70 @@ gemm_block_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_c
   tc_fence_after();
   const uint32_t tmem_base = bars->tmem_base;
 
-  if (warp == 0) {
-    // ---------------- TMA producer (one per CTA) ----------------
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int64_t t = cluster_id; ok && t < num_tiles; t += num_clusters) {
-        const TileCoord tc = tile_coord(t, tiles_m, tiles_n, raster);
-        const int row_a = tc.m * PBM + (int)rank * 128;
-        const int row_b = tc.n * PBN + (int)rank * 128;
-        for (int kb = 0; kb < num_kb; ++kb) {
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(BREGS_FEW));
+    if (warp == 0) {
+      // ---------------- TMA producer (one per CTA) ----------------
+      if (lane == 0) {
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int64_t t = cluster_id; ok && t < num_tiles; t += num_clusters) {
+          const TileCoord tc = tile_coord(t, tiles_m, tiles_n, raster);
+          const int row_a = tc.m * PBM + (int)rank * 128;
+          const int row_b = tc.n * PBN + (int)rank * 128;
+          for (int kb = 0; kb < num_kb; ++kb) {
+            if (!pair_wait(&bars->empty[stage], phase ^ 1u, bars, peer, 1u, 64u)) { ok = false; break; }
+            uint8_t* sa = tiles + stage * BSTAGE_BYTES;
+            if (leader) mbar_expect_tx(&bars->full[stage], 2 * BSTAGE_BYTES);
+            const uint32_t full_in_leader = mapa_u32(smem_u32(&bars->full[stage]), 0u);
+            tma_load_2d_pair_plain(sa, &tma_a, a_mn ? row_a : kb * BK, a_mn ? kb * BK : row_a, full_in_leader);
+            tma_load_2d_pair_plain(sa + PA_BYTES, &tma_b, b_mn ? row_b : kb * BK, b_mn ? kb * BK : row_b,
+                                   full_in_leader);
+            if (++stage == BSTAGES) { stage = 0; phase ^= 1u; }
+          }
+        }
+        // tail: every release the leader multicast to this CTA's empty barriers has landed
+        for (int s = 0; ok && s < BSTAGES; ++s) {
           if (!pair_wait(&bars->empty[stage], phase ^ 1u, bars, peer, 1u, 64u)) { ok = false; break; }
-          uint8_t* sa = tiles + stage * BSTAGE_BYTES;
-          if (leader) mbar_expect_tx(&bars->full[stage], 2 * BSTAGE_BYTES);
-          const uint32_t full_in_leader = mapa_u32(smem_u32(&bars->full[stage]), 0u);
-          tma_load_2d_pair_plain(sa, &tma_a, a_mn ? row_a : kb * BK, a_mn ? kb * BK : row_a, full_in_leader);
-          tma_load_2d_pair_plain(sa + PA_BYTES, &tma_b, b_mn ? row_b : kb * BK, b_mn ? kb * BK : row_b,
-                                 full_in_leader);
           if (++stage == BSTAGES) { stage = 0; phase ^= 1u; }
         }
+        if (!ok) {  // give the loads in flight time to land before the CTA leaves
+          const long long t0 = clock64();
+          while (clock64() - t0 < 2000000LL) {}
+        }
       }
-      // tail: every release the leader multicast to this CTA's empty barriers has landed
-      for (int s = 0; ok && s < BSTAGES; ++s) {
-        if (!pair_wait(&bars->empty[stage], phase ^ 1u, bars, peer, 1u, 64u)) { ok = false; break; }
-        if (++stage == BSTAGES) { stage = 0; phase ^= 1u; }
-      }
-      if (!ok) {  // give the loads in flight time to land before the CTA leaves
-        const long long t0 = clock64();
-        while (clock64() - t0 < 2000000LL) {}
-      }
-    }
-  } else if (warp == 1) {
-    // ---------------- MMA issuer (leader CTA only) ----------------
-    if (leader && lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      uint32_t g = 0;  // k-blocks issued so far: their accumulators alternate
-      for (int64_t t = cluster_id; ok && t < num_tiles; t += num_clusters) {
-        for (int kb = 0; kb < num_kb; ++kb, ++g) {
-          const uint32_t acc = g & 1u;
-          if (!pair_wait(&bars->full[stage], phase, bars, peer, 4u)) { ok = false; break; }
-          if (!pair_wait(&bars->tmem_empty[acc], ((g >> 1) & 1u) ^ 1u, bars, peer, 2u)) { ok = false; break; }
-          tc_fence_after();
-          const uint32_t a_addr = smem_u32(tiles + stage * BSTAGE_BYTES);
-          const uint64_t da = a_mn ? make_smem_desc_mn(a_addr, PA_BYTES) : make_smem_desc(a_addr);
-          const uint64_t db = b_mn ? make_smem_desc_mn(a_addr + PA_BYTES, PB_BYTES) : make_smem_desc(a_addr + PA_BYTES);
-          const uint32_t tmem_d = tmem_base + acc * (uint32_t)PBN;
-#pragma unroll
-          for (int kk = 0; kk < BK / UMMA_K; ++kk)
-            tc_mma_f8_pair(tmem_d, da + (uint64_t)kk * step_a, db + (uint64_t)kk * step_b, idesc, kk != 0 ? 1u : 0u);
-          tc_commit_pair(&bars->empty[stage]);
-          tc_commit_pair(&bars->tmem_full[acc]);
-          if (++stage == BSTAGES) { stage = 0; phase ^= 1u; }
+    } else if (warp == 1) {
+      // ---------------- MMA issuer (leader CTA only) ----------------
+      if (leader && lane == 0) {
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        uint32_t g = 0;  // k-blocks issued so far: their accumulators alternate
+        for (int64_t t = cluster_id; ok && t < num_tiles; t += num_clusters) {
+          for (int kb = 0; kb < num_kb; ++kb, ++g) {
+            const uint32_t acc = g & 1u;
+            if (!pair_wait(&bars->full[stage], phase, bars, peer, 4u)) { ok = false; break; }
+            if (!pair_wait(&bars->tmem_empty[acc], ((g >> 1) & 1u) ^ 1u, bars, peer, 2u)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t a_addr = smem_u32(tiles + stage * BSTAGE_BYTES);
+            const uint64_t da = a_mn ? make_smem_desc_mn(a_addr, PA_BYTES) : make_smem_desc(a_addr);
+            const uint64_t db = b_mn ? make_smem_desc_mn(a_addr + PA_BYTES, PB_BYTES) : make_smem_desc(a_addr + PA_BYTES);
+            const uint32_t tmem_d = tmem_base + acc * (uint32_t)PBN;
+  #pragma unroll
+            for (int kk = 0; kk < BK / UMMA_K; ++kk)
+              tc_mma_f8_pair(tmem_d, da + (uint64_t)kk * step_a, db + (uint64_t)kk * step_b, idesc, kk != 0 ? 1u : 0u);
+            tc_commit_pair(&bars->empty[stage]);
+            tc_commit_pair(&bars->tmem_full[acc]);
+            if (++stage == BSTAGES) { stage = 0; phase ^= 1u; }
+          }
         }
       }
     }
   } else {
-    // ---------------- epilogue (warps 2..9 of both CTAs) ----------------
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(BREGS_MANY));
+    // ---------------- epilogue (warps 4..11 of both CTAs) ----------------
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
     const uint32_t taddr0 = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128);
     const uint32_t empty_in_leader[2] = {mapa_u32(smem_u32(&bars->tmem_empty[0]), 0u),
                                          mapa_u32(smem_u32(&bars->tmem_empty[1]), 0u)};
@@ -215,9 +224,9 @@ gemm_block_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_c
       if constexpr (PER_COL) load_cols(0); else sb = cols_in ? __ldg(pb) : 0.f;
       for (int kb = 0; kb < num_kb; ++kb, ++g) {
         const uint32_t buf = g & 1u;
-        const float* cs = bars->col_scale[warp - 2][kb & 1];
+        const float* cs = bars->col_scale[warp - 4][kb & 1];
         if constexpr (PER_COL) {
-          float* w = bars->col_scale[warp - 2][kb & 1];
+          float* w = bars->col_scale[warp - 4][kb & 1];
 #pragma unroll
           for (int j = 0; j < 4; ++j) w[lane + 32 * j] = sc[j];
           __syncwarp();
@@ -365,6 +374,10 @@ gemm_block_few_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
   const int num_kb_all = (k + BK - 1) / BK;
   const int kb0 = (int)((int64_t)num_kb_all * rank / split), kb1 = (int)((int64_t)num_kb_all * (rank + 1) / split);
   const int row_w = (int)blockIdx.y * 128, row_x = (int)blockIdx.z * T;
+  // Each tile of B starts at another k-block of its share and wraps around: in step, all CTAs would ask for the same
+  // 128 bytes of A's rows and for equal offsets of B's at the same time (72 against 61 us at 37 x 28672 x 8192).
+  const int rot = (int)(((int64_t)blockIdx.y * 5) % max(1, kb1 - kb0));
+  auto block_of = [&](int i) { const int v = i + rot; return v < kb1 ? v : v - (kb1 - kb0); };
   const uint64_t step_w = desc_k_step(w_mn != 0), step_x = desc_k_step(false);
 
   if (threadIdx.x == 0) {
@@ -401,8 +414,9 @@ gemm_block_few_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
         if (!few_wait(&bars->empty[stage], phase ^ 1u, bars, 1u)) { ok = false; break; }
         uint8_t* sw = tiles + stage * Cfg::kStageBytes;
         mbar_expect_tx(&bars->full[stage], Cfg::kStageBytes);
-        tma_load_2d(sw, &tma_w, w_mn ? row_w : kb * BK, w_mn ? kb * BK : row_w, &bars->full[stage]);
-        tma_load_2d(sw + 128 * BK, &tma_x, kb * BK, row_x, &bars->full[stage]);
+        const int at = block_of(kb) * BK;
+        tma_load_2d(sw, &tma_w, w_mn ? row_w : at, w_mn ? at : row_w, &bars->full[stage]);
+        tma_load_2d(sw + 128 * BK, &tma_x, at, row_x, &bars->full[stage]);
         if (++stage == S) { stage = 0; phase ^= 1u; }
       }
       // tail: the MMAs have read every stage (the stages are reused for the sums below)
@@ -451,7 +465,8 @@ gemm_block_few_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
       px[j] = scale_x.p + (int64_t)((px_in[j] ? r : 0) >> scale_x.shift) * scale_x.row_stride;
     }
     float sx[XL], sw = 0.f;
-    auto fetch = [&](int kb) {
+    auto fetch = [&](int i) {
+      const int kb = block_of(i);
       sw = __ldg(pw + (int64_t)kb * scale_w.kb_stride);
 #pragma unroll
       for (int j = 0; j < XL; ++j) sx[j] = px_in[j] ? __ldg(px[j] + (int64_t)kb * scale_x.kb_stride) : 0.f;
@@ -1029,11 +1044,12 @@ static uint32_t make_idesc_few(int w_kind, int x_kind, int w_mn, int cols) {
          ((uint32_t)(cols >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 
-// CTAs of one cluster that split K: as many as keep the grid within two CTAs per SM and leave each at least four
-// k-blocks, in powers of two up to 8 (the portable cluster size).
-static int few_split(int64_t tiles, int num_kb) {
+// CTAs of one cluster that split K: as many as the GPU holds at once and leave each at least four k-blocks, in powers of
+// two up to 8.  Measured (us, split 1 / 2 / 4 / 8): 8 x 8192 x 8192 33 / 25 / 25 / 29, 64 x 8192 x 28672 170 / 98 / 68 /
+// 76, 128 x 4096 x 4096 27 / 21 / 17 / 31, 37 x 28672 x 8192 72 / 80 / 82 / 94.
+static int few_split(int64_t tiles, int num_kb, int ctas_per_sm) {
   int split = 1;
-  while (split < 8 && tiles * split * 2 <= 2 * sm_count() && num_kb >= split * 2 * 4) split *= 2;
+  while (split < FEW_MAX_SPLIT && tiles * split * 2 <= (int64_t)ctas_per_sm * sm_count() && num_kb >= split * 2 * 4) split *= 2;
   return split;
 }
 
@@ -1072,7 +1088,7 @@ extern "C" int f8b200_gemm_blockwise(const void* a, int a_kind, int a_layout, in
       rc = b_layout ? gemm::encode_operand_map_mn(&mb, b, n, k, ldb) : gemm::encode_operand_map(&mb, b, n, k, ldb, 128);
     if (rc != F8B200_OK) return rc;
     const uint32_t idesc = make_idesc_few(b_kind, a_kind, b_layout, t);
-    const int split = few_split((n + 127) / 128, (int)((k + 127) / 128));
+    const int split = few_split((n + 127) / 128, (int)((k + 127) / 128), t <= 64 ? FewCfg<64>::kCtas : FewCfg<128>::kCtas);
     return dispatch_out_dtype(out_dtype, [&](auto* tag) {
       using OutT = std::remove_pointer_t<decltype(tag)>;
       auto go = [&](auto t_const) {
