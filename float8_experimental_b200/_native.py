@@ -638,6 +638,74 @@ def gemm_blockwise(a: torch.Tensor, lda: int, a_mn_major: bool, scale_a: torch.T
         )
 
 
+class BlockForm:
+    """One form of a block-scaled cast at an address inside a caller's buffer: the fp8 bytes of [rows, cols], their factors
+    and exponent bytes.  `by` is "row", "col" or "square"; as in `f8b200_cast_blockwise`.
+
+    A training step holds nine of these tensors; as tensors of their own they would cost more host time than its
+    launches."""
+
+    __slots__ = ("rows", "cols", "by", "pitch", "data", "scale", "exps", "exps_t", "nbytes")
+
+    def __init__(self, rows: int, cols: int, by: str):
+        self.rows, self.cols, self.by, self.pitch = rows, cols, by, -(-cols // 16) * 16
+        kb, rb = -(-cols // 128), -(-rows // 128)
+        factors = kb * rows if by == "row" else rb * cols if by == "col" else rb * kb
+        self.data = 0
+        self.scale = -(-rows * self.pitch // 256) * 256
+        at = self.scale + -(-4 * factors // 256) * 256
+        as_rows, as_cols = -(-rows // 256) * 1024 * -(-cols // 512), -(-cols // 256) * 1024 * -(-rows // 512)
+        self.exps = self.exps_t = None  # of the matrix and of its transpose, as operands
+        if by != "col":
+            self.exps, at = at, at + as_rows
+        if by != "row":
+            self.exps_t, at = at, at + as_cols
+        self.nbytes = at  # a multiple of 256
+
+    def at(self, base: int) -> "BlockForm":
+        self.data, self.scale = base, self.scale + base
+        self.exps = None if self.exps is None else self.exps + base
+        self.exps_t = None if self.exps_t is None else self.exps_t + base
+        return self
+
+    def operand(self, transposed: bool = False):
+        """(address, MN-major, pitch, factors, row stride, k-block stride, rows per factor, exponents) for the GEMM."""
+        if self.by == "square":
+            strides = (1, -(-self.cols // 128)) if transposed else (-(-self.cols // 128), 1)
+            return (self.data, int(transposed), self.pitch, self.scale, *strides, 128, self.exps_t if transposed else self.exps)
+        if transposed != (self.by == "col"):
+            raise F8B200Error(f"a cast by {self.by} serves the {'matrix' if transposed else 'transpose'} only")
+        return (self.data, int(transposed), self.pitch, self.scale, 1, self.cols if transposed else self.rows, 1,
+                self.exps_t if transposed else self.exps)
+
+
+def block_cast_into(x: torch.Tensor, ld_x: int, row: Optional[BlockForm], col: Optional[BlockForm]) -> None:
+    """`f8b200_cast_blockwise` of the e4m3 forms `row` (or a square one) and `col` of one matrix."""
+    first = row or col
+    square = first.by == "square"
+    r = (row.data, row.pitch, row.scale, -(-row.cols // 128) if square else row.rows, row.exps) if row else (None, 0, None, 0, None)
+    c = (col.data, col.pitch, col.scale, col.cols, col.exps_t) if col else (None, 0, None, 0, row.exps_t if square else None)
+    _require_cuda(x)
+    with _Launch("cast_block", x.device):
+        _check(
+            load().f8b200_cast_blockwise(x.data_ptr(), hp_code(x.dtype), first.rows, first.cols, ld_x, E4M3, int(square), *r, *c,
+                                         _stream(x)),
+            "f8b200_cast_blockwise",
+        )
+
+
+def block_gemm_into(a, b, bias: Optional[torch.Tensor], out: torch.Tensor, m: int, n: int, k: int, ws: int) -> None:
+    """`f8b200_gemm_blockwise` of two e4m3 `BlockForm.operand`s; `ws`: the address of a scheduling word or 0."""
+    _require_cuda(bias, out)
+    with _Launch("gemm_block", out.device):
+        _check(
+            load().f8b200_gemm_blockwise(a[0], E4M3, a[1], a[2], a[3], a[4], a[5], a[6], a[7], b[0], E4M3, b[1], b[2], b[3], b[4],
+                                         b[5], b[6], b[7], _ptr(bias), hp_code(out.dtype), out.data_ptr(), n, m, n, k,
+                                         ws or None, GEMM_WORKSPACE_BYTES if ws else 0, _stream(out)),
+            "f8b200_gemm_blockwise",
+        )
+
+
 def linear_blockwise(x: torch.Tensor, m: int, k: int, ld_x: int, weight: torch.Tensor, ldw: int, w_mn_major: bool,
                      weight_scale: torch.Tensor, bias: Optional[torch.Tensor], out: torch.Tensor, n: int) -> None:
     """out [m, n] = x [m, k] cast by rows, times the transpose of an fp8 weight with one factor per 128 x 128: the cast

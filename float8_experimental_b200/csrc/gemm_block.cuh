@@ -932,6 +932,10 @@ static int launch_block_pair(const CUtensorMap& ma, const CUtensorMap& mb, const
   const cudaError_t attr_err = setup.run(
       [&](int* clusters_out) {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BSMEM_BYTES);
+        cudaFuncAttributes fa;
+        if (e == cudaSuccess) e = cudaFuncGetAttributes(&fa, kernel);
+        // the registers that the first group hands over have to be there, or the others would wait for them
+        if (e == cudaSuccess && fa.numRegs * BTHREADS < 128 * BREGS_FEW + 256 * BREGS_MANY) e = cudaErrorInvalidConfiguration;
         if (e == cudaSuccess) {
           cfg.gridDim = dim3(2 * (sm_count() / 2));
           e = cudaOccupancyMaxActiveClusters(clusters_out, kernel, &cfg);

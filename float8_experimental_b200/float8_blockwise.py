@@ -19,8 +19,8 @@ from torch.autograd.function import once_differentiable
 
 from . import _native as N
 from ._ops import (
-    _blocks, _blockwise_mm_cuda, _cast_blockwise_some, _cast_blockwise_square_cuda, _uncast_blockwise_cuda, eager_cuda,
-    linear_blockwise, ops,
+    _as_matrix, _blocks, _blockwise_mm_cuda, _cast_blockwise_some, _cast_blockwise_square_cuda, eager_cuda,
+    linear_blockwise, _one_device, ops, _uncast_blockwise_cuda,
 )
 from .float8_utils import _kind, e4m3_dtype, e5m2_dtype
 
@@ -184,22 +184,89 @@ class _float8_linear_blockwise(torch.autograd.Function):
     bit of precision.  `need_dw` asks the input's cast for the by-column form that the weight's gradient reads."""
 
     @staticmethod
+    def _forward_eager(ctx, x, x2, weight, bias, need_dw: bool):
+        """The same launches with the casts laid out in two buffers: one that the backward pass reads, one that it does
+        not need."""
+        (m, k), n = x2.shape, weight.shape[0]
+        x2, _, _, ldx = _as_matrix(x2)
+        weight, _, _, ldw = _as_matrix(weight)
+        _one_device("blockwise_mm", x2, weight, bias)
+        xr, xc, w = N.BlockForm(m, k, "row"), N.BlockForm(m, k, "col"), N.BlockForm(n, k, "square")
+        kept = torch.empty(w.nbytes + (xc.nbytes if need_dw else 0), dtype=torch.uint8, device=x.device)
+        passing = torch.empty(xr.nbytes + N.GEMM_WORKSPACE_BYTES, dtype=torch.uint8, device=x.device)
+        w.at(kept.data_ptr())
+        if need_dw:
+            xc.at(kept.data_ptr() + w.nbytes)
+        xr.at(passing.data_ptr())
+        N.block_cast_into(x2, ldx, xr, xc if need_dw else None)
+        N.block_cast_into(weight, ldw, w, None)
+        y = torch.empty((m, n), dtype=x.dtype, device=x.device)
+        if bias is not None and bias.dtype != x.dtype:
+            bias = bias.to(x.dtype)
+        N.block_gemm_into(xr.operand(), w.operand(), bias, y, m, n, k, passing.data_ptr() + xr.nbytes)
+        ctx.save_for_backward(kept)
+        ctx.forms = (w, xc if need_dw else None)
+        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], n)
+
+    @staticmethod
+    def _backward_eager(ctx, go, go2, need_dx, need_dw):
+        (kept,), (w, xc) = ctx.saved_tensors, ctx.forms
+        if kept.data_ptr() != w.data:  # packed away and unpacked elsewhere meanwhile
+            moved = kept.data_ptr() - w.data
+            w = N.BlockForm(w.rows, w.cols, "square").at(w.data + moved)
+            xc = xc and N.BlockForm(xc.rows, xc.cols, "col").at(xc.data + moved)
+        (m, n), k = go2.shape, w.cols
+        go2, _, _, ldg = _as_matrix(go2)
+        _one_device("blockwise_mm", kept, go2)
+        gr, gc = N.BlockForm(m, n, "row") if need_dx else None, N.BlockForm(m, n, "col") if need_dw else None
+        sizes = [f.nbytes if f else 0 for f in (gr, gc)]
+        buf = torch.empty(sum(sizes) + 2 * N.GEMM_WORKSPACE_BYTES, dtype=torch.uint8, device=go.device)
+        at = buf.data_ptr()
+        if need_dx:
+            gr.at(at)
+        if need_dw:
+            gc.at(at + sizes[0])
+        ws = at + sum(sizes)
+        N.block_cast_into(go2, ldg, gr, gc)
+        dx = dw = None
+        if need_dx:  # dX = dY @ W: the weight's bytes and factors read transposed
+            dx = torch.empty((m, k), dtype=go.dtype, device=go.device)
+            N.block_gemm_into(gr.operand(), w.operand(transposed=True), None, dx, m, k, n, ws)
+            dx = dx if go.dim() == 2 else dx.reshape(*go.shape[:-1], k)
+        if need_dw:  # dW = dY^T @ X, summed over rows: both by columns
+            dw = torch.empty((n, k), dtype=ctx.dtypes[0], device=go.device)
+            N.block_gemm_into(gc.operand(transposed=True), xc.operand(transposed=True), None, dw, n, k, m,
+                              ws + N.GEMM_WORKSPACE_BYTES)
+        return dx, dw
+
+    @staticmethod
     def forward(ctx, x, weight, bias, need_dw: bool):
         x2 = x.reshape(-1, x.shape[-1])
+        ctx.dtypes = (weight.dtype, bias.dtype if bias is not None else None)
+        ctx.forms = None
+        if x2.shape[1] != weight.shape[1]:
+            raise RuntimeError(f"blockwise linear: the input has {x2.shape[1]} features, the weight {weight.shape[1]}")
+        if eager_cuda(x) and eager_cuda(weight) and x2.numel() and weight.numel():
+            return _float8_linear_blockwise._forward_eager(ctx, x, x2, weight, bias, need_dw)
         (x8, sx, ex), by_col = _cast(x2, N.E4M3, True, need_dw)
         w8, sw, ew, ewt = _cast_square(weight, N.E4M3)
         y = _mm(x8, w8, sx, sw, 1, BLOCK, ex, ew, bias, x.dtype)
         ctx.save_for_backward(*by_col, w8, sw, ewt)
-        ctx.dtypes = (weight.dtype, bias.dtype if bias is not None else None)
         return y.reshape(*x.shape[:-1], y.shape[-1])
 
     @staticmethod
     @once_differentiable
     def backward(ctx, go):
-        x8c, sxc, exc, w8, sw, ewt = ctx.saved_tensors
         need_dx, need_dw, need_db = ctx.needs_input_grad[:3]
         go2 = go.reshape(-1, go.shape[-1])
         dx = dw = db = None
+        if ctx.forms is not None:
+            if need_dx or need_dw:
+                dx, dw = _float8_linear_blockwise._backward_eager(ctx, go, go2, need_dx, need_dw)
+            if need_db:
+                db = go2.sum(0, dtype=torch.float32).to(ctx.dtypes[1])
+            return dx, dw, db, None
+        x8c, sxc, exc, w8, sw, ewt = ctx.saved_tensors
         if need_dx or need_dw:
             (g8, sg, eg), (g8c, sgc, egc) = _cast(go2, N.E4M3, need_dx, need_dw)
         if need_dx:  # dX = dY @ W: the weight's bytes and factors read transposed
