@@ -369,7 +369,10 @@ ln_bwd_kernel(const T* __restrict__ x, int64_t ld_x, const T* __restrict__ g, in
 }
 
 // ---- any width, any alignment -----------------------------------------------------------------------
-template <typename T, typename W>
+// Element by element, neighbours by neighbouring threads, so the accesses still fill whole lines.  A short row stays in
+// registers between the sums (up to 16 elements per thread forward, 4 backward: with two rows of values in registers too
+// few warps fit, 16384 x 3001 took twice the time); a longer one (E = 0) is read again from the caches.
+template <typename T, typename W, int E>
 __global__ void __launch_bounds__(kThreads)
 ln_fwd_any_kernel(const T* __restrict__ x, int64_t ld_x, int64_t rows, int64_t cols, const W* __restrict__ weight,
                   const W* __restrict__ bias, float eps, T* __restrict__ y, int64_t ld_y, float* __restrict__ mean_out,
@@ -378,27 +381,44 @@ ln_fwd_any_kernel(const T* __restrict__ x, int64_t ld_x, int64_t rows, int64_t c
   const float inv_c = 1.0f / (float)cols;
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* row = x + r * ld_x;
+    float v[E > 0 ? E : 1];
+    // fn(column, the row's value there)
+    auto each = [&](auto&& fn) {
+      if constexpr (E > 0) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          const int c = (int)threadIdx.x + i * kThreads;
+          if (c < (int)cols) fn((int64_t)c, v[i]);
+        }
+      } else {
+        for (int64_t c = threadIdx.x; c < cols; c += kThreads) fn(c, to_f32(row[c]));
+      }
+    };
+    if constexpr (E > 0) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const int c = (int)threadIdx.x + i * kThreads;
+        v[i] = c < (int)cols ? to_f32(row[c]) : 0.f;
+      }
+    }
     float s = 0.f;
-    for (int64_t c = threadIdx.x; c < cols; c += kThreads) s += to_f32(row[c]);
+    each([&](int64_t, float a) { s += a; });
     const float mean = row_sum<kThreads>(s, smem) * inv_c;
     s = 0.f;
-    for (int64_t c = threadIdx.x; c < cols; c += kThreads) {
-      const float d = to_f32(row[c]) - mean;
-      s = fmaf(d, d, s);
-    }
+    each([&](int64_t, float a) { s = fmaf(a - mean, a - mean, s); });
     const float rstd = 1.0f / sqrtf(row_sum<kThreads>(s, smem) * inv_c + eps);
     if (threadIdx.x == 0 && mean_out != nullptr) {
       mean_out[r] = mean;
       rstd_out[r] = rstd;
     }
-    for (int64_t c = threadIdx.x; c < cols; c += kThreads) {
+    each([&](int64_t c, float a) {
       const float w = weight != nullptr ? to_f32(weight[c]) : 1.f, b = bias != nullptr ? to_f32(bias[c]) : 0.f;
-      y[r * ld_y + c] = from_f32<T>(fmaf((to_f32(row[c]) - mean) * rstd, w, b));
-    }
+      y[r * ld_y + c] = from_f32<T>(fmaf((a - mean) * rstd, w, b));
+    });
   }
 }
 
-template <typename T, typename W>
+template <typename T, typename W, int E>
 __global__ void __launch_bounds__(kThreads)
 ln_dx_any_kernel(const T* __restrict__ x, int64_t ld_x, const T* __restrict__ g, int64_t ld_g, int64_t rows, int64_t cols,
                  const W* __restrict__ weight, const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
@@ -408,19 +428,42 @@ ln_dx_any_kernel(const T* __restrict__ x, int64_t ld_x, const T* __restrict__ g,
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T *xr = x + r * ld_x, *gr = g + r * ld_g;
     const float mean = mean_in[r], rstd = rstd_in[r];
-    float s1 = 0.f, s2 = 0.f;
-    for (int64_t c = threadIdx.x; c < cols; c += kThreads) {
-      const float h = to_f32(gr[c]) * (weight != nullptr ? to_f32(weight[c]) : 1.f);
-      s1 += h;
-      s2 = fmaf(h, (to_f32(xr[c]) - mean) * rstd, s2);
+    float n[E > 0 ? E : 1], h[E > 0 ? E : 1];
+    auto load = [&](int64_t c, float& nv, float& hv) {
+      nv = (to_f32(xr[c]) - mean) * rstd;
+      hv = to_f32(gr[c]) * (weight != nullptr ? to_f32(weight[c]) : 1.f);
+    };
+    auto each = [&](auto&& fn) {
+      if constexpr (E > 0) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          const int c = (int)threadIdx.x + i * kThreads;
+          if (c < (int)cols) fn((int64_t)c, n[i], h[i]);
+        }
+      } else {
+        for (int64_t c = threadIdx.x; c < cols; c += kThreads) {
+          float nv, hv;
+          load(c, nv, hv);
+          fn(c, nv, hv);
+        }
+      }
+    };
+    if constexpr (E > 0) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const int c = (int)threadIdx.x + i * kThreads;
+        n[i] = h[i] = 0.f;
+        if (c < (int)cols) load(c, n[i], h[i]);
+      }
     }
+    float s1 = 0.f, s2 = 0.f;
+    each([&](int64_t, float nv, float hv) {
+      s1 += hv;
+      s2 = fmaf(hv, nv, s2);
+    });
     s1 = row_sum<kThreads>(s1, smem) * inv_c;
     s2 = row_sum<kThreads>(s2, smem) * inv_c;
-    for (int64_t c = threadIdx.x; c < cols; c += kThreads) {
-      const float h = to_f32(gr[c]) * (weight != nullptr ? to_f32(weight[c]) : 1.f);
-      const float nv = (to_f32(xr[c]) - mean) * rstd;
-      dx[r * ld_dx + c] = from_f32<T>(rstd * (h - s1 - nv * s2));
-    }
+    each([&](int64_t c, float nv, float hv) { dx[r * ld_dx + c] = from_f32<T>(rstd * (hv - s1 - nv * s2)); });
   }
 }
 
@@ -435,6 +478,7 @@ ln_dw_any_kernel(const T* __restrict__ x, int64_t ld_x, const T* __restrict__ g,
   const int64_t c = (int64_t)blockIdx.x * 64 + cx;
   float dw = 0.f, db = 0.f;
   if (c < cols) {
+#pragma unroll 4
     for (int64_t r = (int64_t)blockIdx.y * 4 + ry; r < rows; r += (int64_t)gridDim.y * 4) {
       const float gv = to_f32(g[r * ld_g + c]);
       dw = fmaf(gv, (to_f32(x[r * ld_x + c]) - mean_in[r]) * rstd_in[r], dw);
@@ -501,7 +545,12 @@ int ln_fwd(const void* x, int64_t rows, int64_t cols, int64_t ld_x, const void* 
   else if (vec && chunks <= 512) F8_LN(256, 2);
   else if (vec && chunks <= 1024) F8_LN(256, 4);
   else if (vec && chunks <= 2048) F8_LN(256, 8);
-  else ln_fwd_any_kernel<T, W><<<row_grid(rows), kThreads, 0, st>>>(xp, ld_x, rows, cols, wp, bp, eps, yp, ld_y, mean, rstd);
+#undef F8_LN
+#define F8_LN(E) ln_fwd_any_kernel<T, W, E><<<row_grid(rows), kThreads, 0, st>>>(xp, ld_x, rows, cols, wp, bp, eps, yp, ld_y, mean, rstd)
+  else if (cols <= 4 * kThreads) F8_LN(4);
+  else if (cols <= 8 * kThreads) F8_LN(8);
+  else if (cols <= 16 * kThreads) F8_LN(16);
+  else F8_LN(0);
 #undef F8_LN
   return check_launch();
 }
@@ -552,9 +601,13 @@ int ln_bwd(const void* x, const void* g, int64_t rows, int64_t cols, int64_t ld_
                                                                             static_cast<W*>(db));
     return check_launch();
   }
-  if (dx != nullptr)
-    ln_dx_any_kernel<T, W><<<row_grid(rows), kThreads, 0, st>>>(xp, ld_x, gp, ld_g, rows, cols, static_cast<const W*>(weight),
-                                                                mean, rstd, static_cast<T*>(dx), ld_dx);
+#define F8_LN(E)                                                                                                      \
+  ln_dx_any_kernel<T, W, E><<<row_grid(rows), kThreads, 0, st>>>(xp, ld_x, gp, ld_g, rows, cols, static_cast<const W*>(weight), \
+                                                                 mean, rstd, static_cast<T*>(dx), ld_dx)
+  if (dx == nullptr) {}
+  else if (cols <= 4 * kThreads) F8_LN(4);
+  else F8_LN(0);
+#undef F8_LN
   if (dw != nullptr || db != nullptr) {
     const int64_t groups = (rows + 3) / 4;
     const int parts = (int)(groups < kMaxParts ? groups : kMaxParts);
