@@ -63,12 +63,15 @@ class Float8BlockTensor:
         self._exps = self._exps_t = self._version = None
 
     def _with_exponents(self, exps, exps_t) -> "Float8BlockTensor":
-        self._exps, self._exps_t, self._version = exps, exps_t, self.scale_inv._version
+        if not self.scale_inv.is_inference():  # those do not tell when they are written to
+            self._exps, self._exps_t, self._version = exps, exps_t, self.scale_inv._version
         return self
 
     def _exponents(self, transposed: bool = False) -> Optional[torch.Tensor]:
         """The exponent bytes, unless the factors were written to since the cast."""
-        return (self._exps_t if transposed else self._exps) if self._version == self.scale_inv._version else None
+        if self._version is None or self._version != self.scale_inv._version:
+            return None
+        return self._exps_t if transposed else self._exps
 
     @property
     def shape(self) -> torch.Size:

@@ -7,6 +7,8 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.distributed._functional_collectives import AsyncCollectiveTensor
+from torch.distributed._tensor import DTensor
 
 from . import _native as N
 from ._ops import ops
@@ -267,7 +269,7 @@ class Float8Linear(torch.nn.Linear):
 
     def _forward_blockwise(self, input: torch.Tensor) -> torch.Tensor:
         for name, t in (("input", input), ("weight", self.weight)):
-            if type(t) not in (torch.Tensor, torch.nn.Parameter):
+            if isinstance(t, (DTensor, AsyncCollectiveTensor, Float8Tensor)):
                 raise RuntimeError(f"ScalingType.BLOCKWISE takes plain tensors, got a {type(t).__name__} as {name}")
         if torch.is_autocast_enabled(input.device.type):
             input = input.to(torch.get_autocast_dtype(input.device.type))

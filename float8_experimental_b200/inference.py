@@ -100,7 +100,7 @@ class Float8InferenceLinear(torch.nn.Linear):
         return torch.nn.functional.linear(x_fp8, self.weight, self.bias)
 
     def _forward_blockwise(self, input: torch.Tensor) -> torch.Tensor:
-        if type(input) not in (torch.Tensor, nn.Parameter):
+        if tensor_already_casted_to_fp8(input):
             raise RuntimeError(f"ActivationCasting.BLOCKWISE takes plain tensors, got a {type(input).__name__}")
         return linear_by_rows(input, self.weight, self.weight_scale_inv, self.bias)
 

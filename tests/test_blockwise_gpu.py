@@ -1,4 +1,5 @@
 """Block-scaled casts and products on the GPU against 64-bit restatements."""
+import gc
 import pytest
 import torch
 
@@ -12,6 +13,16 @@ from float8_experimental_b200.float8_blockwise import (
 from float8_experimental_b200.float8_linear import Float8Linear
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True, scope="module")
+def leave_no_tensors():
+    """What failed calls left in reference cycles (tracebacks hold their frames) goes now, not in the middle of another
+    file's count of allocated bytes."""
+    yield
+    gc.collect()
+
+
 E4, E5 = torch.float8_e4m3fn, torch.float8_e5m2
 BF, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
 
@@ -392,6 +403,29 @@ def test_streams_and_graphs():
                     g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(o, layer(x)) for o, x in zip(outs, static))
+
+
+def test_inference_mode():
+    x, w = randn(200, 256, seed=1).to(BF), randn(64, 256, seed=2).to(BF)
+    layer = Float8Linear.from_float(torch.nn.Linear(256, 64, device="cuda", dtype=BF), blockwise_config())
+    want = layer(x).detach()
+    with torch.inference_mode():
+        a, b = cast_to_float8_blockwise(x), cast_to_float8_blockwise(w, (128, 128))
+        y = blockwise_mm(a, b.t(), FP32)
+        assert torch.equal(layer(x), want)
+    ref, mag = product(a.data, a.scale_inv, 1, b.data, b.scale_inv, 128)
+    assert float(((y - ref).abs() - product_tolerance(ref, mag, 256, FP32)).max()) <= 0
+
+
+def test_saved_tensors_may_move():
+    """A step whose saved tensors are packed away and come back as copies gives the same gradients."""
+    layer = Float8Linear.from_float(torch.nn.Linear(384, 256, device="cuda", dtype=BF), blockwise_config())
+    x, go = randn(300, 384, seed=1).to(BF).requires_grad_(), randn(300, 256, seed=2).to(BF)
+    want = torch.autograd.grad(layer(x), [x, layer.weight, layer.bias], go)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.cuda()):
+        y = layer(x)
+    got = torch.autograd.grad(y, [x, layer.weight, layer.bias], go)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
 
 
 def test_refusals_on_the_gpu():

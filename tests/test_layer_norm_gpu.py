@@ -1,4 +1,5 @@
 """Layer norm, forward and backward, against a 64-bit restatement and against differences."""
+import gc
 import pytest
 import torch
 
@@ -7,6 +8,16 @@ from float8_experimental_b200._ops import ops
 from float8_experimental_b200.layer_norm import layer_norm, LayerNorm
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True, scope="module")
+def leave_no_tensors():
+    """What failed calls left in reference cycles (tracebacks hold their frames) goes now, not in the middle of another
+    file's count of allocated bytes."""
+    yield
+    gc.collect()
+
+
 BF, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
 EPS = 1e-5
 U = 2.0 ** -24  # half a step of fp32
