@@ -376,16 +376,20 @@ def _uncast_blockwise_cuda(q, scale_inv, block_rows: int, block_cols: int, dtype
     return y
 
 
+def _check_factors(name: str, s, rows: int, k: int, block: int) -> None:
+    if s.dtype != torch.float32 or s.shape != (-(-rows // 128) if block == 128 else rows, -(-k // 128)):
+        want = (_blocks(rows) if block == 128 else rows, _blocks(k))
+        raise RuntimeError(f"blockwise_mm: {name} must be float32 {want}, got {s.dtype} {tuple(s.shape)}")
+
+
 def _blockwise_mm_cuda(a, b_t, scale_a, scale_b, a_block_rows: int, b_block_rows: int, exp_a, exp_b, bias, out_dtype):
     _one_device("blockwise_mm", a, b_t, scale_a, scale_b, exp_a, exp_b, bias)
     m, k = a.shape
     n, k2 = b_t.shape
     if k != k2:
         raise RuntimeError(f"blockwise_mm: inner dimensions differ ({k} vs {k2})")
-    for name, s, rows, block in (("scale_a", scale_a, m, a_block_rows), ("scale_b", scale_b, n, b_block_rows)):
-        want = (_blocks(rows) if block == 128 else rows, _blocks(k))
-        if s.dtype != torch.float32 or tuple(s.shape) != want:
-            raise RuntimeError(f"blockwise_mm: {name} must be float32 {want}, got {s.dtype} {tuple(s.shape)}")
+    _check_factors("scale_a", scale_a, m, k, a_block_rows)
+    _check_factors("scale_b", scale_b, n, k, b_block_rows)
     for name, e, rows in (("exp_a", exp_a, m), ("exp_b", exp_b, n)):
         if e is not None and (e.dtype != torch.uint8 or not e.is_contiguous() or e.numel() != _exponent_bytes(rows, k)):
             raise RuntimeError(f"blockwise_mm: {name} must be the {_exponent_bytes(rows, k)} exponent bytes of its cast")
@@ -444,20 +448,26 @@ def _affine_dtype(x, weight, bias) -> torch.dtype:
     return affine
 
 
-def _layer_norm_cuda(x, weight, bias, eps: float, save_stats: bool):
+def layer_norm_into(x, weight, bias, eps: float, mean, rstd):
+    """y, and the rows' mean and 1/std when they are asked for: eager CUDA tensors, without autograd."""
     _one_device("layer_norm", x, weight, bias)
     if x.dim() == 0 or x.shape[-1] == 0:
         raise RuntimeError("layer_norm: the last dimension must have at least one element")
     affine = _affine_dtype(x, weight, bias)
     xm, rows, cols, ld = _as_matrix(x)
-    y = _empty_like_shape(x, x.dtype)
-    # two tensors of their own: views of one would share its version counter and outlive it together
-    mean = torch.empty(rows if save_stats else 0, dtype=torch.float32, device=x.device)
-    rstd = torch.empty(rows if save_stats else 0, dtype=torch.float32, device=x.device)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if rows:
         N.layer_norm(xm, rows, cols, ld, None if weight is None else weight.contiguous(),
-                     None if bias is None else bias.contiguous(), affine, eps, y, mean if save_stats else None,
-                     rstd if save_stats else None)
+                     None if bias is None else bias.contiguous(), affine, eps, y, mean, rstd)
+    return y
+
+
+def _layer_norm_cuda(x, weight, bias, eps: float, save_stats: bool):
+    rows = x.numel() // x.shape[-1] if save_stats and x.dim() and x.shape[-1] else 0
+    # two tensors of their own: views of one would share its version counter and outlive it together
+    mean = torch.empty(rows, dtype=torch.float32, device=x.device)
+    rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
+    y = layer_norm_into(x, weight, bias, eps, mean if save_stats else None, rstd if save_stats else None)
     return y, mean, rstd
 
 

@@ -62,10 +62,16 @@ class Float8BlockTensor:
         self.data, self.scale_inv, self.block, self.orig_dtype = data, scale_inv, block, orig_dtype
         self._exps = self._exps_t = self._version = None
 
-    def _with_exponents(self, exps, exps_t) -> "Float8BlockTensor":
-        if not self.scale_inv.is_inference():  # those do not tell when they are written to
-            self._exps, self._exps_t, self._version = exps, exps_t, self.scale_inv._version
-        return self
+    @classmethod
+    def _of_cast(cls, data, scale_inv, block, orig_dtype, exps, exps_t) -> "Float8BlockTensor":
+        """What a cast made: nothing to check, and the exponent bytes beside it."""
+        out = object.__new__(cls)
+        out.data, out.scale_inv, out.block, out.orig_dtype = data, scale_inv, block, orig_dtype
+        if scale_inv.is_inference():  # does not tell when it is written to
+            exps = exps_t = None
+        out._exps, out._exps_t = exps, exps_t
+        out._version = None if exps is None and exps_t is None else scale_inv._version
+        return out
 
     def _exponents(self, transposed: bool = False) -> Optional[torch.Tensor]:
         """The exponent bytes, unless the factors were written to since the cast."""
@@ -83,7 +89,8 @@ class Float8BlockTensor:
 
     def t(self) -> "Float8BlockTensor":
         """The transposed matrix: the same bytes and factors, nothing copied."""
-        out = Float8BlockTensor(self.data.t(), self.scale_inv.t(), self.block[::-1], self.orig_dtype)
+        out = object.__new__(Float8BlockTensor)
+        out.data, out.scale_inv, out.block, out.orig_dtype = self.data.t(), self.scale_inv.t(), self.block[::-1], self.orig_dtype
         out._exps, out._exps_t, out._version = self._exps_t, self._exps, self._version
         return out
 
@@ -116,7 +123,7 @@ def _matrix(x: torch.Tensor, what: str) -> torch.Tensor:
     if x.dim() != 2:
         raise ValueError(f"{what}: takes a matrix, got {x.dim()} dimensions")
     N.hp_code(x.dtype)  # bf16, fp16 or fp32
-    return x.detach()
+    return x.detach() if x.requires_grad else x
 
 
 def cast_to_float8_blockwise(x: torch.Tensor, block: Tuple[int, int] = (1, BLOCK),
@@ -134,7 +141,7 @@ def cast_to_float8_blockwise(x: torch.Tensor, block: Tuple[int, int] = (1, BLOCK
     else:
         _, (data, scale, exps_t) = _cast(x, kind, False, True)
         exps = None
-    return Float8BlockTensor(data, scale, block, x.dtype)._with_exponents(exps, exps_t)
+    return Float8BlockTensor._of_cast(data, scale, block, x.dtype, exps, exps_t)
 
 
 def cast_to_float8_blockwise_both(x: torch.Tensor, float8_dtype: torch.dtype = e4m3_dtype
@@ -142,8 +149,8 @@ def cast_to_float8_blockwise_both(x: torch.Tensor, float8_dtype: torch.dtype = e
     """`x` cast by rows (1 x 128 blocks) and by columns (128 x 1), from one read of it."""
     x = _matrix(x, "cast_to_float8_blockwise_both")
     (data, scale, exps), (data_c, scale_c, exps_c) = _cast(x, _kind(float8_dtype), True, True)
-    return (Float8BlockTensor(data, scale, (1, BLOCK), x.dtype)._with_exponents(exps, None),
-            Float8BlockTensor(data_c, scale_c, (BLOCK, 1), x.dtype)._with_exponents(None, exps_c))
+    return (Float8BlockTensor._of_cast(data, scale, (1, BLOCK), x.dtype, exps, None),
+            Float8BlockTensor._of_cast(data_c, scale_c, (BLOCK, 1), x.dtype, None, exps_c))
 
 
 def blockwise_mm(a: Float8BlockTensor, b: Float8BlockTensor, out_dtype: torch.dtype = torch.bfloat16,

@@ -13,19 +13,16 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native as N
-from ._ops import _layer_norm_bwd_cuda, _layer_norm_cuda, eager_cuda, ops
+from ._ops import _layer_norm_bwd_cuda, _layer_norm_cuda, eager_cuda, layer_norm_into, ops
 
 __all__ = ["layer_norm", "LayerNorm"]
-
-
-def _forward(x, *args):
-    return _layer_norm_cuda(x, *args) if eager_cuda(x) else ops.layer_norm(x, *args)
 
 
 class _LayerNormFunc(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = _forward(x, weight, bias, eps, True)
+        forward = _layer_norm_cuda if eager_cuda(x) else ops.layer_norm
+        y, mean, rstd = forward(x, weight, bias, eps, True)
         ctx.save_for_backward(x, weight, mean, rstd)
         ctx.affine_dtype = next((t.dtype for t in (weight, bias) if t is not None), x.dtype)
         return y
@@ -49,7 +46,9 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     N.hp_code(x.dtype)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         return _LayerNormFunc.apply(x, weight, bias, float(eps))
-    return _forward(x, weight, bias, float(eps), False)[0]
+    if eager_cuda(x):
+        return layer_norm_into(x, weight, bias, float(eps), None, None)
+    return ops.layer_norm(x, weight, bias, float(eps), False)[0]
 
 
 class LayerNorm(torch.nn.LayerNorm):
