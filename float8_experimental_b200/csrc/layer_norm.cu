@@ -8,6 +8,7 @@
 // w and b have x's type or fp32; either may be absent (1 and 0).  Sums run in a fixed order.
 //
 // Memory bounds both directions: x read and y written (4 bytes per 16-bit element), x and g read and dx written (6).
+// 16384 x 8192 bf16: forward 95 us, 5.7 TB/s in the kernel; backward 155 us, 5.2 TB/s.
 #include <type_traits>
 
 #include "common.cuh"
@@ -95,33 +96,37 @@ __device__ __forceinline__ void load_affine(const W* p, int64_t i, float none, f
   }
 }
 
-// Sum over the ROWT threads of a row (a warp, or the whole CTA), the same value in all of them.
+// Sum over the ROWT threads of a row (a warp, several, or the whole CTA), the same value in all of them.  Successive
+// calls take two buffers in turn: a buffer is written again only behind the other one's barrier, so one barrier
+// per sum is enough.
 template <int ROWT>
 __device__ __forceinline__ float row_sum(float v, float* smem) {
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, off);
   if constexpr (ROWT > 32) {
     constexpr int W = ROWT / 32;
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, group = threadIdx.x / ROWT;
     if (lane == 0) smem[w] = v;
-    __syncthreads();
-    v = lane < W ? smem[lane] : 0.f;
+    if constexpr (ROWT == kThreads) __syncthreads();
+    else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(ROWT) : "memory");
+    v = 0.f;
 #pragma unroll
-    for (int off = W / 2; off > 0; off >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, off);
-    v = __shfl_sync(0xFFFFFFFFu, v, 0);
-    __syncthreads();
+    for (int i = 0; i < W; ++i) v += smem[group * W + i];
   }
   return v;
 }
 
 // ---- forward, a row in registers --------------------------------------------------------------------
+// As few threads per row as hold it in four 16-byte pieces each: several rows per CTA then wait for their sums at
+// different times (16384 x 4096 bf16 with 128 threads per row 53 us, with 256 66 us; 32768 x 2048 with 64 53 us, with 256
+// 76 us, with one warp and eight pieces 59 us).
 template <typename T, typename W, int ROWT, int CH>
 __global__ void __launch_bounds__(kThreads)
 ln_fwd_kernel(const T* __restrict__ x, int64_t ld_x, int64_t rows, int64_t cols, const W* __restrict__ weight,
               const W* __restrict__ bias, float eps, T* __restrict__ y, int64_t ld_y, float* __restrict__ mean_out,
               float* __restrict__ rstd_out) {
   constexpr int N = Vec<T>::N, RPB = kThreads / ROWT;
-  __shared__ float smem[kThreads / 32];
+  __shared__ float smem[2][kThreads / 32];
   const int t = threadIdx.x % ROWT;
   const int chunks = (int)(cols / N);
   const float inv_c = 1.0f / (float)cols;
@@ -138,7 +143,7 @@ ln_fwd_kernel(const T* __restrict__ x, int64_t ld_x, int64_t rows, int64_t cols,
 #pragma unroll
       for (int j = 0; j < N; ++j) s += v[j];
     }
-    const float mean = row_sum<ROWT>(s, smem) * inv_c;
+    const float mean = row_sum<ROWT>(s, smem[0]) * inv_c;
     s = 0.f;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
@@ -149,7 +154,7 @@ ln_fwd_kernel(const T* __restrict__ x, int64_t ld_x, int64_t rows, int64_t cols,
         for (int j = 0; j < N; ++j) s = fmaf(v[j] - mean, v[j] - mean, s);
       }
     }
-    const float rstd = 1.0f / sqrtf(row_sum<ROWT>(s, smem) * inv_c + eps);
+    const float rstd = 1.0f / sqrtf(row_sum<ROWT>(s, smem[1]) * inv_c + eps);
     if (t == 0 && mean_out != nullptr) {
       mean_out[r] = mean;
       rstd_out[r] = rstd;
@@ -377,7 +382,7 @@ __global__ void __launch_bounds__(kThreads)
 ln_fwd_any_kernel(const T* __restrict__ x, int64_t ld_x, int64_t rows, int64_t cols, const W* __restrict__ weight,
                   const W* __restrict__ bias, float eps, T* __restrict__ y, int64_t ld_y, float* __restrict__ mean_out,
                   float* __restrict__ rstd_out) {
-  __shared__ float smem[kThreads / 32];
+  __shared__ float smem[2][kThreads / 32];
   const float inv_c = 1.0f / (float)cols;
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* row = x + r * ld_x;
@@ -403,10 +408,10 @@ ln_fwd_any_kernel(const T* __restrict__ x, int64_t ld_x, int64_t rows, int64_t c
     }
     float s = 0.f;
     each([&](int64_t, float a) { s += a; });
-    const float mean = row_sum<kThreads>(s, smem) * inv_c;
+    const float mean = row_sum<kThreads>(s, smem[0]) * inv_c;
     s = 0.f;
     each([&](int64_t, float a) { s = fmaf(a - mean, a - mean, s); });
-    const float rstd = 1.0f / sqrtf(row_sum<kThreads>(s, smem) * inv_c + eps);
+    const float rstd = 1.0f / sqrtf(row_sum<kThreads>(s, smem[1]) * inv_c + eps);
     if (threadIdx.x == 0 && mean_out != nullptr) {
       mean_out[r] = mean;
       rstd_out[r] = rstd;
@@ -423,7 +428,7 @@ __global__ void __launch_bounds__(kThreads)
 ln_dx_any_kernel(const T* __restrict__ x, int64_t ld_x, const T* __restrict__ g, int64_t ld_g, int64_t rows, int64_t cols,
                  const W* __restrict__ weight, const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
                  T* __restrict__ dx, int64_t ld_dx) {
-  __shared__ float smem[kThreads / 32];
+  __shared__ float smem[2][kThreads / 32];
   const float inv_c = 1.0f / (float)cols;
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T *xr = x + r * ld_x, *gr = g + r * ld_g;
@@ -461,8 +466,8 @@ ln_dx_any_kernel(const T* __restrict__ x, int64_t ld_x, const T* __restrict__ g,
       s1 += hv;
       s2 = fmaf(hv, nv, s2);
     });
-    s1 = row_sum<kThreads>(s1, smem) * inv_c;
-    s2 = row_sum<kThreads>(s2, smem) * inv_c;
+    s1 = row_sum<kThreads>(s1, smem[0]) * inv_c;
+    s2 = row_sum<kThreads>(s2, smem[1]) * inv_c;
     each([&](int64_t c, float nv, float hv) { dx[r * ld_dx + c] = from_f32<T>(rstd * (hv - s1 - nv * s2)); });
   }
 }
@@ -541,8 +546,8 @@ int ln_fwd(const void* x, int64_t rows, int64_t cols, int64_t ld_x, const void* 
       xp, ld_x, rows, cols, wp, bp, eps, yp, ld_y, mean, rstd)
   if (vec && chunks <= 32) F8_LN(32, 1);
   else if (vec && chunks <= 128) F8_LN(32, 4);
-  else if (vec && chunks <= 256) F8_LN(256, 1);
-  else if (vec && chunks <= 512) F8_LN(256, 2);
+  else if (vec && chunks <= 256) F8_LN(64, 4);
+  else if (vec && chunks <= 512) F8_LN(128, 4);
   else if (vec && chunks <= 1024) F8_LN(256, 4);
   else if (vec && chunks <= 2048) F8_LN(256, 8);
 #undef F8_LN
