@@ -10,6 +10,7 @@
 //
 // One CTA takes a 128 x 128 tile, so every block lies inside one CTA and x is read once for all the forms asked
 // for: 256 threads, 8 columns and 8 rows (16 apart) per thread, held in registers.
+// Memory bounds it: 16384 x 8192 bf16 by rows 64 us (6.3 TB/s), by rows and columns 111 us (4.8 TB/s), back 70 us (5.8).
 #include "common.cuh"
 
 namespace f8b200 {
