@@ -2,7 +2,7 @@
 (partial sums of every tensor, their sum, the scaling, which the device skips when nothing exceeds the bound) in
 place of several per tensor, and without a host synchronisation.
 
-Gradients of one call lie on one device; bf16, fp16 and fp32 may be mixed.  DTensor gradients (FSDP2, tensor
+Gradients of one call lie on one device and do not overlap in memory; bf16, fp16 and fp32 may be mixed.  DTensor gradients (FSDP2, tensor
 parallel) count once over their mesh: the local sums are all-reduced over the mesh dimensions a tensor is
 sharded on.
 """
@@ -36,11 +36,14 @@ def _local(t: torch.Tensor) -> torch.Tensor:
 
 
 def _gradients(parameters: Union[torch.Tensor, Iterable[torch.Tensor]]) -> List[torch.Tensor]:
-    """The gradients of `parameters`, each once however often its parameter is listed."""
+    """The gradients of `parameters`, each once however often it or its parameter is listed."""
     params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     if len(set(map(id, params))) != len(params):
         params = list({id(p): p for p in params}.values())
-    return [g for p in params if (g := p.grad) is not None]
+    grads = [g for p in params if (g := p.grad) is not None]
+    if len(set(map(id, grads))) != len(grads):  # parameters that share one gradient tensor
+        grads = list({id(g): g for g in grads}.values())
+    return grads
 
 
 def _sharded_groups(t: DTensor):

@@ -138,6 +138,10 @@ def test_each_parameter_counts_once():
     assert float(clip_grad_norm_([p, p], 3.0)) == 6.0
     assert bool(((g - 1.5).abs() <= 1e-6).all())
     assert float(clip_grad_norm_(p, 100.0)) == pytest.approx(3.0, rel=1e-6)
+    shared = torch.full((4,), 3.0, device="cuda")
+    tied = params_of([shared, shared])
+    assert float(clip_grad_norm_(tied, 3.0)) == 6.0
+    assert bool(((shared - 1.5).abs() <= 1e-6).all())
     gen_params = (q for q in [p])
     assert float(clip_grad_norm_(gen_params, 100.0)) == pytest.approx(3.0, rel=1e-6)
 
