@@ -579,11 +579,19 @@ gemm_block_few_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
 // ---------------------------------------------------------------------------------------------------
 // Factors that are powers of two: the tensor cores apply them.  tcgen05.mma.kind::mxf8f6f4.block_scale multiplies the
 // products of 32 consecutive k by 2^(ea + eb - 254), one exponent byte per operand row and 32 k, read from tensor
-// memory; a block of 128 is four such steps with the same byte, so the accumulator stays in tensor memory over all
-// of K and the epilogue runs once per tile, as in the kernels with one factor per tensor.
+// memory; a block of 128 is four such steps with the same byte, so the accumulator stays in tensor memory over many
+// of them and the epilogue runs once per tile and chunk of K.
+//
+// The tensor cores cut each new sum of a step of 32 k off towards zero at fp32's last place: the error has one sign and grows
+// with the number of steps added to one accumulator (values of one sign, relative to the result: 5e-7 at K = 2048, 3.8e-6 at
+// 8192, 1.9e-5 at 28672, 5.9e-5 at 65536; normal values a quarter to an eighth of that).  So K is cut into equal chunks of
+// at most XCHUNK_* k-blocks, each with an accumulator of its own; eight epilogue warps per CTA add the chunks, rounding
+// to nearest, in registers, one row and 128 columns per thread.  A chunk's hand-over costs half a microsecond per tile
+// (16384 x 8192 x 8192: 833 us uncut, 834 with 64 k-blocks per chunk, 848 with 32, 877 with 16, 932 with 8).  16-bit outputs
+// take 32: the error stays below 1.4e-6, a hundredth of fp16's half step and less of bf16's; fp32 outputs 16: below 5e-7.
 //
 // Tensor memory (512 columns): two accumulators of 256 columns that share 64 of them, at 0 and 192, and the
-// factors at 448.  The epilogue reads the shared columns first and then lets the next tile's MMAs start, which go to
+// factors at 448.  The epilogue reads the shared columns first and then lets the next chunk's MMAs start, which go to
 // the other accumulator, while it drains the rest.
 // Factors: one 32-bit word per operand row holds a group of four k-blocks' bytes.  Per group TMA brings 128 words of A
 // (this CTA's rows) and 256 of B (the pair's), tcgen05.cp takes them to tensor memory, and the instruction descriptor
@@ -594,7 +602,8 @@ gemm_block_few_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
 // another block's MMAs, cost 2 % more time than copies that the group's own MMAs follow; a ring of their own
 // with its own commits cost 9 %.)
 // ---------------------------------------------------------------------------------------------------
-constexpr int XTHREADS = 192;  // TMA warp, MMA warp, 4 epilogue warps
+constexpr int XTHREADS = BTHREADS;  // warps as in the kernel above; 56 + 2 * 224 = 3 * 168 registers
+constexpr int XREGS_FEW = 56, XREGS_MANY = 224;  // the MMA warp's loop spills with 40 (1.2 % of the time)
 constexpr int XSTAGES = 5;
 constexpr int XSF_A = 512, XSF_B = 1024;  // bytes of factors per CTA and four k-blocks
 constexpr int XSTAGE_BYTES = PA_BYTES + PB_BYTES;
@@ -606,12 +615,14 @@ struct __align__(16) ScaledBars {
   uint64_t full[XSTAGES];
   uint64_t empty[XSTAGES];
   uint64_t tmem_full[2];
-  uint64_t tmem_shared_free;  // in the leader: 8 arrivals, the shared columns have been read
+  uint64_t tmem_shared_free;  // in the leader: 16 arrivals, the shared columns have been read
   TileRing ring;  // written in both CTAs by the leader's producer thread
   uint32_t tmem_base;
   volatile uint32_t abort_flag;
 };
-constexpr int XSMEM_BYTES = XSTAGES * (XSTAGE_BYTES + XSF_BYTES) + EPI_STAGING_BYTES + 1024 + (int)sizeof(ScaledBars);
+constexpr int XSTAGING_BYTES = 8 /*warps*/ * EPI_BOX_BYTES;
+constexpr int XSMEM_BYTES = XSTAGES * (XSTAGE_BYTES + XSF_BYTES) + XSTAGING_BYTES + 1024 + (int)sizeof(ScaledBars);
+constexpr int XCHUNK_32 = 16, XCHUNK_16 = 32;  // k-blocks per accumulator for fp32 and 16-bit outputs
 
 __device__ __forceinline__ void tc_mma_mx_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
                                                uint32_t tmem_sa, uint32_t tmem_sb, uint32_t accumulate) {
@@ -641,10 +652,9 @@ static uint32_t make_idesc_scaled(int a_kind, int b_kind, int a_mn, int b_mn) {
          ((uint32_t)(PBN >> 3) << 17) | (1u << 23) | ((uint32_t)(PBM >> 4) << 24);
 }
 
-// 64 accumulator columns of this warp's 32 rows, already in registers, to the output.
+// 64 columns of this warp's 32 rows to the output, through one staging box per warp (128 bytes wide).
 template <typename OutT>
-__device__ __forceinline__ void store_columns(const EpilogueArgs<OutT>& e, const uint32_t (&r)[2][32], int row0, int col,
-                                              uint32_t& boxes) {
+__device__ __forceinline__ void store_columns(const EpilogueArgs<OutT>& e, const float* v64, int row0, int col, uint32_t& boxes) {
   constexpr int COLS_PER_BOX = 128 / (int)sizeof(OutT);
   const int lane = threadIdx.x & 31, row = row0 + lane;
 #pragma unroll
@@ -652,7 +662,7 @@ __device__ __forceinline__ void store_columns(const EpilogueArgs<OutT>& e, const
     const int c0 = col + 32 * h, ncols = min(32, e.n - c0);
     float v[32];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[h][i]);
+    for (int i = 0; i < 32; ++i) v[i] = v64[32 * h + i];
     if (e.bias != nullptr && ncols > 0) {
 #pragma unroll
       for (int i = 0; i < 32; ++i)
@@ -665,12 +675,11 @@ __device__ __forceinline__ void store_columns(const EpilogueArgs<OutT>& e, const
     const bool first = COLS_PER_BOX == 32 || h == 0, last = COLS_PER_BOX == 32 || h == 1;
     const int box_col = COLS_PER_BOX == 32 ? c0 : col;
     if (box_col >= e.n || row0 >= e.m) continue;  // the same for the whole warp; partial boxes are clipped by the map
-    uint8_t* box = e.staging + (boxes & 1u) * EPI_BOX_BYTES;
-    if (first && boxes >= 2u) {  // the store issued two boxes ago must have read this one
-      if (lane == 0) bulk_wait_read<1>();
+    if (first && boxes != 0u) {  // the store before this one must have read the box
+      if (lane == 0) bulk_wait_read<0>();
       __syncwarp();
     }
-    uint8_t* rowp = box + lane * 128;  // 16-byte chunk j of row `lane` lives at j ^ (lane & 7)
+    uint8_t* rowp = e.staging + lane * 128;  // 16-byte chunk j of row `lane` lives at j ^ (lane & 7)
     if constexpr (sizeof(OutT) == 2) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -691,7 +700,7 @@ __device__ __forceinline__ void store_columns(const EpilogueArgs<OutT>& e, const
       fence_async_smem();
       __syncwarp();
       if (lane == 0) {
-        tma_store_2d_hint(e.tma_out, box, box_col, row0, l2_policy(1));
+        tma_store_2d_hint(e.tma_out, e.staging, box_col, row0, l2_policy(1));
         bulk_commit();
       }
       ++boxes;
@@ -705,11 +714,11 @@ gemm_block_scaled_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid
                          const __grid_constant__ CUtensorMap tma_ea, const __grid_constant__ CUtensorMap tma_eb,
                          const __grid_constant__ CUtensorMap tma_out, const OutT* __restrict__ bias,
                          OutT* __restrict__ out, int64_t ldo, int m, int n, int k, uint32_t idesc, int out_vec_ok,
-                         int use_tma_store, int raster, uint32_t* sched) {
+                         int use_tma_store, int raster, int chunk_kb, uint32_t* sched) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* staging = tiles + XSTAGES * XSTAGE_BYTES;
-  uint8_t* factors = staging + EPI_STAGING_BYTES;  // per stage: 512 bytes of A's, 1024 of B's
+  uint8_t* factors = staging + XSTAGING_BYTES;  // per stage: 512 bytes of A's, 1024 of B's
   ScaledBars* bars = reinterpret_cast<ScaledBars*>(factors + XSTAGES * XSF_BYTES);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -730,7 +739,7 @@ gemm_block_scaled_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid
     }
     mbar_init(&bars->tmem_full[0], 1);
     mbar_init(&bars->tmem_full[1], 1);
-    mbar_init(&bars->tmem_shared_free, 8);
+    mbar_init(&bars->tmem_shared_free, 16);
     for (int r = 0; r < RING; ++r) mbar_init(&bars->ring.full[r], 1);
     bars->abort_flag = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -747,145 +756,167 @@ gemm_block_scaled_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid
   tc_fence_after();
   const uint32_t tmem_base = bars->tmem_base;
 
-  if (warp == 0) {
-    // ---------------- TMA producer (one per CTA) ----------------
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      const int claim_kb = num_kb > 4 ? num_kb - 4 : 0;
-      uint32_t entry = 0;  // ring entries published (leader) or read (partner) so far
-      int64_t t = cluster_id;
-      while (ok && t < num_tiles) {
-        const TileCoord tc = tile_coord(t, tiles_m, tiles_n, raster);
-        const int row_a = tc.m * PBM + (int)rank * 128;
-        const int row_b = tc.n * PBN + (int)rank * 128;
-        int64_t next = t + num_clusters;
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (sched != nullptr && leader && kb == claim_kb) next = num_clusters + (int64_t)atomicAdd(sched, 1u);
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(XREGS_FEW));
+    if (warp == 0) {
+      // ---------------- TMA producer (one per CTA) ----------------
+      if (lane == 0) {
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        const int claim_kb = num_kb > 4 ? num_kb - 4 : 0;
+        uint32_t entry = 0;  // ring entries published (leader) or read (partner) so far
+        int64_t t = cluster_id;
+        while (ok && t < num_tiles) {
+          const TileCoord tc = tile_coord(t, tiles_m, tiles_n, raster);
+          const int row_a = tc.m * PBM + (int)rank * 128;
+          const int row_b = tc.n * PBN + (int)rank * 128;
+          int64_t next = t + num_clusters;
+          for (int kb = 0; kb < num_kb; ++kb) {
+            if (sched != nullptr && leader && kb == claim_kb) next = num_clusters + (int64_t)atomicAdd(sched, 1u);
+            if (!pair_wait(&bars->empty[stage], phase ^ 1u, bars, peer, 1u, 64u)) { ok = false; break; }
+            uint8_t* sa = tiles + stage * XSTAGE_BYTES;
+            const bool with_factors = (kb & 3) == 0;
+            if (leader) mbar_expect_tx(&bars->full[stage], 2 * (XSTAGE_BYTES + (with_factors ? XSF_A + XSF_B : 0)));
+            const uint32_t full_in_leader = mapa_u32(smem_u32(&bars->full[stage]), 0u);
+            if (with_factors) {
+              uint8_t* sf = factors + stage * XSF_BYTES;
+              tma_load_2d_pair_plain(sf, &tma_ea, row_a, kb >> 2, full_in_leader);
+              tma_load_2d_pair_plain(sf + XSF_A, &tma_eb, tc.n * PBN, kb >> 2, full_in_leader);
+            }
+            tma_load_2d_pair_plain(sa, &tma_a, a_mn ? row_a : kb * BK, a_mn ? kb * BK : row_a, full_in_leader);
+            tma_load_2d_pair_plain(sa + PA_BYTES, &tma_b, b_mn ? row_b : kb * BK, b_mn ? kb * BK : row_b,
+                                   full_in_leader);
+            if (++stage == XSTAGES) { stage = 0; phase ^= 1u; }
+          }
+          if (!ok) break;
+          if (sched != nullptr) {
+            if (leader) {
+              const uint32_t e = entry & (RING - 1);
+              const int32_t v = next < num_tiles ? (int32_t)next : -1;
+              bars->ring.tile[e] = v;
+              mbar_arrive(&bars->ring.full[e]);
+              st_cluster_u32(mapa_u32(smem_u32(&bars->ring.tile[e]), 1u), (uint32_t)v);
+              mbar_arrive_release_cluster(mapa_u32(smem_u32(&bars->ring.full[e]), 1u));
+            } else {
+              const int32_t v = pair_ring_read(bars, entry, peer, 64u, 32u);
+              if (v == -2) { ok = false; break; }
+              next = v < 0 ? num_tiles : (int64_t)v;
+            }
+            ++entry;
+          }
+          t = next;
+        }
+        // tail: every release the leader multicast to this CTA's empty barriers has landed
+        for (int s = 0; ok && s < XSTAGES; ++s) {
           if (!pair_wait(&bars->empty[stage], phase ^ 1u, bars, peer, 1u, 64u)) { ok = false; break; }
-          uint8_t* sa = tiles + stage * XSTAGE_BYTES;
-          const bool with_factors = (kb & 3) == 0;
-          if (leader) mbar_expect_tx(&bars->full[stage], 2 * (XSTAGE_BYTES + (with_factors ? XSF_A + XSF_B : 0)));
-          const uint32_t full_in_leader = mapa_u32(smem_u32(&bars->full[stage]), 0u);
-          if (with_factors) {
-            uint8_t* sf = factors + stage * XSF_BYTES;
-            tma_load_2d_pair_plain(sf, &tma_ea, row_a, kb >> 2, full_in_leader);
-            tma_load_2d_pair_plain(sf + XSF_A, &tma_eb, tc.n * PBN, kb >> 2, full_in_leader);
-          }
-          tma_load_2d_pair_plain(sa, &tma_a, a_mn ? row_a : kb * BK, a_mn ? kb * BK : row_a, full_in_leader);
-          tma_load_2d_pair_plain(sa + PA_BYTES, &tma_b, b_mn ? row_b : kb * BK, b_mn ? kb * BK : row_b,
-                                 full_in_leader);
           if (++stage == XSTAGES) { stage = 0; phase ^= 1u; }
         }
-        if (!ok) break;
-        if (sched != nullptr) {
-          if (leader) {
-            const uint32_t e = entry & (RING - 1);
-            const int32_t v = next < num_tiles ? (int32_t)next : -1;
-            bars->ring.tile[e] = v;
-            mbar_arrive(&bars->ring.full[e]);
-            st_cluster_u32(mapa_u32(smem_u32(&bars->ring.tile[e]), 1u), (uint32_t)v);
-            mbar_arrive_release_cluster(mapa_u32(smem_u32(&bars->ring.full[e]), 1u));
-          } else {
-            const int32_t v = pair_ring_read(bars, entry, peer, 64u, 32u);
-            if (v == -2) { ok = false; break; }
-            next = v < 0 ? num_tiles : (int64_t)v;
-          }
-          ++entry;
+        if (!ok) {
+          const long long t0 = clock64();
+          while (clock64() - t0 < 2000000LL) {}
         }
-        t = next;
       }
-      // tail: every release the leader multicast to this CTA's empty barriers has landed
-      for (int s = 0; ok && s < XSTAGES; ++s) {
-        if (!pair_wait(&bars->empty[stage], phase ^ 1u, bars, peer, 1u, 64u)) { ok = false; break; }
-        if (++stage == XSTAGES) { stage = 0; phase ^= 1u; }
-      }
-      if (!ok) {
-        const long long t0 = clock64();
-        while (clock64() - t0 < 2000000LL) {}
-      }
-    }
-  } else if (warp == 1) {
-    // ---------------- MMA issuer (leader CTA only) ----------------
-    if (leader && lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      int set = 0;
-      bool ok = true;
-      uint32_t local = 0;
-      int64_t t = cluster_id;
-      for (; ok && t < num_tiles; ++local) {
-        const uint32_t acc = local & 1u;
-        const uint32_t tmem_d = tmem_base + acc * (uint32_t)XACC_STEP;
-        // the columns that this accumulator shares with the previous tile's have been read
-        if (local > 0 && !pair_wait(&bars->tmem_shared_free, (local - 1) & 1u, bars, peer, 2u)) { ok = false; break; }
-        uint32_t sf = 0;
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!pair_wait(&bars->full[stage], phase, bars, peer, 4u)) { ok = false; break; }
-          tc_fence_after();
-          if ((kb & 3) == 0) {
-            const uint32_t f = smem_u32(factors + stage * XSF_BYTES);
-            sf = tmem_base + XSF_COL + set * XSF_SET;
-            tc_copy_factors_pair(sf, f);
-            tc_copy_factors_pair(sf + 4, f + XSF_A);
-            tc_copy_factors_pair(sf + 8, f + XSF_A + 512);
-            if (++set == XSF_SETS) set = 0;
-          }
-          const uint32_t a_addr = smem_u32(tiles + stage * XSTAGE_BYTES);
-          const uint32_t id = idesc | ((uint32_t)(kb & 3) << 4) | ((uint32_t)(kb & 3) << 29);
-          const uint64_t da = a_mn ? make_smem_desc_mn(a_addr, PA_BYTES) : make_smem_desc(a_addr);
-          const uint64_t db = b_mn ? make_smem_desc_mn(a_addr + PA_BYTES, PB_BYTES) : make_smem_desc(a_addr + PA_BYTES);
+    } else if (warp == 1) {
+      // ---------------- MMA issuer (leader CTA only) ----------------
+      if (leader && lane == 0) {
+        int stage = 0;
+        uint32_t phase = 0;
+        int set = 0;
+        bool ok = true;
+        uint32_t local = 0, chunk = 0;
+        int64_t t = cluster_id;
+        for (; ok && t < num_tiles; ++local) {
+          for (int kb0 = 0; ok && kb0 < num_kb; kb0 += chunk_kb, ++chunk) {
+            const uint32_t acc = chunk & 1u;
+            const uint32_t tmem_d = tmem_base + acc * (uint32_t)XACC_STEP;
+            // the columns that this accumulator shares with the previous chunk's have been read, and all of the one before
+            if (chunk > 0 && !pair_wait(&bars->tmem_shared_free, (chunk - 1) & 1u, bars, peer, 2u)) { ok = false; break; }
+            const int blocks = min(chunk_kb, num_kb - kb0);  // kb0 is a multiple of four: groups of factors lie within a chunk
+            uint32_t sf = 0;
+            for (int kb = 0; kb < blocks; ++kb) {
+              if (!pair_wait(&bars->full[stage], phase, bars, peer, 4u)) { ok = false; break; }
+              tc_fence_after();
+              if ((kb & 3) == 0) {
+                const uint32_t f = smem_u32(factors + stage * XSF_BYTES);
+                sf = tmem_base + XSF_COL + set * XSF_SET;
+                tc_copy_factors_pair(sf, f);
+                tc_copy_factors_pair(sf + 4, f + XSF_A);
+                tc_copy_factors_pair(sf + 8, f + XSF_A + 512);
+                if (++set == XSF_SETS) set = 0;
+              }
+              const uint32_t a_addr = smem_u32(tiles + stage * XSTAGE_BYTES);
+              const uint32_t id = idesc | ((uint32_t)(kb & 3) << 4) | ((uint32_t)(kb & 3) << 29);
+              const uint64_t da = a_mn ? make_smem_desc_mn(a_addr, PA_BYTES) : make_smem_desc(a_addr);
+              const uint64_t db = b_mn ? make_smem_desc_mn(a_addr + PA_BYTES, PB_BYTES) : make_smem_desc(a_addr + PA_BYTES);
 #pragma unroll
-          for (int kk = 0; kk < BK / UMMA_K; ++kk)
-            tc_mma_mx_pair(tmem_d, da + (uint64_t)kk * step_a, db + (uint64_t)kk * step_b, id, sf, sf + 4,
-                           (kb | kk) != 0 ? 1u : 0u);
-          tc_commit_pair(&bars->empty[stage]);
-          if (++stage == XSTAGES) { stage = 0; phase ^= 1u; }
-        }
-        if (!ok) break;
-        tc_commit_pair(&bars->tmem_full[acc]);
-        if (sched != nullptr) {
-          const int32_t v = pair_ring_read(bars, local, peer, 16u, 0u);
-          if (v == -2) { ok = false; break; }
-          t = v < 0 ? num_tiles : (int64_t)v;
-        } else {
-          t += num_clusters;
+              for (int kk = 0; kk < BK / UMMA_K; ++kk)
+                tc_mma_mx_pair(tmem_d, da + (uint64_t)kk * step_a, db + (uint64_t)kk * step_b, id, sf, sf + 4,
+                               (kb | kk) != 0 ? 1u : 0u);
+              tc_commit_pair(&bars->empty[stage]);
+              if (++stage == XSTAGES) { stage = 0; phase ^= 1u; }
+            }
+            if (ok) tc_commit_pair(&bars->tmem_full[acc]);
+          }
+          if (!ok) break;
+          if (sched != nullptr) {
+            const int32_t v = pair_ring_read(bars, local, peer, 16u, 0u);
+            if (v == -2) { ok = false; break; }
+            t = v < 0 ? num_tiles : (int64_t)v;
+          } else {
+            t += num_clusters;
+          }
         }
       }
     }
   } else {
-    // ---------------- epilogue (warps 2..5 of both CTAs) ----------------
-    const int quarter = warp & 3;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(XREGS_MANY));
+    // ---------------- epilogue (warps 4..11 of both CTAs) ----------------
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
     const EpilogueArgs<OutT> ea{bias, out, ldo, m, n, out_vec_ok, use_tma_store, &tma_out,
-                                staging + (warp - 2) * 2 * EPI_BOX_BYTES, 1.0f, 1, nullptr};
+                                staging + (warp - 4) * EPI_BOX_BYTES, 1.0f, 1, nullptr};
     const uint32_t free_in_leader = mapa_u32(smem_u32(&bars->tmem_shared_free), 0u);
-    uint32_t boxes = 0, local = 0;
+    // The shared columns are the last 64 of accumulator 0, read by half 1, and the first of accumulator 1, read by half 0:
+    // half 1 takes its two pieces of 64 columns in the other order.
+    const int piece[2] = {half * 64, 64 - half * 64};
+    uint32_t boxes = 0, local = 0, chunk = 0;
     int64_t t = cluster_id;
     for (; t < num_tiles; ++local) {
       const TileCoord tc = tile_coord(t, tiles_m, tiles_n, raster);
-      const uint32_t acc = local & 1u;
+      float sum[128];
       int got = 1;
-      if (lane == 0) got = pair_wait(&bars->tmem_full[acc], (local >> 1) & 1u, bars, peer, 8u, WAIT_BY_HINT | 1000u) ? 1 : 0;
-      got = __shfl_sync(0xFFFFFFFFu, got, 0);
-      if (got == 0) break;
-      tc_fence_after();
-      const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * (uint32_t)XACC_STEP;
-      const int row0 = tc.m * PBM + (int)rank * 128 + quarter * 32;
-#pragma unroll 1
-      for (int b = 0; b < 4; ++b) {
-        const int part = acc == 0 ? (b + 3) & 3 : b;  // the shared columns first: the last 64 of accumulator 0, the first of 1
-        uint32_t r[2][32];
-        tc_ld_32x32b_x32(taddr + (uint32_t)(part * 64), r[0]);
-        tc_ld_32x32b_x32(taddr + (uint32_t)(part * 64 + 32), r[1]);
-        tc_wait_ld();
-        if (b == 0) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(free_in_leader);
+      for (int kb = 0; kb < num_kb; kb += chunk_kb, ++chunk) {
+        const uint32_t acc = chunk & 1u;
+        if (lane == 0) got = pair_wait(&bars->tmem_full[acc], (chunk >> 1) & 1u, bars, peer, 8u, WAIT_BY_HINT | 1000u) ? 1 : 0;
+        got = __shfl_sync(0xFFFFFFFFu, got, 0);
+        if (got == 0) break;
+        tc_fence_after();
+        const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * (uint32_t)XACC_STEP + (uint32_t)(half * 128);
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          uint32_t r[2][32];
+          tc_ld_32x32b_x32(taddr + (uint32_t)piece[p], r[0]);
+          tc_ld_32x32b_x32(taddr + (uint32_t)(piece[p] + 32), r[1]);
+          tc_wait_ld();
+          if (p == 0) {  // also says that this warp has read all of the previous chunk's accumulator
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(free_in_leader);
+          }
+          if (kb == 0) {
+#pragma unroll
+            for (int i = 0; i < 64; ++i) sum[p * 64 + i] = __uint_as_float(r[i >> 5][i & 31]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 64; ++i) sum[p * 64 + i] += __uint_as_float(r[i >> 5][i & 31]);
+          }
         }
-        store_columns<OutT>(ea, r, row0, tc.n * PBN + part * 64, boxes);
       }
+      if (got == 0) break;
+      const int row0 = tc.m * PBM + (int)rank * 128 + quarter * 32;
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+        store_columns<OutT>(ea, sum + p * 64, row0, tc.n * PBN + half * 128 + piece[p], boxes);
       if (sched != nullptr) {
         int v = 0;
         if (lane == 0) v = pair_ring_read(bars, local, peer, 32u, 64u);
@@ -992,6 +1023,10 @@ static int launch_block_scaled(const CUtensorMap& ma, const CUtensorMap& mb, con
   const cudaError_t attr_err = setup.run(
       [&](int* clusters_out) {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, XSMEM_BYTES);
+        cudaFuncAttributes fa;
+        if (e == cudaSuccess) e = cudaFuncGetAttributes(&fa, kernel);
+        // as in launch_block_pair: the registers that the first group hands over have to be there
+        if (e == cudaSuccess && fa.numRegs * XTHREADS < 128 * XREGS_FEW + 256 * XREGS_MANY) e = cudaErrorInvalidConfiguration;
         if (e == cudaSuccess) {
           cfg.gridDim = dim3(2 * (sm_count() / 2));
           e = cudaOccupancyMaxActiveClusters(clusters_out, kernel, &cfg);
@@ -1011,9 +1046,11 @@ static int launch_block_scaled(const CUtensorMap& ma, const CUtensorMap& mb, con
     const cudaError_t e = cudaMemsetAsync(sched, 0, sizeof(uint32_t), st);
     if (e != cudaSuccess) return record_cuda_error(e);
   }
+  const int num_kb = (k + BK - 1) / BK, most = sizeof(OutT) == 4 ? XCHUNK_32 : XCHUNK_16;
+  const int chunks = (num_kb + most - 1) / most, chunk_kb = ((num_kb + chunks - 1) / chunks + 3) / 4 * 4;  // <= most
   return record_cuda_error(cudaLaunchKernelEx(&cfg, kernel, ma, mb, mea, meb, mo, static_cast<const OutT*>(bias),
                                               static_cast<OutT*>(out), ldo, m, n, k, idesc, vec_ok, use_tma,
-                                              choose_raster(m, n, k, PBM, PBN) | layouts, sched));
+                                              choose_raster(m, n, k, PBM, PBN) | layouts, chunk_kb, sched));
 }
 
 template <typename OutT, int T>
