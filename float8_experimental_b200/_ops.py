@@ -382,6 +382,15 @@ def _check_factors(name: str, s, rows: int, k: int, block: int) -> None:
         raise RuntimeError(f"blockwise_mm: {name} must be float32 {want}, got {s.dtype} {tuple(s.shape)}")
 
 
+def _dense_bias(bias: Optional[torch.Tensor], n: int, dtype: torch.dtype) -> Optional[torch.Tensor]:
+    """The bias as the products read it: n neighbouring elements of the result's type."""
+    if bias is None:
+        return None
+    if bias.shape != (n,):
+        raise RuntimeError(f"blockwise_mm: the bias must have {n} elements, got {tuple(bias.shape)}")
+    return bias.to(dtype).contiguous()
+
+
 def _blockwise_mm_cuda(a, b_t, scale_a, scale_b, a_block_rows: int, b_block_rows: int, exp_a, exp_b, bias, out_dtype):
     _one_device("blockwise_mm", a, b_t, scale_a, scale_b, exp_a, exp_b, bias)
     m, k = a.shape
@@ -393,10 +402,7 @@ def _blockwise_mm_cuda(a, b_t, scale_a, scale_b, a_block_rows: int, b_block_rows
     for name, e, rows in (("exp_a", exp_a, m), ("exp_b", exp_b, n)):
         if e is not None and (e.dtype != torch.uint8 or not e.is_contiguous() or e.numel() != _exponent_bytes(rows, k)):
             raise RuntimeError(f"blockwise_mm: {name} must be the {_exponent_bytes(rows, k)} exponent bytes of its cast")
-    if bias is not None and tuple(bias.shape) != (n,):
-        raise RuntimeError(f"blockwise_mm: the bias must have {n} elements, got {tuple(bias.shape)}")
-    if bias is not None:
-        bias = bias.to(out_dtype).contiguous()
+    bias = _dense_bias(bias, n, out_dtype)
     out = torch.empty((m, n), dtype=out_dtype, device=a.device)
     if m == 0 or n == 0:
         return out
@@ -420,10 +426,7 @@ def linear_blockwise(x, weight, weight_scale, bias):
         raise RuntimeError(f"blockwise_mm: scale_b must be float32 {(_blocks(n), _blocks(k))}, got {weight_scale.dtype} "
                            f"{tuple(weight_scale.shape)}")
     _one_device("blockwise_mm", x, weight, weight_scale, bias)
-    if bias is not None:
-        if tuple(bias.shape) != (n,):
-            raise RuntimeError(f"blockwise_mm: the bias must have {n} elements, got {tuple(bias.shape)}")
-        bias = bias.to(x.dtype).contiguous()
+    bias = _dense_bias(bias, n, x.dtype)
     out = torch.empty((m, n), dtype=x.dtype, device=x.device)
     if m == 0 or n == 0:
         return out

@@ -19,8 +19,8 @@ from torch.autograd.function import once_differentiable
 
 from . import _native as N
 from ._ops import (
-    _as_matrix, _blocks, _blockwise_mm_cuda, _cast_blockwise_some, _cast_blockwise_square_cuda, eager_cuda,
-    linear_blockwise, _one_device, ops, _uncast_blockwise_cuda,
+    _as_matrix, _blocks, _blockwise_mm_cuda, _cast_blockwise_some, _cast_blockwise_square_cuda, _dense_bias,
+    eager_cuda, linear_blockwise, _one_device, ops, _uncast_blockwise_cuda,
 )
 from .float8_utils import _kind, e4m3_dtype, e5m2_dtype
 
@@ -201,6 +201,7 @@ class _float8_linear_blockwise(torch.autograd.Function):
         x2, _, _, ldx = _as_matrix(x2)
         weight, _, _, ldw = _as_matrix(weight)
         _one_device("blockwise_mm", x2, weight, bias)
+        bias = _dense_bias(bias, n, x.dtype)
         xr, xc, w = N.BlockForm(m, k, "row"), N.BlockForm(m, k, "col"), N.BlockForm(n, k, "square")
         kept = torch.empty(w.nbytes + (xc.nbytes if need_dw else 0), dtype=torch.uint8, device=x.device)
         passing = torch.empty(xr.nbytes + N.GEMM_WORKSPACE_BYTES, dtype=torch.uint8, device=x.device)
@@ -211,8 +212,6 @@ class _float8_linear_blockwise(torch.autograd.Function):
         N.block_cast_into(x2, ldx, xr, xc if need_dw else None)
         N.block_cast_into(weight, ldw, w, None)
         y = torch.empty((m, n), dtype=x.dtype, device=x.device)
-        if bias is not None and bias.dtype != x.dtype:
-            bias = bias.to(x.dtype)
         N.block_gemm_into(xr.operand(), w.operand(), bias, y, m, n, k, passing.data_ptr() + xr.nbytes)
         ctx.save_for_backward(kept)
         ctx.forms = (w, xc if need_dw else None)
