@@ -224,9 +224,11 @@ gemm_block_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_c
       if constexpr (PER_COL) load_cols(0); else sb = cols_in ? __ldg(pb) : 0.f;
       for (int kb = 0; kb < num_kb; ++kb, ++g) {
         const uint32_t buf = g & 1u;
-        const float* cs = bars->col_scale[warp - 4][kb & 1];
+        // Alternating over all blocks, not within the tile: before a buffer is written again every lane has passed the
+        // barriers of the block between, behind its own reads.
+        const float* cs = bars->col_scale[warp - 4][buf];
         if constexpr (PER_COL) {
-          float* w = bars->col_scale[warp - 4][kb & 1];
+          float* w = bars->col_scale[warp - 4][buf];
 #pragma unroll
           for (int j = 0; j < 4; ++j) w[lane + 32 * j] = sc[j];
           __syncwarp();
