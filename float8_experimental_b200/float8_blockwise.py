@@ -30,6 +30,16 @@ BLOCK = 128
 _BLOCKS = ((1, BLOCK), (BLOCK, 1), (BLOCK, BLOCK))
 
 
+class _Exponents:
+    """The exponent bytes of a cast's factors: of the matrix, and of its transpose, as a product's operand.  Shared by the
+    tensors that hold the same factors."""
+
+    __slots__ = ("matrix", "transpose")
+
+    def __init__(self, matrix: Optional[torch.Tensor], transpose: Optional[torch.Tensor]):
+        self.matrix, self.transpose = matrix, transpose
+
+
 class Float8BlockTensor:
     """A matrix held as fp8 bytes and one factor per block: `data[i, j] * scale_inv[i // block[0], j // block[1]]`.
 
@@ -39,10 +49,11 @@ class Float8BlockTensor:
     orig_dtype the dtype `to_original_precision` returns by default
 
     A cast also keeps its power-of-two factors as the exponent bytes that the tensor cores read (of the matrix, and
-    of its transpose, as a product's operand).  They go with `scale_inv`: to give a matrix other factors, make a new
-    Float8BlockTensor of its `data`."""
+    of its transpose, as a product's operand).  Whoever asks for `scale_inv` may write to it, in ways that leave no
+    trace (a collective, `.data`, another library's kernel), so asking for it drops the bytes, of transposes too: products
+    of more than 128 rows then take the factors themselves, in a slower kernel.  `scale_inv` may be assigned."""
 
-    __slots__ = ("data", "scale_inv", "block", "orig_dtype", "_exps", "_exps_t", "_version")
+    __slots__ = ("data", "_scale", "block", "orig_dtype", "_exps", "_transposed")
 
     def __init__(self, data: torch.Tensor, scale_inv: torch.Tensor, block: Tuple[int, int],
                  orig_dtype: torch.dtype = torch.bfloat16):
@@ -51,33 +62,40 @@ class Float8BlockTensor:
             raise ValueError(f"Float8BlockTensor: block must be one of {_BLOCKS}, got {block}")
         if data.dim() != 2 or data.dtype not in (e4m3_dtype, e5m2_dtype):
             raise ValueError(f"Float8BlockTensor: data must be a float8 matrix, got {data.dtype} {tuple(data.shape)}")
-        want = tuple(_blocks(size) if b == BLOCK else size for size, b in zip(data.shape, block))
-        if scale_inv.dtype != torch.float32 or tuple(scale_inv.shape) != want:
-            raise ValueError(
-                f"Float8BlockTensor: scale_inv must be float32 {want} for blocks of {block}, got "
-                f"{scale_inv.dtype} {tuple(scale_inv.shape)}"
-            )
-        if scale_inv.device != data.device:
-            raise ValueError(f"Float8BlockTensor: data on {data.device}, scale_inv on {scale_inv.device}")
-        self.data, self.scale_inv, self.block, self.orig_dtype = data, scale_inv, block, orig_dtype
-        self._exps = self._exps_t = self._version = None
+        self.data, self.block, self.orig_dtype = data, block, orig_dtype
+        self.scale_inv = scale_inv
 
     @classmethod
     def _of_cast(cls, data, scale_inv, block, orig_dtype, exps, exps_t) -> "Float8BlockTensor":
         """What a cast made: nothing to check, and the exponent bytes beside it."""
         out = object.__new__(cls)
-        out.data, out.scale_inv, out.block, out.orig_dtype = data, scale_inv, block, orig_dtype
-        if scale_inv.is_inference():  # does not tell when it is written to
-            exps = exps_t = None
-        out._exps, out._exps_t = exps, exps_t
-        out._version = None if exps is None and exps_t is None else scale_inv._version
+        out.data, out._scale, out.block, out.orig_dtype = data, scale_inv, block, orig_dtype
+        out._exps, out._transposed = _Exponents(exps, exps_t), False
         return out
 
+    @property
+    def scale_inv(self) -> torch.Tensor:
+        if self._exps is not None:
+            self._exps.matrix = self._exps.transpose = None
+        return self._scale
+
+    @scale_inv.setter
+    def scale_inv(self, scale_inv: torch.Tensor) -> None:
+        want = tuple(_blocks(size) if b == BLOCK else size for size, b in zip(self.data.shape, self.block))
+        if scale_inv.dtype != torch.float32 or tuple(scale_inv.shape) != want:
+            raise ValueError(
+                f"Float8BlockTensor: scale_inv must be float32 {want} for blocks of {self.block}, got "
+                f"{scale_inv.dtype} {tuple(scale_inv.shape)}"
+            )
+        if scale_inv.device != self.data.device:
+            raise ValueError(f"Float8BlockTensor: data on {self.data.device}, scale_inv on {scale_inv.device}")
+        self._scale, self._exps, self._transposed = scale_inv, None, False
+
     def _exponents(self, transposed: bool = False) -> Optional[torch.Tensor]:
-        """The exponent bytes, unless the factors were written to since the cast."""
-        if self._version is None or self._version != self.scale_inv._version:
+        """The exponent bytes, unless the factors may have been written to since the cast."""
+        if self._exps is None:
             return None
-        return self._exps_t if transposed else self._exps
+        return self._exps.transpose if transposed != self._transposed else self._exps.matrix
 
     @property
     def shape(self) -> torch.Size:
@@ -90,12 +108,12 @@ class Float8BlockTensor:
     def t(self) -> "Float8BlockTensor":
         """The transposed matrix: the same bytes and factors, nothing copied."""
         out = object.__new__(Float8BlockTensor)
-        out.data, out.scale_inv, out.block, out.orig_dtype = self.data.t(), self.scale_inv.t(), self.block[::-1], self.orig_dtype
-        out._exps, out._exps_t, out._version = self._exps_t, self._exps, self._version
+        out.data, out._scale, out.block, out.orig_dtype = self.data.t(), self._scale.t(), self.block[::-1], self.orig_dtype
+        out._exps, out._transposed = self._exps, not self._transposed
         return out
 
     def to_original_precision(self, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-        args = (self.data, self.scale_inv, *self.block, dtype or self.orig_dtype)
+        args = (self.data, self._scale, *self.block, dtype or self.orig_dtype)
         return _uncast_blockwise_cuda(*args) if eager_cuda(self.data) else ops.uncast_blockwise(*args)
 
     def __repr__(self):
@@ -167,7 +185,7 @@ def blockwise_mm(a: Float8BlockTensor, b: Float8BlockTensor, out_dtype: torch.dt
     if a.shape[1] != b.shape[0]:
         raise ValueError(f"blockwise_mm: inner dimensions differ ({a.shape[1]} vs {b.shape[0]})")
     N.hp_code(out_dtype)
-    return _mm(a.data, b.data.t(), a.scale_inv, b.scale_inv.t(), a.block[0], b.block[1], a._exponents(),
+    return _mm(a.data, b.data.t(), a._scale, b._scale.t(), a.block[0], b.block[1], a._exponents(),
                b._exponents(transposed=True), None if bias is None else bias.detach(), out_dtype)
 
 
