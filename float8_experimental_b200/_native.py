@@ -668,6 +668,18 @@ class BlockForm:
         self.exps_t = None if self.exps_t is None else self.exps_t + base
         return self
 
+    def tensors(self, buf: torch.Tensor, start: int):
+        """The form as tensors, views of the buffer `buf` (uint8) in which it lies from byte `start` on: (bytes, factors,
+        exponent bytes as an operand by columns or transposed, otherwise by rows)."""
+        kb, rb = -(-self.cols // 128), -(-self.rows // 128)
+        shape = {"row": (kb, self.rows), "col": (rb, self.cols), "square": (rb, kb)}[self.by]
+        exps, nbytes = (self.exps, -(-self.rows // 256) * 1024 * -(-self.cols // 512)) if self.by == "row" else \
+            (self.exps_t, -(-self.cols // 256) * 1024 * -(-self.rows // 512))
+        scale_at, exps_at = start + self.scale - self.data, start + exps - self.data
+        data = buf[start:start + self.rows * self.pitch].view(self.rows, self.pitch)[:, : self.cols].view(torch.float8_e4m3fn)
+        scale = buf[scale_at:scale_at + 4 * shape[0] * shape[1]].view(torch.float32).view(shape)
+        return data, scale.t() if self.by == "row" else scale, buf[exps_at:exps_at + nbytes]
+
     def operand(self, transposed: bool = False):
         """(address, MN-major, pitch, factors, row stride, k-block stride, rows per factor, exponents) for the GEMM."""
         if self.by == "square":

@@ -557,11 +557,23 @@ _lib.impl("scaled_mm", _scaled_mm_cuda, "CUDA")
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
 
 
+_dispatch_modes = torch._C._len_torch_dispatch_stack
+_pre_dispatch_modes = torch._ops._len_torch_dispatch_stack_pre_dispatch
+_jit_tracing = torch._C._is_tracing
+_functorch_level = torch._C._functorch.peek_interpreter_stack
+
+
+def nothing_watches() -> bool:
+    """Whether no trace (`make_fx`, `torch.jit.trace`), dispatch mode (selective checkpointing, counters, fake tensors) or
+    functorch transform would have to see the ops that run here.  All of these show plain tensors."""
+    return not _dispatch_modes() and not _jit_tracing() and _functorch_level() is None and not _pre_dispatch_modes()
+
+
 def eager_cuda(t: torch.Tensor) -> bool:
-    """Whether an op on `t` would come straight to its CUDA implementation here: a plain CUDA tensor, nothing tracing.
+    """Whether an op on `t` would come straight to its CUDA implementation here: a plain CUDA tensor, nothing watching.
     Callers that run without autograd (inside an autograd function, or with nothing to differentiate) then call
     the implementation themselves: a trip through the dispatcher costs more host time than a small launch."""
-    return type(t) in _PLAIN and t.is_cuda and not torch.compiler.is_compiling()
+    return not torch.compiler.is_compiling() and type(t) in _PLAIN and t.is_cuda and nothing_watches()
 
 
 # ---------------------------------------------------------------------------

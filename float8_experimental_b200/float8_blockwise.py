@@ -287,13 +287,18 @@ class _float8_linear_blockwise(torch.autograd.Function):
         need_dx, need_dw, need_db = ctx.needs_input_grad[:3]
         go2 = go.reshape(-1, go.shape[-1])
         dx = dw = db = None
-        if ctx.forms is not None:
+        if ctx.forms is not None and eager_cuda(go):
             if need_dx or need_dw:
                 dx, dw = _float8_linear_blockwise._backward_eager(ctx, go, go2, need_dx, need_dw)
             if need_db:
                 db = go2.sum(0, dtype=torch.float32).to(ctx.dtypes[1])
             return dx, dw, db, None
-        x8c, sxc, exc, w8, sw, ewt = ctx.saved_tensors
+        if ctx.forms is not None:  # an eager forward whose backward is traced or watched
+            (kept,), (w, xc) = ctx.saved_tensors, ctx.forms
+            x8c, sxc, exc = xc.tensors(kept, w.nbytes) if xc is not None else (None, None, None)
+            w8, sw, ewt = w.tensors(kept, 0)
+        else:
+            x8c, sxc, exc, w8, sw, ewt = ctx.saved_tensors
         if need_dx or need_dw:
             (g8, sg, eg), (g8c, sgc, egc) = _cast(go2, N.E4M3, need_dx, need_dw)
         if need_dx:  # dX = dY @ W: the weight's bytes and factors read transposed
