@@ -696,7 +696,10 @@ def _cast_blockwise_square_fake(x, fp8_kind):
 
 @torch.library.register_fake("f8b200::uncast_blockwise")
 def _uncast_blockwise_fake(q, scale_inv, block_rows, block_cols, dtype):
-    return q.new_empty(q.shape, dtype=dtype)
+    rows, cols = q.shape
+    if rows != 1 and cols != 1 and q.stride(0) == 1:  # a transposed matrix stays one
+        return q.new_empty((cols, rows), dtype=dtype).t()
+    return q.new_empty((rows, cols), dtype=dtype)
 
 
 @torch.library.register_fake("f8b200::blockwise_mm")
@@ -706,8 +709,8 @@ def _blockwise_mm_fake(a, b_t, scale_a, scale_b, a_block_rows, b_block_rows, exp
 
 @torch.library.register_fake("f8b200::layer_norm")
 def _layer_norm_fake(x, weight, bias, eps, save_stats):
-    stats = x.new_empty((2, x.numel() // max(x.shape[-1], 1) if save_stats else 0), dtype=torch.float32)
-    return x.new_empty(x.shape), stats[0], stats[1]
+    rows = x.numel() // x.shape[-1] if save_stats else 0
+    return x.new_empty(x.shape), x.new_empty((rows,), dtype=torch.float32), x.new_empty((rows,), dtype=torch.float32)
 
 
 @torch.library.register_fake("f8b200::layer_norm_bwd")
