@@ -50,10 +50,10 @@ def _sharded_groups(t: DTensor):
     """The process groups whose ranks hold different parts of `t`."""
     groups = []
     for dim, placement in enumerate(t.placements):
-        if placement.is_shard():
-            groups.append(t.device_mesh.get_group(dim))
-        elif placement.is_partial():
+        if placement.is_partial():
             raise NotImplementedError("gradient norm of a Partial DTensor")
+        if not placement.is_replicate():  # Shard, or FSDP2's strided shard on top of a tensor-parallel one: no Shard by its type
+            groups.append(t.device_mesh.get_group(dim))
     return tuple(groups)
 
 
