@@ -66,8 +66,11 @@ EXPORTS = (
 )
 
 
+ERR_BAD_ARG = -1
+
+
 class F8B200Error(RuntimeError):
-    pass
+    status = 0  # of the entry point that returned it
 
 
 def lib_path() -> str:
@@ -151,7 +154,9 @@ def _check(status: int, what: str) -> None:
     lib = load()
     msg = lib.f8b200_status_string(status).decode()
     detail = lib.f8b200_last_cuda_error().decode() if status == -4 else ""
-    raise F8B200Error(f"{what}: {msg}" + (f" [{detail}]" if detail else ""))
+    error = F8B200Error(f"{what}: {msg}" + (f" [{detail}]" if detail else ""))
+    error.status = status
+    raise error
 
 
 def hp_code(dtype: torch.dtype) -> int:
@@ -808,8 +813,14 @@ def multi_clip(xs: TensorArrays, total_norm: torch.Tensor, max_norm: float) -> N
     n = xs.n
     _require_cuda(total_norm)
     with _Launch("multi_clip", total_norm.device, -(-n // MULTI_TENSORS_PER_LAUNCH)):
-        _check(load().f8b200_multi_clip(xs.ptrs, xs.numels, xs.codes, n, total_norm.data_ptr(), float(max_norm),
-                                        _stream(total_norm)), "f8b200_multi_clip")
+        try:
+            _check(load().f8b200_multi_clip(xs.ptrs, xs.numels, xs.codes, n, total_norm.data_ptr(), float(max_norm),
+                                            _stream(total_norm)), "f8b200_multi_clip")
+        except F8B200Error as e:
+            if e.status != ERR_BAD_ARG:
+                raise
+            # the only bad argument that tensors can be
+            raise F8B200Error("f8b200_multi_clip: tensors that overlap in memory cannot be scaled together") from None
 
 
 def check_device_error() -> None:

@@ -9,6 +9,9 @@
 // Memory bounds it: the norm reads every gradient once, the scaling reads and writes it once more and is skipped
 // on the device when the factor is 1.  The scaling walks the chunks backwards: the ones the norm read
 // last are still in L2.
+#include <algorithm>
+#include <new>
+
 #include "common.cuh"
 
 namespace f8b200 {
@@ -247,6 +250,37 @@ int check_list(const void* const* ptrs, const int64_t* numels, const int* hp_dty
   return F8B200_OK;
 }
 
+// Whether two of the tensors have bytes in common: they would be scaled twice, by CTAs that do not wait for each other.
+// Tensors that lie in the order of their addresses, as the gradients of one buffer do, need no sorting.
+int check_apart(void* const* ptrs, const int64_t* numels, const int* hp_dtypes, int n) {
+  struct Span {
+    uintptr_t begin, end;
+  };
+  auto span = [&](int i) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(ptrs[i]);
+    return Span{p, p + (uintptr_t)numels[i] * (uintptr_t)hp_size_of(hp_dtypes[i])};
+  };
+  uintptr_t end = 0;
+  bool ascending = true;
+  for (int i = 0; i < n && ascending; ++i) {
+    if (numels[i] == 0) continue;
+    const Span s = span(i);
+    ascending = s.begin >= end;
+    end = s.end;
+  }
+  if (ascending) return F8B200_OK;
+  Span* spans = new (std::nothrow) Span[n];
+  if (spans == nullptr) return F8B200_ERR_UNSUPPORTED;
+  int used = 0;
+  for (int i = 0; i < n; ++i)
+    if (numels[i] != 0) spans[used++] = span(i);
+  std::sort(spans, spans + used, [](const Span& a, const Span& b) { return a.begin < b.begin; });
+  bool apart = true;
+  for (int i = 1; i < used; ++i) apart = apart && spans[i].begin >= spans[i - 1].end;
+  delete[] spans;
+  return apart ? F8B200_OK : F8B200_ERR_BAD_ARG;
+}
+
 // Cuts the tensors into lists of kTensors and calls fn(list, chunks of the list, chunks before it).
 template <typename Fn>
 int for_each_list(const void* const* ptrs, const int64_t* numels, const int* hp_dtypes, int n, Fn&& fn) {
@@ -316,6 +350,7 @@ extern "C" int f8b200_multi_clip(void* const* ptrs, const int64_t* numels, const
                                  float max_norm, void* stream) {
   if (total_norm == nullptr) return F8B200_ERR_BAD_ARG;
   int rc = check_list(ptrs, numels, hp_dtypes, n);
+  if (rc == F8B200_OK) rc = check_apart(ptrs, numels, hp_dtypes, n);
   if (rc != F8B200_OK) return rc;
   if (reinterpret_cast<uintptr_t>(total_norm) % 4 != 0) return F8B200_ERR_ALIGNMENT;
   rc = f8b200_device_check();

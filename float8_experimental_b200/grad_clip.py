@@ -2,9 +2,10 @@
 (partial sums of every tensor, their sum, the scaling, which the device skips when nothing exceeds the bound) in
 place of several per tensor, and without a host synchronisation.
 
-Gradients of one call lie on one device and do not overlap in memory; bf16, fp16 and fp32 may be mixed.  DTensor gradients (FSDP2, tensor
-parallel) count once over their mesh: the local sums are all-reduced over the mesh dimensions a tensor is
-sharded on.
+Gradients of one call lie on one device; bf16, fp16 and fp32 may be mixed.  Clipping refuses gradients that overlap in
+memory, except for one gradient tensor under several parameters, which counts and is scaled once.  DTensor
+gradients (FSDP2, tensor parallel) count once over their mesh: the local sums are all-reduced over the mesh
+dimensions a tensor is sharded on.
 """
 from __future__ import annotations
 
@@ -87,6 +88,7 @@ def _check_finite(total: torch.Tensor, norm_type: float) -> None:
 def get_total_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: float = 2.0,
                    error_if_nonfinite: bool = False) -> torch.Tensor:
     """The `norm_type` (1, 2 or inf) norm of all `tensors` together, fp32, 0-dim, on their device.  No tensors: 0.
+    A tensor that is listed twice counts twice (the functions that take parameters count each gradient once).
 
     Squares are formed in fp32 as in torch: an element beyond 1.8e19 makes the 2-norm infinite."""
     kind = _kind_of(norm_type)

@@ -479,7 +479,7 @@ int f8b200_layer_norm_bwd(const void* x, const void* grad_y, int hp_dtype, int64
  *                    with root == 0 the sum of powers itself (kind 2).  `workspace`: at least
  *                    f8b200_multi_norm_workspace_bytes(numels, n) bytes, 8-byte aligned.  Sums run in a fixed order.
  * f8b200_multi_clip  x = RN(x * f), f = min(1, max_norm / (total_norm[0] + 1e-6)), in place; nothing is touched when
- *                    f == 1.  The tensors must not overlap.
+ *                    f == 1.  Tensors that overlap are refused (F8B200_ERR_BAD_ARG).
  */
 int64_t f8b200_multi_norm_workspace_bytes(const int64_t* numels, int n);
 int f8b200_multi_norm(const void* const* ptrs, const int64_t* numels, const int* hp_dtypes, int n,
