@@ -36,6 +36,7 @@ from __future__ import annotations
 from typing import List, Optional, Tuple
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _native as N
 
@@ -520,12 +521,13 @@ def _multi_norm_cuda(xs: List[torch.Tensor], kind: int, root: bool):
 
 
 def _multi_clip_cuda(xs: List[torch.Tensor], total_norm, max_norm: float) -> None:
-    xs = TensorList("multi_clip_", xs)
-    if xs.device not in (None, total_norm.device):
-        raise RuntimeError(f"multi_clip_: tensors on different devices ({xs.device} and {total_norm.device})")
+    tensors = TensorList("multi_clip_", xs)
+    if tensors.device not in (None, total_norm.device):
+        raise RuntimeError(f"multi_clip_: tensors on different devices ({tensors.device} and {total_norm.device})")
     if total_norm.numel() != 1 or total_norm.dtype != torch.float32:
         raise RuntimeError("multi_clip_: total_norm must be one float32 value")
-    N.multi_clip(xs, total_norm, max_norm)
+    N.multi_clip(tensors, total_norm, max_norm)
+    increment_version(xs)  # a kernel's writes leave the versions that autograd compares alone
 
 
 _lib.impl("cast_blockwise", _cast_blockwise_cuda, "CUDA")

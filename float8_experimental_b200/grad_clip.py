@@ -14,6 +14,7 @@ from typing import Dict, Iterable, List, Union
 
 import torch
 import torch.distributed as dist
+from torch.autograd.graph import increment_version
 from torch.distributed._tensor import DTensor
 
 from . import _native as N
@@ -76,6 +77,13 @@ def _total_norm(tensors: List[torch.Tensor], kind: int) -> torch.Tensor:
     return both.max() if kind == 0 else both.sum().sqrt() if kind == 2 else both.sum()
 
 
+def _scale(grads: List[torch.Tensor], total: torch.Tensor, max_norm: float) -> None:
+    ops.multi_clip_([_local(g) for g in grads], total, float(max_norm))
+    wrappers = [g for g in grads if isinstance(g, DTensor)]
+    if wrappers:  # the operator has seen to the versions of what it was given
+        increment_version(wrappers)
+
+
 def _check_finite(total: torch.Tensor, norm_type: float) -> None:
     if not bool(torch.isfinite(total)):
         raise RuntimeError(
@@ -102,9 +110,9 @@ def get_total_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], norm_ty
 def clip_grads_with_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float,
                           total_norm: torch.Tensor) -> None:
     """Multiplies every gradient by min(1, max_norm / (total_norm + 1e-6)), in place.  A NaN norm makes them NaN."""
-    grads = [_local(g) for g in _gradients(parameters)]
+    grads = _gradients(parameters)
     if grads:
-        ops.multi_clip_(grads, total_norm, float(max_norm))
+        _scale(grads, total_norm, max_norm)
 
 
 @torch.no_grad()
@@ -122,11 +130,11 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
         if error_if_nonfinite:
             _check_finite(total, norm_type)
         N.multi_clip(tensors, total, float(max_norm))
+        increment_version(grads)  # a backward pass that still needs one of them must not take the scaled values for it
         return total
     total = _total_norm(grads, kind)
     if error_if_nonfinite:
         _check_finite(total, norm_type)
-    local = [_local(g) for g in grads]
-    if local:
-        ops.multi_clip_(local, total, float(max_norm))
+    if grads:
+        _scale(grads, total, max_norm)
     return total

@@ -1,4 +1,4 @@
-"""Clipping of gradients that share memory."""
+"""Clipping of gradients that share memory, and of gradients that a later backward pass needs."""
 import pytest
 import torch
 
@@ -40,3 +40,34 @@ def test_views_that_lie_apart_are_scaled():
     want = torch.ones(300, device="cuda")
     want[:128] = want[200:] = 1.0 / 228 ** 0.5
     assert torch.allclose(buf, want, rtol=1e-5)
+
+
+CLIPS = {"clip_grad_norm_": lambda p, total: clip_grad_norm_([p], 0.1),
+         "clip_grads_with_norm_": lambda p, total: clip_grads_with_norm_([p], 0.1, total),
+         "the operator": lambda p, total: ops.multi_clip_([p.grad], total, 0.1)}
+
+
+@pytest.mark.parametrize("name", CLIPS)
+def test_a_gradient_that_backward_still_needs(name):
+    """As with torch's own clipping, the second backward pass notices that its gradient has changed."""
+    w = torch.nn.Parameter(torch.full((8,), 2.0, device="cuda"))
+    g, = torch.autograd.grad((w ** 3).sum(), [w], create_graph=True)
+    penalty = (g * g).sum()
+    total = get_total_norm([g.detach()])
+    w.grad = g
+    before = g._version
+    with torch.no_grad():
+        CLIPS[name](w, total)
+    assert g._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(penalty, [w])
+
+
+def test_gradients_made_in_inference_mode():
+    with torch.inference_mode():
+        g = torch.full((8,), 2.0, device="cuda")
+        p = torch.nn.Parameter(torch.zeros(8, device="cuda"))
+        p.grad = g
+        clip_grad_norm_([p], 1.0)
+        clip_grads_with_norm_([p], 1.0, torch.ones((), device="cuda"))
+        assert torch.allclose(g, torch.full((8,), 8 ** -0.5, device="cuda"))

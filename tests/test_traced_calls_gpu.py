@@ -149,3 +149,13 @@ def test_compiled(name):
     for x, outs in zip((first, second), want):
         for got, ref in zip(values(compiled(x)), outs):
             assert torch.allclose(got.float(), ref.float(), rtol=2.0 ** -7, atol=1e-3) and got.stride() == ref.stride()
+
+
+def test_compiled_clipping():
+    grads = [torch.full((50,), 3.0, device="cuda"), torch.full((50,), 3.0, device="cuda", dtype=BF)]
+    params = [torch.nn.Parameter(torch.zeros_like(g)) for g in grads]
+    for p, g in zip(params, grads):
+        p.grad = g
+    total = torch.compile(lambda: clip_grad_norm_(params, 3.0), backend="aot_eager")()
+    assert float(total) == 30.0
+    assert all(bool(((g.float() - 0.3).abs() < 1e-2).all()) for g in grads)
