@@ -477,7 +477,19 @@ def _layer_norm_cuda(x, weight, bias, eps: float, save_stats: bool):
 
 def _layer_norm_bwd_cuda(x, grad_y, weight, mean, rstd, affine_dtype, need_dx: bool, need_dw: bool, need_db: bool):
     _one_device("layer_norm_bwd", x, grad_y, weight, mean, rstd)
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise RuntimeError("layer_norm_bwd: the last dimension must have at least one element")
+    if grad_y.shape != x.shape or grad_y.dtype != x.dtype:
+        raise RuntimeError(f"layer_norm_bwd: grad_y must be like x, {x.dtype} {tuple(x.shape)}, got {grad_y.dtype} "
+                           f"{tuple(grad_y.shape)}")
+    if affine_dtype != (x.dtype if weight is None else _affine_dtype(x, weight, None)) and \
+            (weight is not None or affine_dtype != torch.float32):
+        raise RuntimeError(f"layer_norm_bwd: affine_dtype {affine_dtype} is not that of the weight and the bias")
     xm, rows, cols, ld = _as_matrix(x)
+    for name, t in (("mean", mean), ("rstd", rstd)):
+        if t.dtype != torch.float32 or t.shape != (rows,) or not t.is_contiguous():
+            raise RuntimeError(f"layer_norm_bwd: {name} must be {rows} contiguous float32 values, got {t.dtype} "
+                               f"{tuple(t.shape)} with strides {t.stride()}")
     gm, _, _, ldg = _as_matrix(grad_y)
     dx = _empty_like_shape(x, x.dtype) if need_dx else x.new_empty((0,))
     # no rows: nothing to sum
