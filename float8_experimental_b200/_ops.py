@@ -366,7 +366,12 @@ def _cast_blockwise_square_cuda(x, fp8_kind: int):
 
 def _uncast_blockwise_cuda(q, scale_inv, block_rows: int, block_cols: int, dtype):
     _one_device("uncast_blockwise", q, scale_inv)
+    if q.dim() != 2 or block_rows not in (1, 128) or block_cols not in (1, 128):
+        raise RuntimeError("uncast_blockwise: takes a matrix in blocks of 1 or 128 each way")
     rows, cols = q.shape
+    want = (_blocks(rows) if block_rows == 128 else rows, _blocks(cols) if block_cols == 128 else cols)
+    if scale_inv.dtype != torch.float32 or scale_inv.shape != want:
+        raise RuntimeError(f"uncast_blockwise: scale_inv must be float32 {want}, got {scale_inv.dtype} {tuple(scale_inv.shape)}")
     if rows != 1 and cols != 1 and q.stride(0) == 1:  # a transposed matrix: read it as it lies
         return _uncast_blockwise_cuda(q.t(), scale_inv.t(), block_cols, block_rows, dtype).t()
     if q.stride(1) != 1 or q.stride(0) < cols:

@@ -54,3 +54,30 @@ def test_layer_norm_backward_refuses_what_does_not(launches, changes, match):
     with pytest.raises(RuntimeError, match=match):
         backward(**changes)
     assert not launches
+
+
+Q = torch.zeros(130, 300).to(torch.float8_e4m3fn)
+
+
+def test_uncast_takes_what_fits(launches):
+    for scale, block in ((torch.ones(130, 3), (1, 128)), (torch.ones(2, 300), (128, 1)), (torch.ones(2, 3), (128, 128)),
+                         (torch.ones(1, 1).expand(2, 3), (128, 128)), (torch.ones(3, 130).t(), (1, 128))):
+        assert _ops._uncast_blockwise_cuda(Q, scale, *block, BF).shape == (130, 300)
+        assert _ops._uncast_blockwise_cuda(Q.t(), scale.t(), *block[::-1], BF).shape == (300, 130)
+    assert len(launches) == 10
+
+
+@pytest.mark.parametrize("scale,block,match", [
+    (torch.ones(130, 2), (1, 128), "scale_inv must be"), (torch.ones(129, 3), (1, 128), "scale_inv must be"),
+    (torch.ones(2, 3), (1, 128), "scale_inv must be"), (torch.ones(130, 3), (128, 128), "scale_inv must be"),
+    (torch.ones(6), (128, 128), "scale_inv must be"), (torch.ones(2, 3).half(), (128, 128), "scale_inv must be"),
+    (torch.ones(3, 5), (64, 64), "blocks of 1 or 128"),
+])
+def test_uncast_refuses_what_does_not(launches, scale, block, match):
+    with pytest.raises(RuntimeError, match=match):
+        _ops._uncast_blockwise_cuda(Q, scale, *block, BF)
+    with pytest.raises(RuntimeError, match=match):
+        _ops._uncast_blockwise_cuda(Q.t(), scale.t(), *block[::-1], BF)
+    with pytest.raises(RuntimeError, match="takes a matrix"):
+        _ops._uncast_blockwise_cuda(Q[0], scale, *block, BF)
+    assert not launches
