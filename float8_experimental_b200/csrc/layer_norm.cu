@@ -3,8 +3,10 @@
 //   y  = n * w + b
 //   dx = rstd * (h - sum(h) / C - n * sum(h * n) / C),  h = g * w
 //   dw = sum over rows of g * n,   db = sum over rows of g
-// All in fp32 whatever the type of x; y, dx, dw and db are rounded once.  The variance is the second moment about the
-// mean that was just found, not a difference of two large sums, so a large mean costs no digits.
+// All in fp32 whatever the type of x; y, dx, dw and db are rounded once.  The first mean m is off by about |mean| * 2^-24
+// (its sum, and 1 / C, are rounded), which is much where the mean is large against the spread, so the second pass adds up
+// what it leaves:  d = x - m,  r = sum(d) / C,  var = sum(d^2) / C - r^2,  n = d * rstd - r * rstd.  The forward's n then costs
+// no digits to a large mean; the backward takes the mean m + r as it was stored, rounded to fp32.
 // w and b have x's type or fp32; either may be absent (1 and 0).  Sums run in a fixed order.
 //
 // Memory bounds both directions: x read and y written (4 bytes per 16-bit element), x and g read and dx written (6).
@@ -116,17 +118,67 @@ __device__ __forceinline__ float row_sum(float v, float* smem) {
   return v;
 }
 
+// The same of two values at once, behind one barrier.
+template <int ROWT>
+__device__ __forceinline__ float2 row_sum2(float a, float b, float2* smem) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    a += __shfl_xor_sync(0xFFFFFFFFu, a, off);
+    b += __shfl_xor_sync(0xFFFFFFFFu, b, off);
+  }
+  if constexpr (ROWT > 32) {
+    constexpr int W = ROWT / 32;
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, group = threadIdx.x / ROWT;
+    if (lane == 0) smem[w] = make_float2(a, b);
+    if constexpr (ROWT == kThreads) __syncthreads();
+    else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(ROWT) : "memory");
+    a = b = 0.f;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const float2 v = smem[group * W + i];
+      a += v.x;
+      b += v.y;
+    }
+  }
+  return make_float2(a, b);
+}
+
+// two fp32 operations in one instruction
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{.reg .b64 x, y, z;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{.reg .b64 w, x, y, z;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 w, {%6, %7};\n\tfma.rn.f32x2 z, x, y, w;\n\tmov.b64 {%0, %1}, z;}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+
+// r and rstd from the sums of d and d^2 (a rounding below zero is none; a NaN stays)
+__device__ __forceinline__ float2 residual_and_rstd(float2 sums, float inv_c, float eps) {
+  const float r = sums.x * inv_c, var = fmaf(-r, r, sums.y * inv_c);
+  return make_float2(r, 1.0f / sqrtf((var < 0.f ? 0.f : var) + eps));
+}
+
 // ---- forward, a row in registers --------------------------------------------------------------------
 // As few threads per row as hold it in four 16-byte pieces each: several rows per CTA then wait for their sums at
 // different times (16384 x 4096 bf16 with 128 threads per row 53 us, with 256 66 us; 32768 x 2048 with 64 53 us, with 256
-// 76 us, with one warp and eight pieces 59 us).
+// 76 us, with one warp and eight pieces 59 us).  Arithmetic in pairs keeps the second sum of the second pass free
+// (16384 x 8192: 100 us with and without it, 106 element by element); groups of less than a CTA need four CTAs per SM
+// (53 us against 59 with three).
 template <typename T, typename W, int ROWT, int CH>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, ROWT < kThreads && CH > 1 ? 4 : 0)
 ln_fwd_kernel(const T* __restrict__ x, int64_t ld_x, int64_t rows, int64_t cols, const W* __restrict__ weight,
               const W* __restrict__ bias, float eps, T* __restrict__ y, int64_t ld_y, float* __restrict__ mean_out,
               float* __restrict__ rstd_out) {
   constexpr int N = Vec<T>::N, RPB = kThreads / ROWT;
-  __shared__ float smem[2][kThreads / 32];
+  __shared__ float smem[kThreads / 32];
+  __shared__ float2 smem2[kThreads / 32];
   const int t = threadIdx.x % ROWT;
   const int chunks = (int)(cols / N);
   const float inv_c = 1.0f / (float)cols;
@@ -143,20 +195,25 @@ ln_fwd_kernel(const T* __restrict__ x, int64_t ld_x, int64_t rows, int64_t cols,
 #pragma unroll
       for (int j = 0; j < N; ++j) s += v[j];
     }
-    const float mean = row_sum<ROWT>(s, smem[0]) * inv_c;
-    s = 0.f;
+    const float first = row_sum<ROWT>(s, smem) * inv_c;
+    float2 s2 = make_float2(0.f, 0.f), d2 = s2;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       if (t + i * ROWT < chunks) {
         float v[N];
         Vec<T>::widen(q[i], v);
 #pragma unroll
-        for (int j = 0; j < N; ++j) s = fmaf(v[j] - mean, v[j] - mean, s);
+        for (int j = 0; j < N; j += 2) {
+          const float2 d = add2(make_float2(v[j], v[j + 1]), make_float2(-first, -first));
+          d2 = add2(d2, d);
+          s2 = fma2(d, d, s2);
+        }
       }
     }
-    const float rstd = 1.0f / sqrtf(row_sum<ROWT>(s, smem[1]) * inv_c + eps);
+    const float2 rest = residual_and_rstd(row_sum2<ROWT>(d2.x + d2.y, s2.x + s2.y, smem2), inv_c, eps);
+    const float rstd = rest.y, shift = -rest.x * rstd;
     if (t == 0 && mean_out != nullptr) {
-      mean_out[r] = mean;
+      mean_out[r] = first + rest.x;
       rstd_out[r] = rstd;
     }
     uint4* out = reinterpret_cast<uint4*>(y + r * ld_y);
@@ -169,7 +226,12 @@ ln_fwd_kernel(const T* __restrict__ x, int64_t ld_x, int64_t rows, int64_t cols,
         load_affine<W, N>(weight, (int64_t)c * N, 1.f, w);
         load_affine<W, N>(bias, (int64_t)c * N, 0.f, b);
 #pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = fmaf((v[j] - mean) * rstd, w[j], b[j]);
+        for (int j = 0; j < N; j += 2) {
+          const float2 d = add2(make_float2(v[j], v[j + 1]), make_float2(-first, -first));
+          const float2 n = fma2(d, make_float2(rstd, rstd), make_float2(shift, shift));
+          const float2 r2 = fma2(n, make_float2(w[j], w[j + 1]), make_float2(b[j], b[j + 1]));
+          v[j] = r2.x, v[j + 1] = r2.y;
+        }
         __stcs(out + c, Vec<T>::narrow(v));
       }
     }
@@ -382,7 +444,8 @@ __global__ void __launch_bounds__(kThreads)
 ln_fwd_any_kernel(const T* __restrict__ x, int64_t ld_x, int64_t rows, int64_t cols, const W* __restrict__ weight,
                   const W* __restrict__ bias, float eps, T* __restrict__ y, int64_t ld_y, float* __restrict__ mean_out,
                   float* __restrict__ rstd_out) {
-  __shared__ float smem[2][kThreads / 32];
+  __shared__ float smem[kThreads / 32];
+  __shared__ float2 smem2[kThreads / 32];
   const float inv_c = 1.0f / (float)cols;
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* row = x + r * ld_x;
@@ -408,17 +471,22 @@ ln_fwd_any_kernel(const T* __restrict__ x, int64_t ld_x, int64_t rows, int64_t c
     }
     float s = 0.f;
     each([&](int64_t, float a) { s += a; });
-    const float mean = row_sum<kThreads>(s, smem[0]) * inv_c;
+    const float first = row_sum<kThreads>(s, smem) * inv_c;
     s = 0.f;
-    each([&](int64_t, float a) { s = fmaf(a - mean, a - mean, s); });
-    const float rstd = 1.0f / sqrtf(row_sum<kThreads>(s, smem[1]) * inv_c + eps);
+    float d = 0.f;
+    each([&](int64_t, float a) {
+      d += a - first;
+      s = fmaf(a - first, a - first, s);
+    });
+    const float2 rest = residual_and_rstd(row_sum2<kThreads>(d, s, smem2), inv_c, eps);
+    const float rstd = rest.y, shift = -rest.x * rstd;
     if (threadIdx.x == 0 && mean_out != nullptr) {
-      mean_out[r] = mean;
+      mean_out[r] = first + rest.x;
       rstd_out[r] = rstd;
     }
     each([&](int64_t c, float a) {
       const float w = weight != nullptr ? to_f32(weight[c]) : 1.f, b = bias != nullptr ? to_f32(bias[c]) : 0.f;
-      y[r * ld_y + c] = from_f32<T>(fmaf((a - mean) * rstd, w, b));
+      y[r * ld_y + c] = from_f32<T>(fmaf(fmaf(a - first, rstd, shift), w, b));
     });
   }
 }

@@ -453,7 +453,7 @@ int f8b200_gemm_blockwise(const void* a, int a_kind, int a_layout, int64_t lda, 
 /*
  * Layer norm over the columns of x [rows, cols], T = hp_dtype:
  *   n = (x - mean) * rstd,  rstd = 1 / sqrt(mean of (x - mean)^2 + eps),  y = RN_T(n * weight + bias)
- * in fp32.  weight and bias [cols] have affine_dtype (hp_dtype or FP32); either may be NULL (1 and 0).
+ * in fp32 (n as if the mean had no rounding).  weight and bias [cols] have affine_dtype (hp_dtype or FP32); either may be NULL (1 and 0).
  * mean_out and rstd_out [rows] are both given or both NULL.
  *
  * f8b200_layer_norm_bwd  from x, grad_y and the saved mean and rstd, with h = grad_y * weight:
