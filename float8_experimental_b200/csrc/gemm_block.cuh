@@ -1114,6 +1114,7 @@ extern "C" int f8b200_gemm_blockwise(const void* a, int a_kind, int a_layout, in
   if (!strides_ok(sa) || !strides_ok(sb)) return F8B200_ERR_BAD_ARG;
   if (workspace != nullptr && workspace_bytes < F8B200_GEMM_WORKSPACE_BYTES) return F8B200_ERR_BAD_ARG;
   if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return F8B200_ERR_ALIGNMENT;
+  if (reinterpret_cast<uintptr_t>(scale_a) % 4 != 0 || reinterpret_cast<uintptr_t>(scale_b) % 4 != 0) return F8B200_ERR_ALIGNMENT;
   bool empty = false;
   int rc = gemm_fp8_validate(a, a_kind, a_layout, lda, b, b_kind, b_layout, ldb, scale_a, scale_b, bias, out_dtype, out,
                              ldo, m, n, k, &empty);

@@ -721,7 +721,8 @@ extern "C" int f8b200_layer_norm(const void* x, int hp_dtype, int64_t rows, int6
   if ((mean_out == nullptr) != (rstd_out == nullptr)) return F8B200_ERR_BAD_ARG;
   if (rows == 0) return F8B200_OK;
   if (x == nullptr || y == nullptr || ld_x < cols || ld_y < cols) return F8B200_ERR_BAD_ARG;
-  if (!ln_aligned(x, hp_dtype) || !ln_aligned(y, hp_dtype) || !ln_aligned(weight, affine_dtype) || !ln_aligned(bias, affine_dtype))
+  if (!ln_aligned(x, hp_dtype) || !ln_aligned(y, hp_dtype) || !ln_aligned(weight, affine_dtype) || !ln_aligned(bias, affine_dtype) ||
+      !ln_aligned(mean_out, F8B200_FP32) || !ln_aligned(rstd_out, F8B200_FP32))
     return F8B200_ERR_ALIGNMENT;
   const int rc = f8b200_device_check();
   if (rc != F8B200_OK) return rc;
@@ -745,7 +746,7 @@ extern "C" int f8b200_layer_norm_bwd(const void* x, const void* grad_y, int hp_d
   const bool sums = dweight != nullptr || dbias != nullptr;
   if (sums && (workspace == nullptr || workspace_bytes < f8b200_layer_norm_bwd_workspace_bytes(cols))) return F8B200_ERR_BAD_ARG;
   if (!ln_aligned(x, hp_dtype) || !ln_aligned(grad_y, hp_dtype) || !ln_aligned(dx, hp_dtype) ||
-      !ln_aligned(weight, affine_dtype) || !ln_aligned(dweight, affine_dtype) || !ln_aligned(dbias, affine_dtype) ||
+      !ln_aligned(mean, F8B200_FP32) || !ln_aligned(rstd, F8B200_FP32) || !ln_aligned(weight, affine_dtype) || !ln_aligned(dweight, affine_dtype) || !ln_aligned(dbias, affine_dtype) ||
       reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
     return F8B200_ERR_ALIGNMENT;
   const int rc = f8b200_device_check();
