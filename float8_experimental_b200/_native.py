@@ -227,7 +227,8 @@ class _Launch:
     def __init__(self, kind: str, device: torch.device, n: int = 1):
         self.kind, self.n, self.start = kind, n, None
         idx = device.index
-        self.guard = None if (idx is None or idx == torch.cuda.current_device()) else torch.cuda.device(idx)
+        # the tensor at hand has initialised CUDA, which torch.cuda.current_device would see to first
+        self.guard = None if (idx is None or idx == torch._C._cuda_getDevice()) else torch.cuda.device(idx)
 
     def __enter__(self):
         global _launches

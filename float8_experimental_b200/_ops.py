@@ -364,14 +364,17 @@ def _cast_blockwise_square_cuda(x, fp8_kind: int):
     return data, scale, exps, exps_t
 
 
+_BLOCK_SIZES = (1, 128)
+
+
 def _uncast_blockwise_cuda(q, scale_inv, block_rows: int, block_cols: int, dtype):
-    _one_device("uncast_blockwise", q, scale_inv)
-    if q.dim() != 2 or block_rows not in (1, 128) or block_cols not in (1, 128):
+    if q.dim() != 2 or block_rows not in _BLOCK_SIZES or block_cols not in _BLOCK_SIZES:
         raise RuntimeError("uncast_blockwise: takes a matrix in blocks of 1 or 128 each way")
     rows, cols = q.shape
-    want = (_blocks(rows) if block_rows == 128 else rows, _blocks(cols) if block_cols == 128 else cols)
-    if scale_inv.dtype != torch.float32 or scale_inv.shape != want:
+    want = (-(-rows // block_rows), -(-cols // block_cols))
+    if scale_inv.dtype is not torch.float32 or scale_inv.shape != want:
         raise RuntimeError(f"uncast_blockwise: scale_inv must be float32 {want}, got {scale_inv.dtype} {tuple(scale_inv.shape)}")
+    _one_device("uncast_blockwise", q, scale_inv)
     if rows != 1 and cols != 1 and q.stride(0) == 1:  # a transposed matrix: read it as it lies
         return _uncast_blockwise_cuda(q.t(), scale_inv.t(), block_cols, block_rows, dtype).t()
     if q.stride(1) != 1 or q.stride(0) < cols:
@@ -480,21 +483,31 @@ def _layer_norm_cuda(x, weight, bias, eps: float, save_stats: bool):
     return y, mean, rstd
 
 
-def _layer_norm_bwd_cuda(x, grad_y, weight, mean, rstd, affine_dtype, need_dx: bool, need_dw: bool, need_db: bool):
-    _one_device("layer_norm_bwd", x, grad_y, weight, mean, rstd)
+def _refuse_layer_norm_bwd(x, grad_y, weight, mean, rstd, affine_dtype, rows: int):
+    """Says what of the arguments does not fit."""
     if x.dim() == 0 or x.shape[-1] == 0:
         raise RuntimeError("layer_norm_bwd: the last dimension must have at least one element")
     if grad_y.shape != x.shape or grad_y.dtype != x.dtype:
         raise RuntimeError(f"layer_norm_bwd: grad_y must be like x, {x.dtype} {tuple(x.shape)}, got {grad_y.dtype} "
                            f"{tuple(grad_y.shape)}")
-    if affine_dtype != (x.dtype if weight is None else _affine_dtype(x, weight, None)) and \
-            (weight is not None or affine_dtype != torch.float32):
-        raise RuntimeError(f"layer_norm_bwd: affine_dtype {affine_dtype} is not that of the weight and the bias")
-    xm, rows, cols, ld = _as_matrix(x)
     for name, t in (("mean", mean), ("rstd", rstd)):
         if t.dtype != torch.float32 or t.shape != (rows,) or not t.is_contiguous():
             raise RuntimeError(f"layer_norm_bwd: {name} must be {rows} contiguous float32 values, got {t.dtype} "
                                f"{tuple(t.shape)} with strides {t.stride()}")
+    _affine_dtype(x, weight, None)
+    raise RuntimeError(f"layer_norm_bwd: affine_dtype {affine_dtype} is not that of the weight and the bias")
+
+
+def _layer_norm_bwd_cuda(x, grad_y, weight, mean, rstd, affine_dtype, need_dx: bool, need_dw: bool, need_db: bool):
+    _one_device("layer_norm_bwd", x, grad_y, weight, mean, rstd)
+    xm, rows, cols, ld = _as_matrix(x)
+    f32, dtype, stats = torch.float32, x.dtype, (rows,)
+    fits = (cols > 0 and x.dim() > 0 and grad_y.shape == x.shape and grad_y.dtype is dtype and mean.shape == stats and rstd.shape == stats
+            and mean.dtype is f32 and rstd.dtype is f32 and mean.is_contiguous() and rstd.is_contiguous()
+            and (affine_dtype is dtype or affine_dtype is f32)
+            and (weight is None or (weight.dtype is affine_dtype and weight.shape == (cols,))))
+    if not fits:
+        _refuse_layer_norm_bwd(x, grad_y, weight, mean, rstd, affine_dtype, rows)
     gm, _, _, ldg = _as_matrix(grad_y)
     dx = _empty_like_shape(x, x.dtype) if need_dx else x.new_empty((0,))
     # no rows: nothing to sum
@@ -576,8 +589,9 @@ _lib.impl("scaled_mm", _scaled_mm_cuda, "CUDA")
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
 
 
+_is_compiling = torch.compiler.is_compiling
 _dispatch_modes = torch._C._len_torch_dispatch_stack
-_pre_dispatch_modes = torch._ops._len_torch_dispatch_stack_pre_dispatch
+_pre_dispatch_modes = torch._ops.mode_stack_state_for_pre_dispatch().count
 _jit_tracing = torch._C._is_tracing
 _functorch_level = torch._C._functorch.peek_interpreter_stack
 
@@ -589,10 +603,11 @@ def nothing_watches() -> bool:
 
 
 def eager_cuda(t: torch.Tensor) -> bool:
-    """Whether an op on `t` would come straight to its CUDA implementation here: a plain CUDA tensor, nothing watching.
+    """Whether an op on `t` would come straight to its CUDA implementation here: a plain CUDA tensor, `nothing_watches`.
     Callers that run without autograd (inside an autograd function, or with nothing to differentiate) then call
     the implementation themselves: a trip through the dispatcher costs more host time than a small launch."""
-    return not torch.compiler.is_compiling() and type(t) in _PLAIN and t.is_cuda and nothing_watches()
+    return (not _is_compiling() and type(t) in _PLAIN and t.is_cuda
+            and not _dispatch_modes() and not _jit_tracing() and _functorch_level() is None and not _pre_dispatch_modes())
 
 
 # ---------------------------------------------------------------------------

@@ -30,16 +30,6 @@ BLOCK = 128
 _BLOCKS = ((1, BLOCK), (BLOCK, 1), (BLOCK, BLOCK))
 
 
-class _Exponents:
-    """The exponent bytes of a cast's factors: of the matrix, and of its transpose, as a product's operand.  Shared by the
-    tensors that hold the same factors."""
-
-    __slots__ = ("matrix", "transpose")
-
-    def __init__(self, matrix: Optional[torch.Tensor], transpose: Optional[torch.Tensor]):
-        self.matrix, self.transpose = matrix, transpose
-
-
 class Float8BlockTensor:
     """A matrix held as fp8 bytes and one factor per block: `data[i, j] * scale_inv[i // block[0], j // block[1]]`.
 
@@ -53,6 +43,7 @@ class Float8BlockTensor:
     trace (a collective, `.data`, another library's kernel), so asking for it drops the bytes, of transposes too: products
     of more than 128 rows then take the factors themselves, in a slower kernel.  `scale_inv` may be assigned."""
 
+    # _exps: [bytes of the matrix, of its transpose], one list for all the tensors that hold the same factors
     __slots__ = ("data", "_scale", "block", "orig_dtype", "_exps", "_transposed")
 
     def __init__(self, data: torch.Tensor, scale_inv: torch.Tensor, block: Tuple[int, int],
@@ -70,13 +61,13 @@ class Float8BlockTensor:
         """What a cast made: nothing to check, and the exponent bytes beside it."""
         out = object.__new__(cls)
         out.data, out._scale, out.block, out.orig_dtype = data, scale_inv, block, orig_dtype
-        out._exps, out._transposed = _Exponents(exps, exps_t), False
+        out._exps, out._transposed = [exps, exps_t], False
         return out
 
     @property
     def scale_inv(self) -> torch.Tensor:
         if self._exps is not None:
-            self._exps.matrix = self._exps.transpose = None
+            self._exps[:] = None, None
         return self._scale
 
     @scale_inv.setter
@@ -95,7 +86,7 @@ class Float8BlockTensor:
         """The exponent bytes, unless the factors may have been written to since the cast."""
         if self._exps is None:
             return None
-        return self._exps.transpose if transposed != self._transposed else self._exps.matrix
+        return self._exps[transposed != self._transposed]
 
     @property
     def shape(self) -> torch.Size:

@@ -39,11 +39,9 @@ def _local(t: torch.Tensor) -> torch.Tensor:
 
 def _gradients(parameters: Union[torch.Tensor, Iterable[torch.Tensor]]) -> List[torch.Tensor]:
     """The gradients of `parameters`, each once however often it or its parameter is listed."""
-    params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
-    if len(set(map(id, params))) != len(params):
-        params = list({id(p): p for p in params}.values())
+    params = [parameters] if isinstance(parameters, torch.Tensor) else parameters
     grads = [g for p in params if (g := p.grad) is not None]
-    if len(set(map(id, grads))) != len(grads):  # parameters that share one gradient tensor
+    if len(set(map(id, grads))) != len(grads):  # a parameter listed twice, or parameters that share one gradient tensor
         grads = list({id(g): g for g in grads}.values())
     return grads
 
