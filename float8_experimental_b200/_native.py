@@ -6,6 +6,7 @@ exception.  Nothing here runs on the CPU.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from array import array
 from typing import Optional, Sequence
@@ -216,6 +217,11 @@ def kernel_event_totals():
     """{kind: (total_ms, launches)} of the launches recorded since reset_counters()."""
     torch.cuda.synchronize()
     return {k: (sum(a.elapsed_time(b) for a, b in v), len(v)) for k, v in _events.items()}
+
+
+@functools.lru_cache(maxsize=None)
+def _sm_pairs(device: int) -> int:
+    return torch.cuda.get_device_properties(device).multi_processor_count // 2
 
 
 class _Launch:
@@ -628,10 +634,11 @@ def gemm_blockwise(a: torch.Tensor, lda: int, a_mn_major: bool, scale_a: torch.T
                    exp_a: Optional[torch.Tensor], b: torch.Tensor, ldb: int, b_mn_major: bool, scale_b: torch.Tensor,
                    b_block_rows: int, exp_b: Optional[torch.Tensor], bias: Optional[torch.Tensor], out: torch.Tensor, ldo: int, m: int, n: int, k: int) -> None:
     _require_cuda(a, b, scale_a, scale_b, exp_a, exp_b, bias, out)
-    # tiles are handed out through a word of memory; it belongs to this launch alone (a word per stream would be shared by
-    # graphs captured on it that are replayed at the same time)
-    ws = torch.empty(GEMM_WORKSPACE_BYTES, dtype=torch.uint8, device=a.device) if exp_a is not None and exp_b is not None \
-        and m * n > 74 * 256 * 256 else None
+    # more 256 x 256 tiles than CTA pairs are handed out through a word of memory; it belongs to this launch alone (a word per
+    # stream would be shared by graphs captured on it that are replayed at the same time)
+    ws = None
+    if exp_a is not None and exp_b is not None and -(-m // 256) * -(-n // 256) > _sm_pairs(a.get_device()):
+        ws = torch.empty(GEMM_WORKSPACE_BYTES, dtype=torch.uint8, device=a.device)
     with _Launch("gemm_block", a.device):
         _check(
             load().f8b200_gemm_blockwise(a.data_ptr(), fp8_code(a.dtype), int(a_mn_major), lda, scale_a.data_ptr(),
