@@ -82,3 +82,18 @@ def test_gradients_with_large_means(cols):
     assert float(((dx.double() - ref).abs() - tol).max()) <= 0
     tol = (24 + 8) * U * (gd * n).abs().sum(0) + (gd.abs() * e_n).sum(0)
     assert float(((dw.double() - (gd * n).sum(0)).abs() - tol).max()) <= 0
+
+
+@pytest.mark.parametrize("cols", WIDTHS)
+@pytest.mark.parametrize("dtype", [BF, FP32])
+def test_squares_that_overflow(cols, dtype):
+    """The variance is infinite, so every value is zero deviations from the mean; other rows are as they are alone."""
+    gen = torch.Generator(device="cuda").manual_seed(cols)
+    x = torch.randn(6, cols, device="cuda", generator=gen).to(dtype)
+    alone = layer_norm(x)
+    x[1] = 1e30
+    x[3] *= 1e25
+    x[4] = x[4] * 1e25 + 1e30
+    y = layer_norm(x)
+    assert bool((y[[1, 3, 4]] == 0).all())
+    assert torch.equal(y[[0, 2, 5]], alone[[0, 2, 5]])
