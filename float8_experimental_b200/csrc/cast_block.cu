@@ -10,7 +10,8 @@
 //
 // One CTA takes a 128 x 128 tile, so every block lies inside one CTA and x is read once for all the forms asked
 // for: 256 threads, 8 columns and 8 rows (16 apart) per thread, held in registers.
-// Memory bounds it: 16384 x 8192 bf16 by rows 64 us (6.3 TB/s), by rows and columns 111 us (4.8 TB/s), back 70 us (5.8).
+// Memory bounds it: 16384 x 8192 bf16 by rows 70 us (5.7 TB/s), by columns 73, by squares 72, by rows and columns 118
+// (4.6 TB/s), back 71 (5.7), 75 from columns; per call of ten in a replayed graph.
 #include "common.cuh"
 
 namespace f8b200 {
@@ -234,7 +235,8 @@ __global__ void __launch_bounds__(kThreads, HP == F8B200_FP32 ? 2 : (FORMS == kB
   }
   if constexpr ((FORMS & (kByRow | kByCol)) != 0) {
     // the tile's factors leave together, neighbours from neighbouring threads: stored by the threads that found them,
-    // one here and one there, they cost as much as the bytes (330 against 148 us for both forms of 16384 x 8192 bf16)
+    // one here and one there, they cost as much as the bytes (this step took both forms of 16384 x 8192 bf16 from 330 to
+    // 148 us, packed maxima from there to 118)
     __syncthreads();
     const int t = threadIdx.x & 127;
     if (threadIdx.x < 128) {

@@ -7,10 +7,12 @@
 // own: every block's MMAs start a fresh tensor-memory accumulator, and the epilogue warps add it, multiplied by
 // its scale, to fp32 sums that stay in registers for the whole tile.  Per block that costs a 128x256 tile's
 // CTA 32768 fp32 FMAs (256 cycles of its FMA pipes) and as many tensor-memory words against the 512 cycles of the
-// MMAs, and it runs beside them: two accumulators alternate.  16384 x 8192 x 8192: 1.07 ms, 2.06 PFLOP/s; with a factor
-// per row on both sides one more multiplication per element, 2.07 ms.
+// MMAs, and two accumulators alternate so that it can run beside them.  It does not quite: 16384 x 8192 x 8192 takes
+// 1.11 ms (1.98 PFLOP/s), and at 4096 x 4096 x 8192 the tensor pipe is active 38 % of the time, the FMA pipe 19 %, so each
+// waits for the other's hand-over.  With a factor per row on both sides there is one more multiplication per
+// element and a shared-memory read per pair (that pipe 50 % busy, the tensor pipe 22 %): 2.11 ms.
 //
-// Two kernels:
+// Factors that are powers of two go to a third kernel, below, which leaves them to the tensor cores.  Two kernels here:
 //   block pair kernel   two CTAs per 256x256 tile, tcgen05.mma.cta_group::2 as in the pair kernel of gemm.cu;
 //                       eight epilogue warps per CTA, one row and 128 columns per thread.
 //   few-rows kernel     A has few rows (tokens being served): B's rows take the 128-wide side of the MMA and A's
@@ -1088,8 +1090,9 @@ static uint32_t make_idesc_few(int w_kind, int x_kind, int w_mn, int cols) {
 }
 
 // CTAs of one cluster that split K: as many as the GPU holds at once and leave each at least four k-blocks, in powers of
-// two up to 8.  Measured (us, split 1 / 2 / 4 / 8): 8 x 8192 x 8192 33 / 25 / 25 / 29, 64 x 8192 x 28672 170 / 98 / 68 /
-// 76, 128 x 4096 x 4096 27 / 21 / 17 / 31, 37 x 28672 x 8192 72 / 80 / 82 / 94.
+// two up to 8.  Measured (us, single calls in a graph with cold caches, split 1 / 2 / 4 / 8): 8 x 8192 x 8192 35 / 27 / 25 / 29,
+// 16 x 2048 x 8192 35 / 23 / 16 / 16, 64 x 8192 x 28672 121 / 72 / 61 / 68, 128 x 4096 x 4096 33 / 25 / 21 / 35, 128 x 8192 x
+// 8192 55 / 37 / 43 / 68, 37 x 28672 x 8192 61 / 68 / 76 / 88.
 static int few_split(int64_t tiles, int num_kb, int ctas_per_sm) {
   int split = 1;
   while (split < FEW_MAX_SPLIT && tiles * split * 2 <= (int64_t)ctas_per_sm * sm_count() && num_kb >= split * 2 * 4) split *= 2;

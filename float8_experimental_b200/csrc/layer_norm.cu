@@ -10,7 +10,7 @@
 // w and b have x's type or fp32; either may be absent (1 and 0).  Sums run in a fixed order.
 //
 // Memory bounds both directions: x read and y written (4 bytes per 16-bit element), x and g read and dx written (6).
-// 16384 x 8192 bf16: forward 95 us, 5.7 TB/s in the kernel; backward 155 us, 5.2 TB/s.
+// 16384 x 8192 bf16, per call of ten in a replayed graph: forward 93 us, 5.8 TB/s; backward 155 us, 5.2 TB/s.
 #include <type_traits>
 
 #include "common.cuh"
@@ -169,8 +169,8 @@ __device__ __forceinline__ float2 residual_and_rstd(float2 sums, float inv_c, fl
 // As few threads per row as hold it in four 16-byte pieces each: several rows per CTA then wait for their sums at
 // different times (16384 x 4096 bf16 with 128 threads per row 53 us, with 256 66 us; 32768 x 2048 with 64 53 us, with 256
 // 76 us, with one warp and eight pieces 59 us).  Arithmetic in pairs keeps the second sum of the second pass free
-// (16384 x 8192: 100 us with and without it, 106 element by element); groups of less than a CTA need four CTAs per SM
-// (53 us against 59 with three).
+// (16384 x 8192, single calls with cold caches as above: 102 us with it, 100 without, 106 element by element); groups of
+// less than a CTA need four CTAs per SM (53 us against 59 with three).
 template <typename T, typename W, int ROWT, int CH>
 __global__ void __launch_bounds__(kThreads, ROWT < kThreads && CH > 1 ? 4 : 0)
 ln_fwd_kernel(const T* __restrict__ x, int64_t ld_x, int64_t rows, int64_t cols, const W* __restrict__ weight,
