@@ -502,8 +502,8 @@ def _layer_norm_bwd_cuda(x, grad_y, weight, mean, rstd, affine_dtype, need_dx: b
     _one_device("layer_norm_bwd", x, grad_y, weight, mean, rstd)
     xm, rows, cols, ld = _as_matrix(x)
     f32, dtype, stats = torch.float32, x.dtype, (rows,)
-    fits = (cols > 0 and x.dim() > 0 and grad_y.shape == x.shape and grad_y.dtype is dtype and mean.shape == stats and rstd.shape == stats
-            and mean.dtype is f32 and rstd.dtype is f32 and mean.is_contiguous() and rstd.is_contiguous()
+    fits = (cols > 0 and x.dim() > 0 and grad_y.shape == x.shape and grad_y.dtype is dtype
+            and mean.shape == stats and rstd.shape == stats and mean.dtype is f32 and rstd.dtype is f32 and mean.is_contiguous() and rstd.is_contiguous()
             and (affine_dtype is dtype or affine_dtype is f32)
             and (weight is None or (weight.dtype is affine_dtype and weight.shape == (cols,))))
     if not fits:
@@ -606,6 +606,7 @@ def eager_cuda(t: torch.Tensor) -> bool:
     """Whether an op on `t` would come straight to its CUDA implementation here: a plain CUDA tensor, `nothing_watches`.
     Callers that run without autograd (inside an autograd function, or with nothing to differentiate) then call
     the implementation themselves: a trip through the dispatcher costs more host time than a small launch."""
+    # its checks spelt out: one more Python call costs as much as two of them
     return (not _is_compiling() and type(t) in _PLAIN and t.is_cuda
             and not _dispatch_modes() and not _jit_tracing() and _functorch_level() is None and not _pre_dispatch_modes())
 
@@ -743,7 +744,7 @@ def _blockwise_mm_fake(a, b_t, scale_a, scale_b, a_block_rows, b_block_rows, exp
 
 @torch.library.register_fake("f8b200::layer_norm")
 def _layer_norm_fake(x, weight, bias, eps, save_stats):
-    rows = x.numel() // x.shape[-1] if save_stats else 0
+    rows = x.numel() // max(x.shape[-1], 1) if save_stats else 0
     return x.new_empty(x.shape), x.new_empty((rows,), dtype=torch.float32), x.new_empty((rows,), dtype=torch.float32)
 
 

@@ -434,7 +434,8 @@ int f8b200_uncast_blockwise(const void* q, int fp8_kind, int64_t rows, int64_t c
 
 /*
  * out[m, n] = sum_j sa(m, j) * sb(n, j) * (sum of A[m, k] * B[n, k] over k in block j)  (+ bias[n])
- * with blocks of 128 along K, fp32 sums, one rounding to out_dtype.  Operands, layouts, pitches and alignment as in
+ * with blocks of 128 along K, fp32 sums, one rounding to out_dtype.  A sum inside the tensor cores, whose steps are cut off
+ * towards zero, runs over one block, or with exponent bytes over at most 4096 k (out_dtype FP32: 2048).  Operands, layouts, pitches and alignment as in
  * f8b200_gemm_fp8_ws; K may be any number, the last block being shorter.  The factor of A's row m and block j lies
  * at scale_a[(m / a_block_rows) * sa_row_stride + j * sa_kb_stride], a_block_rows 1 or 128, strides >= 0
  * (elements); B's likewise.  Factors are arbitrary fp32 values.  exp_a and exp_b (each may be NULL) are the exponent
